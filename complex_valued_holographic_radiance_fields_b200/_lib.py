@@ -13,6 +13,7 @@ _lock = threading.Lock()
 _lib = None
 
 c_int, c_float, c_size_t, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_longlong = ctypes.c_longlong
 c_float_p = ctypes.POINTER(ctypes.c_float)
 
 # name -> (restype, argtypes); must match include/cvhrf.h
@@ -95,6 +96,21 @@ SIGNATURES = {
     "cvhrf_density_classify": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cvhrf_density_apply": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cvhrf_opacity_regularization": (c_int, [c_void_p, c_int, c_float, c_void_p, c_void_p]),
+    "cvhrf_table_lookup": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_int, c_longlong,
+                                   c_float, c_void_p, c_void_p]),
+    "cvhrf_table_gradient_workspace_bytes": (c_size_t, [c_longlong, c_longlong, c_int]),
+    "cvhrf_table_gradient": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_longlong, c_float,
+                                     c_void_p, c_longlong, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cvhrf_group_rows_workspace_bytes": (c_size_t, [c_longlong, c_int]),
+    "cvhrf_group_rows": (c_int, [c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_size_t, c_void_p]),
+    "cvhrf_rows_to_groups": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
+                                     c_void_p, c_void_p]),
+    "cvhrf_groups_to_rows": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
+                                     c_int, c_void_p, c_void_p]),
+    "cvhrf_groups_to_rows_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_longlong, c_int,
+                                              c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                              c_void_p]),
 }
 
 

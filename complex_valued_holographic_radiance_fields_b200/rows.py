@@ -1,0 +1,270 @@
+"""Rows that many entries share, and rows sorted by an integer group and back.
+
+A Gaussian scene with a codebook keeps one table of attribute rows and an integer per
+Gaussian; training it needs the rows looked up and their gradients summed over the
+Gaussians that share them:
+
+* ``table_lookup(table, index, scale)``: ``scale * table[index]``, differentiable in the table;
+* ``table_gradient(grad, index, num_rows, scale)``: that gradient by itself, with the mask
+  of the rows it touched, as ``SparseGaussianAdam.step(row_mask=...)`` takes it.
+
+Rows that go by group (depth plane, owning GPU, expert), with one or several groups per row:
+
+* ``group_rows(index, num_groups)``: the entries sorted stably by group (a ``RowGroups``);
+* ``rows_to_groups(x, groups)``: each row copied to its places, differentiable;
+* ``groups_to_rows(y, groups, weights)``: the weighted sum of a row's places, differentiable
+  in ``y`` and ``weights``.
+
+An index or group outside its range (-1, say) leaves the entry out: it looks up zeros, adds
+nothing to a gradient or a sum, and whatever its weight or gradient holds is not read.
+Rows are float32, bfloat16 or float16, contiguous within a row (a slice of a wider tensor
+or a row expanded over a batch is used as it is); sums are float32 in a fixed order, so
+results repeat bit for bit, and are rounded once.  Nothing is read back to the host: every
+call can be captured in a CUDA graph.  Every step runs in libcvhrf (cvhrf_table_lookup,
+cvhrf_table_gradient, cvhrf_group_rows, cvhrf_rows_to_groups, cvhrf_groups_to_rows); the
+reference, whose Gaussians own all their attributes, has no counterpart.
+"""
+import torch
+
+from . import _lib
+from .profiling import timed
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
+_MAX_ENTRIES = 2 ** 30 - 1
+_MAX_WIDTH = 2 ** 20
+
+
+def _call(name, device, *args):
+    """One libcvhrf call on `device` and its current stream."""
+    f = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = f(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+
+
+def _rows(t, name):
+    """A 2-D tensor of rows whose elements are adjacent, and the elements between its rows."""
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dim() != 2 or not 1 <= t.shape[1] <= _MAX_WIDTH:
+        raise ValueError(f"{name} must be rows x width with 1 <= width <= {_MAX_WIDTH}, got {tuple(t.shape)}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _index(index, device, name="index"):
+    if index.dtype not in _INDEX_BYTES:
+        raise TypeError(f"{name} must be int32 or int64, got {index.dtype}")
+    if index.device != device:
+        raise ValueError(f"{name} must be on {device}, got {index.device}")
+    if index.numel() > _MAX_ENTRIES:
+        raise ValueError(f"{name} has {index.numel()} entries: {_MAX_ENTRIES} at most")
+    return index.contiguous()
+
+
+def _scale(scale):
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("scale must be a number, not a tensor")
+    return float(scale)
+
+
+# ---- shared rows ----------------------------------------------------------------------
+def _lookup(table, index, scale):
+    table, stride = _rows(table, "table")
+    index = _index(index, table.device)
+    rows, width = table.shape
+    out = torch.empty(*index.shape, width, dtype=table.dtype, device=table.device)
+    with timed("table_lookup"):
+        _call("cvhrf_table_lookup", table.device, table.data_ptr(), rows, width, stride, _TYPES[table.dtype],
+              index.data_ptr(), _INDEX_BYTES[index.dtype], index.numel(), scale, out.data_ptr())
+    return out
+
+
+def _gradient(grad, index, num_rows, scale, with_mask):
+    width = grad.shape[-1]
+    grad, stride = _rows(grad.reshape(-1, width), "grad")
+    device = grad.device
+    index = _index(index, device)
+    n = index.numel()
+    out = torch.empty(num_rows, width, dtype=grad.dtype, device=device)
+    mask = torch.empty(num_rows, dtype=torch.uint8, device=device) if with_mask else None
+    nbytes = _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with timed("table_gradient"):
+        _call("cvhrf_table_gradient", device, grad.data_ptr(), stride, _TYPES[grad.dtype], width, index.data_ptr(),
+              _INDEX_BYTES[index.dtype], n, scale, out.data_ptr(), num_rows, mask.data_ptr() if with_mask else None,
+              ws.data_ptr(), nbytes)
+    return out, mask
+
+
+class TableLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale):
+        ctx.save_for_backward(index)
+        ctx.num_rows, ctx.scale = table.shape[0], scale
+        return _lookup(table, index, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        index, = ctx.saved_tensors
+        return _gradient(grad, index, ctx.num_rows, ctx.scale, False)[0], None, None
+
+
+def table_lookup(table, index, scale=1.0):
+    """scale * table[index] for a table of rows (V, D) and an int32 or int64 index of any
+    shape: (*index.shape, D) in the table's type, zeros where the index is outside [0, V).
+    Differentiable in the table (a dense (V, D) gradient, see ``table_gradient``)."""
+    scale = _scale(scale)
+    if table.requires_grad and torch.is_grad_enabled():
+        return TableLookup.apply(table, index, scale)
+    return _lookup(table, index, scale)
+
+
+@torch.no_grad()
+def table_gradient(grad, index, num_rows, scale=1.0):
+    """The gradient of ``table_lookup`` with respect to its table of `num_rows` rows: row v is
+    scale times the sum of grad[t] over the entries with index[t] = v.  grad has the
+    lookup's shape (*index.shape, D).  Returns (gradient (num_rows, D) in grad's type,
+    row_mask (num_rows,) uint8: 1 where an entry names the row), so that
+    ``SparseGaussianAdam.step(row_mask=row_mask)`` updates the rows that were used."""
+    if grad.dim() < 1 or grad.shape[:-1] != index.shape:
+        raise ValueError(f"grad must have the shape {tuple(index.shape)} and a row's width, got {tuple(grad.shape)}")
+    if not 0 <= num_rows < 2 ** 31 - 1:
+        raise ValueError(f"num_rows must be in [0, 2^31 - 1), got {num_rows}")
+    return _gradient(grad, index, num_rows, _scale(scale), True)
+
+
+# ---- rows by group --------------------------------------------------------------------
+class RowGroups:
+    """Entries sorted by group (``group_rows``), all int32 on the device: ``order`` (M,) the
+    entry at each place, ``slots`` (the index's shape) the place of each entry or -1,
+    ``offsets`` (num_groups + 1,) where each group begins and the last one ends."""
+
+    __slots__ = ("order", "slots", "offsets", "num_groups", "num_rows", "choices")
+
+    def __init__(self, order, slots, offsets, num_groups, num_rows, choices):
+        self.order, self.slots, self.offsets = order, slots, offsets
+        self.num_groups, self.num_rows, self.choices = num_groups, num_rows, choices
+
+    def _used(self):
+        return self.offsets.data_ptr() + 4 * self.num_groups
+
+
+def group_rows(index, num_groups):
+    """Sort the entries of `index`, (N,) or (N, k) int32 or int64 groups of N rows, stably by
+    group.  Entries outside [0, num_groups) come behind the last group and have slot -1."""
+    if not index.is_cuda:
+        raise ValueError("index must be a CUDA tensor")
+    if index.dim() not in (1, 2) or (index.dim() == 2 and index.shape[1] < 1):
+        raise ValueError(f"index must be (N,) or (N, k) with k >= 1, got {tuple(index.shape)}")
+    if not 1 <= num_groups < 2 ** 31 - 1:
+        raise ValueError(f"num_groups must be in [1, 2^31 - 1), got {num_groups}")
+    device = index.device
+    index = _index(index, device)
+    n = index.numel()
+    order = torch.empty(n, dtype=torch.int32, device=device)
+    slots = torch.empty(index.shape, dtype=torch.int32, device=device)
+    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
+    nbytes = _lib.lib().cvhrf_group_rows_workspace_bytes(n, num_groups)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with timed("group_rows"):
+        _call("cvhrf_group_rows", device, index.data_ptr(), _INDEX_BYTES[index.dtype], n, num_groups,
+              order.data_ptr(), slots.data_ptr(), offsets.data_ptr(), ws.data_ptr(), nbytes)
+    return RowGroups(order, slots, offsets, num_groups, index.shape[0], index.shape[1] if index.dim() == 2 else 1)
+
+
+def _to_groups(x, groups):
+    x, stride = _rows(x, "x")
+    out = torch.empty(groups.num_rows * groups.choices, x.shape[1], dtype=x.dtype, device=x.device)
+    with timed("rows_to_groups"):
+        _call("cvhrf_rows_to_groups", x.device, x.data_ptr(), stride, _TYPES[x.dtype], groups.num_rows,
+              groups.choices, x.shape[1], groups.slots.data_ptr(), groups._used(), out.data_ptr())
+    return out
+
+
+def _to_rows(y, groups, weights):
+    y, stride = _rows(y, "y")
+    out = torch.empty(groups.num_rows, y.shape[1], dtype=y.dtype, device=y.device)
+    with timed("groups_to_rows"):
+        _call("cvhrf_groups_to_rows", y.device, y.data_ptr(), stride, _TYPES[y.dtype], groups.num_rows,
+              groups.choices, y.shape[1], groups.slots.data_ptr(), None if weights is None else weights.data_ptr(),
+              0 if weights is None else _TYPES[weights.dtype], out.data_ptr())
+    return out
+
+
+class RowsToGroups(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups):
+        ctx.groups = groups
+        return _to_groups(x, groups)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return _to_rows(grad, ctx.groups, None), None
+
+
+class GroupsToRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, groups, weights):
+        ctx.groups = groups
+        ctx.save_for_backward(y, weights)
+        return _to_rows(y, groups, weights)
+
+    @staticmethod
+    def backward(ctx, grad):
+        y, weights = ctx.saved_tensors
+        groups = ctx.groups
+        grad, grad_stride = _rows(grad, "grad")
+        y, stride = _rows(y, "y")
+        need_y, _, need_w = ctx.needs_input_grad
+        grad_y = torch.empty(y.shape, dtype=y.dtype, device=y.device) if need_y else None
+        grad_w = torch.empty_like(weights) if need_w else None
+        with timed("groups_to_rows_backward"):
+            _call("cvhrf_groups_to_rows_backward", y.device, grad.data_ptr(), grad_stride, y.data_ptr(), stride,
+                  _TYPES[y.dtype], groups.num_rows, groups.choices, y.shape[1], groups.slots.data_ptr(),
+                  groups._used(), None if weights is None else weights.data_ptr(),
+                  0 if weights is None else _TYPES[weights.dtype], grad_y.data_ptr() if need_y else None,
+                  grad_w.data_ptr() if need_w else None)
+        return grad_y, None, grad_w
+
+
+def _check_groups(t, groups, rows, name):
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {tuple(t.shape)}")
+    if t.device != groups.slots.device:
+        raise ValueError(f"{name} must be on {groups.slots.device}, got {t.device}")
+
+
+def rows_to_groups(x, groups):
+    """Rows x (N, D) at their places: (N * k, D), row p the row of entry groups.order[p]; the
+    places behind the last group are zeros.  Differentiable in x (the sum over its places)."""
+    _check_groups(x, groups, groups.num_rows, "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        return RowsToGroups.apply(x, groups)
+    return _to_groups(x, groups)
+
+
+def groups_to_rows(y, groups, weights=None):
+    """Rows y (N * k, D) at their places back to the N rows: out[n] = sum_j weights[n, j]
+    y[groups.slots[n, j]], entries left out counting nothing.  weights have the grouped
+    index's shape, float32 or y's type (None: ones).  Differentiable in y and weights; the
+    gradient of the places behind the last group is zeros."""
+    _check_groups(y, groups, groups.num_rows * groups.choices, "y")
+    if weights is not None:
+        if weights.shape != groups.slots.shape or weights.device != y.device:
+            raise ValueError(f"weights must be {tuple(groups.slots.shape)} on {y.device}, got "
+                             f"{tuple(weights.shape)} on {weights.device}")
+        if weights.dtype not in (torch.float32, y.dtype):
+            raise TypeError(f"weights must be float32 or {y.dtype}, got {weights.dtype}")
+        weights = weights.contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        return GroupsToRows.apply(y, groups, weights)
+    return _to_rows(y, groups, weights)

@@ -540,6 +540,65 @@ int cvhrf_hologram_field_backward(const void* holo, int C, long long n, const fl
                                   const void* grad_field, void* grad_holo, void* workspace, size_t workspace_bytes,
                                   void* stream);
 
+/* ---- rows shared by many entries, and rows sorted by group ------------------- */
+/*
+ * Element types of rows.  Sums are float32 whatever the type; a result is rounded once.
+ */
+#define CVHRF_F32 0
+#define CVHRF_BF16 1
+#define CVHRF_F16 2
+/*
+ * Lookup of table rows (a codebook of attributes that many Gaussians share):
+ *   out[t] = scale * table[index[t]],  t < entries
+ * table: rows x width of type `dtype`, `row_stride` elements between rows; out: entries x
+ * width, contiguous.  index: int32 or int64 (index_bytes 4 or 8).  An index outside
+ * [0, rows) gives a row of zeros.  entries < 2^30, width <= 2^20.  No counterpart in the
+ * reference, whose Gaussians own all their attributes.
+ */
+int cvhrf_table_lookup(const void* table, long long rows, int width, long long row_stride, int dtype,
+                       const void* index, int index_bytes, long long entries, float scale, void* out, void* stream);
+/*
+ * Its gradient: grad_table[v] = scale * sum of grad[t] over the entries with index[t] = v
+ * (zeros where there is none), every row written; row_mask[v] (optional, may be null) = 1
+ * where there is one, the mask cvhrf_sparse_adam_masked takes.  The order of the sums is
+ * fixed (the entries' order, joined between blocks in a fixed order): results repeat bit
+ * for bit.  An entry whose index is outside [0, rows) is left out and its row not read.
+ */
+size_t cvhrf_table_gradient_workspace_bytes(long long entries, long long rows, int width);
+int cvhrf_table_gradient(const void* grad, long long grad_stride, int dtype, int width, const void* index,
+                         int index_bytes, long long entries, float scale, void* grad_table, long long rows,
+                         uint8_t* row_mask, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * The entries of an index array sorted stably by value (the group: a depth plane, an owner):
+ * order[p] = the entry at place p, slots[e] = the place of entry e, offsets[g] = where group
+ * g begins (groups + 1 values; the last is where the last group ends).  Entries whose value
+ * is outside [0, groups) follow behind the last group and have slot -1.
+ */
+size_t cvhrf_group_rows_workspace_bytes(long long entries, int groups);
+int cvhrf_group_rows(const void* index, int index_bytes, long long entries, int groups, int* order, int* slots,
+                     int* offsets, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Rows to their groups and back.  Row n has `choices` entries n * choices + j with places
+ * slots[n * choices + j]; used = (device) the number of places that belong to a group
+ * (offsets + groups of cvhrf_group_rows).
+ *   cvhrf_rows_to_groups:  out[slot] = x[n]  (n * choices rows; those from *used on are zeros)
+ *   cvhrf_groups_to_rows:  out[n] = sum_j weights[n, j] y[slots[n, j]]  (float32 sum; entries
+ *     left out count nothing; weights null: ones).  Without weights it is the gradient of
+ *     cvhrf_rows_to_groups.
+ *   cvhrf_groups_to_rows_backward: grad_y[slot] = weights[n, j] grad[n] (rows from *used on:
+ *     zeros), grad_weights[n, j] = <grad[n], y[slot]> (0 where left out); either may be null.
+ * weights are float32 or of type `dtype`, n x choices, contiguous; x, y and grad take a row
+ * stride, outputs are contiguous.
+ */
+int cvhrf_rows_to_groups(const void* x, long long x_stride, int dtype, long long n, int choices, int width,
+                         const int* slots, const int* used, void* out, void* stream);
+int cvhrf_groups_to_rows(const void* y, long long y_stride, int dtype, long long n, int choices, int width,
+                         const int* slots, const void* weights, int weights_dtype, void* out, void* stream);
+int cvhrf_groups_to_rows_backward(const void* grad, long long grad_stride, const void* y, long long y_stride,
+                                  int dtype, long long n, int choices, int width, const int* slots, const int* used,
+                                  const void* weights, int weights_dtype, void* grad_y, void* grad_weights,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

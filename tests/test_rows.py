@@ -1,0 +1,574 @@
+"""Rows shared by many entries and rows sorted by group (rows.py) against plain 64-bit
+definitions, at the sizes, types, strides and left-out entries where they can go wrong.
+
+Tolerances: u = 2^-24 is half a step of float32, eps(t) / 2 of a result of type t.  A sum of
+n float32 terms in any order is off by at most (n - 1) u sum|term| (first order in u; n is
+used), a product by u, and the rounding to t by eps(t) / 2 of the value (or half the smallest
+subnormal).  No constant beyond these is added, except 1 + 2^-10 for the terms of second order.
+"""
+import ctypes
+
+import pytest
+import torch
+
+from complex_valued_holographic_radiance_fields_b200 import _lib
+from complex_valued_holographic_radiance_fields_b200 import rows as R
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+gpu = pytest.mark.gpu
+
+
+def close(got, exact, slack):
+    """got (any type) against exact (float64), with `slack` (float64) before the last rounding."""
+    t = got.dtype
+    info = torch.finfo(t)
+    tol = (slack + (exact.abs() + slack) * info.eps / 2 + info.smallest_normal * info.eps / 2) * (1 + 2.0 ** -10)
+    off = (got.double() - exact).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), (int(bad.sum()), float(off[bad].max()), float(tol[bad].min()))
+
+
+def normal(shape, dtype, seed, dev="cuda"):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return torch.randn(shape, generator=g, device=dev).to(dtype)
+
+
+def integers(n, high, seed, low=0, dtype=torch.int64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(low, high, (n,), generator=g, device="cuda").to(dtype)
+
+
+def inside_of(index, rows):
+    return (index >= 0) & (index < rows)
+
+
+# ---- shared rows ----------------------------------------------------------------------
+def lookup_64(table, index, scale):
+    index = index.long()
+    out = torch.zeros(*index.shape, table.shape[1], dtype=torch.float64, device=table.device)
+    ok = inside_of(index, table.shape[0])
+    out[ok] = table[index[ok]].double() * scale
+    return out
+
+
+def gradient_64(grad, index, rows, scale):
+    """The exact sums, sum |term| and the number of terms of each row."""
+    index, grad = index.reshape(-1).long(), grad.reshape(-1, grad.shape[-1])
+    at = torch.nonzero(inside_of(index, rows))[:, 0]
+    total = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device=grad.device)
+    size, count = torch.zeros_like(total), torch.zeros(rows, dtype=torch.float64, device=grad.device)
+    g = grad[at].double() * scale
+    total.index_add_(0, index[at], g)
+    size.index_add_(0, index[at], g.abs())
+    count.index_add_(0, index[at], torch.ones_like(at, dtype=torch.float64))
+    return total, size, count
+
+
+def check_gradient(got, mask, grad, index, rows, scale):
+    total, size, count = gradient_64(grad, index, rows, scale)
+    close(got, total, (count[:, None] + 1) * U * size)
+    assert torch.equal(mask, (count > 0).to(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 20, 59, 64, 129, 333, 1024, 4104])
+@pytest.mark.parametrize("n,rows", [(1, 1), (1, 5000), (7, 3), (2049, 64)])
+def test_lookup(cuda, dtype, width, n, rows):
+    table = normal((rows, width), dtype, width)
+    for itype in (torch.int32, torch.int64):
+        index = integers(n, rows + 2, n + rows, -2, itype)   # some outside on either side
+        for scale in (1.0, -0.7, 45.25):
+            out = R.table_lookup(table, index, scale)
+            exact = lookup_64(table, index, scale)
+            assert out.dtype == dtype and out.shape == exact.shape
+            close(out, exact, 0.0 * exact if scale == 1.0 else U * exact.abs())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 8, 12, 20, 59, 64, 130, 256, 333, 1000, 2056])
+@pytest.mark.parametrize("n,rows", [(1, 1), (1, 3000), (5, 2), (513, 1), (2049, 40), (300, 20011), (9000, 700)])
+def test_gradient(cuda, dtype, width, n, rows):
+    grad = normal((n, width), dtype, width + n)
+    for itype in (torch.int32, torch.int64):
+        index = integers(n, rows + 1, n + rows, -1, itype)
+        got, mask = R.table_gradient(grad, index, rows, 0.75)
+        assert got.dtype == dtype
+        check_gradient(got, mask, grad, index, rows, 0.75)
+
+
+def skewed(kind, n, rows):
+    if kind == "one_row":
+        return torch.full((n,), rows // 2, device="cuda")
+    if kind == "first_and_last":
+        return torch.where(integers(n, 2, 1) == 1, rows - 1, 0)
+    if kind == "none":
+        return torch.full((n,), -1, device="cuda")
+    if kind == "sorted":
+        return integers(n, rows, 2).sort()[0]
+    if kind == "reversed":
+        return integers(n, rows, 3).sort(descending=True)[0]
+    if kind == "half_in_one":
+        return torch.where(integers(n, 2, 4) == 1, rows // 3, integers(n, rows, 5))
+    u = torch.rand(n, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    return (u.pow(4) * rows).long().clamp_(max=rows - 1)   # "popular"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["one_row", "first_and_last", "none", "sorted", "reversed", "half_in_one", "popular"])
+@pytest.mark.parametrize("n,rows,width,dtype", [(100003, 4096, 3, torch.float32), (70001, 257, 59, torch.float32),
+                                                (20000, 30000, 264, torch.bfloat16), (40000, 2, 130, torch.float16),
+                                                (3001, 1, 8, torch.float32), (300000, 65536, 4, torch.float32)])
+def test_gradient_of_skewed_rows(cuda, kind, n, rows, width, dtype):
+    grad = (normal((n, width), torch.float32, n) * 0.05).to(dtype)
+    index = skewed(kind, n, rows)
+    got, mask = R.table_gradient(grad, index, rows)
+    check_gradient(got, mask, grad, index, rows, 1.0)
+    again, mask2 = R.table_gradient(grad, index, rows)
+    assert torch.equal(got, again) and torch.equal(mask, mask2)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [255, 256, 257, 65535, 65536, 65537, (1 << 24) + 3])
+def test_gradient_at_the_edges_of_the_sort(cuda, rows):
+    index = torch.cat([integers(5000, rows, rows), torch.tensor([0, rows - 1, rows - 1, rows, -1], device="cuda")])
+    grad = normal((index.numel(), 2), torch.float32, 1)
+    got, mask = R.table_gradient(grad, index, rows)
+    check_gradient(got, mask, grad, index, rows, 1.0)
+
+
+@gpu
+def test_indices_far_outside(cuda):
+    table = normal((100, 6), torch.float32, 0)
+    index = torch.tensor([2 ** 62, -2 ** 63, 2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, 99, 100, 2 ** 63 - 1], device="cuda")
+    out = R.table_lookup(table, index)
+    assert torch.equal(out[5], table[99])
+    assert not out[[0, 1, 2, 3, 4, 6, 7]].any()
+    grad = torch.full((8, 6), float("nan"), device="cuda")
+    grad[5] = 1.0
+    got, mask = R.table_gradient(grad, index, 100)          # what is left out is not read, NaN or not
+    assert torch.equal(mask.nonzero()[:, 0], torch.tensor([99], device="cuda"))
+    assert torch.equal(got[99], torch.ones(6, device="cuda")) and not got[:99].any()
+    groups = R.group_rows(index, 100)
+    assert groups.offsets[100] == 1 and groups.slots[5] == 0
+
+
+@gpu
+def test_infinities_stay_in_their_row(cuda):
+    grad = torch.ones(64, 5, device="cuda")
+    grad[10, 2], grad[11, 2], grad[12, 3] = float("inf"), float("-inf"), float("nan")
+    index = torch.arange(64, device="cuda") // 2
+    got, _ = R.table_gradient(grad, index, 40)
+    exact = torch.zeros(40, 5, device="cuda").index_add_(0, index, grad)
+    assert torch.equal(torch.nan_to_num(got, 7, 8, 9), torch.nan_to_num(exact, 7, 8, 9))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strided_rows(cuda, dtype):
+    big = normal((50, 100), dtype, 0)
+    index = integers(70, 50, 1)
+    for table in (big[:, 8:40], big[:, 3:36], big[::2], big.t(), big[:, ::3], big[:, 5:6]):
+        idx = index % table.shape[0]
+        assert torch.equal(R.table_lookup(table, idx), table[idx])
+    wide = normal((70, 100), dtype, 2)
+    for grad in (wide[:, 8:40], wide[:, 1:34], wide[:, ::2], wide[:1].expand(70, 100), wide[:, :1].expand(70, 20)):
+        got, mask = R.table_gradient(grad, index, 50)
+        check_gradient(got, mask, grad.contiguous(), index, 50, 1.0)
+    # indices of other shapes and orders
+    square = index[:64].reshape(8, 8).t()
+    assert torch.equal(R.table_lookup(big, square), big[square])
+    got, mask = R.table_gradient(wide[:64].reshape(8, 8, 100), square, 50)
+    check_gradient(got, mask, wide[:64], square.reshape(-1), 50, 1.0)
+    assert torch.equal(R.table_lookup(big, index[3]), big[index[3]])          # one index: one row
+
+
+@gpu
+def test_nothing_to_do(cuda):
+    table = normal((5, 12), torch.float32, 0)
+    empty = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert R.table_lookup(table, empty).shape == (0, 12)
+    got, mask = R.table_gradient(torch.empty(0, 12, device="cuda"), empty, 5)
+    assert got.shape == (5, 12) and not got.any() and not mask.any()
+    none = torch.empty(0, 12, device="cuda")
+    assert not R.table_lookup(none, torch.zeros(3, dtype=torch.int64, device="cuda")).any()
+    got, mask = R.table_gradient(table, torch.zeros(5, dtype=torch.int64, device="cuda"), 0)
+    assert got.shape == (0, 12) and mask.shape == (0,)
+    groups = R.group_rows(empty, 3)
+    assert groups.order.numel() == 0 and not groups.offsets.any()
+    assert R.rows_to_groups(none, groups).shape == (0, 12)
+    assert R.groups_to_rows(none, groups).shape == (0, 12)
+
+
+@gpu
+def test_offsets_beyond_32_bits(cuda):
+    rows, width = 1100000, 2048                       # 2.25e9 elements
+    table = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda")
+    last = torch.tensor([rows - 1, 1048576, 1048575, 0, rows - 2], device="cuda")
+    table[last] = normal((5, width), torch.bfloat16, 0)
+    assert torch.equal(R.table_lookup(table, last), table[last])
+    del table
+    grad = normal((5, width), torch.bfloat16, 1)
+    got, mask = R.table_gradient(grad, last, rows)
+    assert torch.equal(got[last], grad)
+    assert int(mask.sum()) == 5 and int(torch.count_nonzero(got)) == int(torch.count_nonzero(grad))
+    del got
+    # a wide batch: the places of the rows go beyond 2^31 elements
+    n = 1050000
+    index = (torch.arange(n, device="cuda") % 3).to(torch.int32)
+    groups = R.group_rows(index, 3)
+    x = torch.empty(n, width, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = normal((3, width), torch.bfloat16, 2)
+    xs = R.rows_to_groups(x, groups)
+    assert torch.equal(xs[groups.slots[-3:].long()], x[-3:])
+    del x
+    assert torch.equal(R.groups_to_rows(xs, groups)[-3:], xs[groups.slots[-3:].long()])
+
+
+# ---- rows by group --------------------------------------------------------------------
+def places_64(index, groups):
+    """(order, slots, offsets) by a stable sort on the host."""
+    flat = index.reshape(-1).long().cpu()
+    key = torch.where(inside_of(flat, groups), flat, groups)
+    order = torch.sort(key, stable=True)[1]
+    place = torch.empty_like(order)
+    place[order] = torch.arange(order.numel())
+    slots = torch.where(key < groups, place, -1).reshape(index.shape)
+    offsets = torch.zeros(groups + 1, dtype=torch.int64)
+    offsets[1:] = torch.bincount(key, minlength=groups + 1)[:groups].cumsum(0)
+    return order, slots, offsets
+
+
+@gpu
+@pytest.mark.parametrize("groups", [1, 2, 3, 7, 64, 254, 255, 256, 257, 1000, 70000])
+@pytest.mark.parametrize("n,k", [(1, 1), (31, 1), (5, 3), (1024, 1), (1025, 2), (20011, 4), (310007, 1)])
+def test_groups(cuda, groups, n, k):
+    for itype in (torch.int32, torch.int64):
+        index = integers(n * k, groups + 1, n + groups, -1, itype).reshape(n, k)
+        index = index[:, 0] if k == 1 else index
+        got = R.group_rows(index, groups)
+        for a, b in zip((got.order, got.slots, got.offsets), places_64(index, groups)):
+            assert a.dtype == torch.int32 and torch.equal(a.long().cpu(), b)
+
+
+@gpu
+def test_groups_of_one_kind(cuda):
+    for value in (0, 2, -1, 9):
+        index = torch.full((5000,), value, dtype=torch.int32, device="cuda")
+        got = R.group_rows(index, 3)
+        for a, b in zip((got.order, got.slots, got.offsets), places_64(index, 3)):
+            assert torch.equal(a.long().cpu(), b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,wtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                         (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                         (torch.float16, None)])
+@pytest.mark.parametrize("width", [1, 3, 8, 20, 59, 64, 333, 1024, 2056])
+@pytest.mark.parametrize("n,k,groups", [(1, 1, 1), (3, 8, 8), (301, 2, 7), (1000, 3, 300)])
+def test_moves_and_their_gradients(cuda, dtype, wtype, width, n, k, groups):
+    index = integers(n * k, groups + 1, n + width, -1).reshape(n, k)
+    if n > 1:
+        index[n // 2] = -1                                   # a row without any group
+    ix = index[:, 0] if k == 1 else index
+    g = R.group_rows(ix, groups)
+    order, slots, offsets = (t.cuda() for t in places_64(ix, groups))
+    used = int(offsets[-1])
+    x = normal((n, width), dtype, 1).requires_grad_(True)
+    y0 = normal((n * k, width), dtype, 2)
+    y0[used:] = float("nan")                                 # what is left out is not read
+    y = y0.clone().requires_grad_(True)
+    w = None
+    if wtype is not None:
+        w0 = torch.rand(ix.shape, device="cuda").to(wtype)
+        w0[~inside_of(ix, groups)] = float("nan")
+        w = w0.clone().requires_grad_(True)
+    d_xs, d_out = normal((n * k, width), dtype, 3), normal((n, width), dtype, 4)
+    d_xs[used:] = float("nan")
+
+    xs = R.rows_to_groups(x, g)
+    assert torch.equal(xs[:used], x.detach()[order[:used] // k]) and not xs[used:].any()
+    out = R.groups_to_rows(y, g, w)
+
+    kept = (slots >= 0).reshape(n, k)
+    at = slots.reshape(n, k).clamp(min=0)
+    weight = torch.ones(n, k, dtype=torch.float64, device="cuda") if w is None else w0.double().reshape(n, k)
+    weight = torch.where(kept, weight, 0.0)
+    rows = torch.where(kept[:, :, None], y0.double()[at], 0.0)
+    terms = weight[:, :, None] * rows
+    close(out, terms.sum(1), k * U * terms.abs().sum(1))
+
+    leaves = (x, y) if w is None else (x, y, w)
+    got = torch.autograd.grad((xs, out), leaves, (d_xs, d_out))
+    terms = torch.where(kept[:, :, None], d_xs.double()[at], 0.0)
+    close(got[0], terms.sum(1), k * U * terms.abs().sum(1))
+    exact = torch.zeros(n * k, width, dtype=torch.float64, device="cuda")
+    exact[at[kept]] = (weight[:, :, None] * d_out.double()[:, None, :])[kept]
+    close(got[1], exact, U * exact.abs())
+    if w is not None:
+        terms = d_out.double()[:, None, :] * rows
+        assert got[2].dtype == wtype and got[2].shape == ix.shape
+        close(got[2].reshape(n, k), terms.sum(2), width * U * terms.abs().sum(2))
+
+
+@gpu
+def test_gradients_only_of_what_is_asked(cuda):
+    g = R.group_rows(integers(40, 5, 0).reshape(20, 2), 4)
+    y, w = normal((40, 6), torch.float32, 1), torch.rand(20, 2, device="cuda")
+    d = normal((20, 6), torch.float32, 2)
+    a, b = y.clone().requires_grad_(), w.clone().requires_grad_()
+    dy, dw = torch.autograd.grad(R.groups_to_rows(a, g, b), (a, b), d)
+    assert torch.equal(torch.autograd.grad(R.groups_to_rows(a, g, w), a, d)[0], dy)
+    assert torch.equal(torch.autograd.grad(R.groups_to_rows(y, g, b), b, d)[0], dw)
+    assert not R.groups_to_rows(y, g, w).requires_grad
+    with torch.no_grad():
+        assert not R.groups_to_rows(a, g, b).requires_grad
+
+
+@gpu
+def test_strided_moves(cuda):
+    g = R.group_rows(integers(60, 4, 0).reshape(30, 2), 4)
+    big, bigy = normal((30, 50), torch.float32, 1), normal((60, 100), torch.float32, 2)
+    w = torch.rand(2, 30, device="cuda").t()                 # weights in the other order
+    for x in (big[:, 4:24], big[:, 1:22], big[:, ::2], big[:1].expand(30, 50)):
+        assert torch.equal(R.rows_to_groups(x, g), R.rows_to_groups(x.contiguous(), g))
+    for y in (bigy[:, 4:24], bigy[:, 1:22], bigy[:, ::3]):
+        assert torch.equal(R.groups_to_rows(y, g, w), R.groups_to_rows(y.contiguous(), g, w.contiguous()))
+        a, b, c, d = y.clone().requires_grad_(), w.clone().requires_grad_(), y.detach().requires_grad_(), w.detach().requires_grad_()
+        for upstream in (torch.ones(30, 1, device="cuda").expand(30, y.shape[1]), big[:, 1:1 + y.shape[1]]):
+            if upstream.shape[1] != y.shape[1]:
+                continue
+            one = torch.autograd.grad(R.groups_to_rows(a, g, b), (a, b), upstream.contiguous())
+            two = torch.autograd.grad(R.groups_to_rows(c, g, d), (c, d), upstream)
+            assert torch.equal(one[0], two[0])
+            # a row that can be read 16 bytes at a time adds its columns to the dot product in
+            # another order than one that cannot, so the two are not bit-equal: each is within
+            # (width) u sum|term| of the exact value
+            terms = upstream.double()[:, None, :] * torch.where(
+                (g.slots >= 0)[:, :, None], y.double()[g.slots.long().clamp(min=0)], 0.0)
+            for dw in (one[1], two[1]):
+                close(dw, terms.sum(2), y.shape[1] * U * terms.abs().sum(2))
+
+
+# ---- gradients against differences -------------------------------------------------------
+@gpu
+def test_gradients_against_differences(cuda):
+    """The operators are linear (bilinear in y and weights), so a central difference with any
+    step is exact up to rounding: small integers make every sum and product exact."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+
+    def ints(*shape):
+        return torch.randint(-4, 5, shape, generator=gen, device="cuda").float()
+
+    index = integers(12, 6, 1, -1)
+    groups = R.group_rows(integers(12, 4, 2, -1).reshape(6, 2), 3)
+    up, up_rows, up_places = ints(12, 3), ints(6, 3), ints(12, 3)
+    cases = [(lambda t: (R.table_lookup(t, index, 2.0) * up).sum(), ints(5, 3)),
+             (lambda x: (R.rows_to_groups(x, groups) * up_places).sum(), ints(6, 3))]
+    y, w = ints(12, 3), ints(6, 2)
+    cases += [(lambda t: (R.groups_to_rows(t, groups, w) * up_rows).sum(), y),
+              (lambda t: (R.groups_to_rows(y, groups, t) * up_rows).sum(), w)]
+    for f, at in cases:
+        leaf = at.clone().requires_grad_(True)
+        f(leaf).backward()
+        for i in range(at.numel()):
+            step = torch.zeros_like(at)
+            step.view(-1)[i] = 1.0
+            assert leaf.grad.view(-1)[i] == (f(at + step) - f(at - step)) / 2
+
+
+# ---- as they are used together ---------------------------------------------------------
+@gpu
+def test_table_trained_with_sparse_adam(cuda):
+    """Lookup, its gradient and the row-sparse optimizer: rows no entry names keep their values."""
+    from complex_valued_holographic_radiance_fields_b200 import SparseGaussianAdam
+    table = normal((50, 3), torch.float32, 0).requires_grad_(True)
+    start = table.detach().clone()
+    index = integers(400, 30, 1)
+    target = normal((400, 3), torch.float32, 2)
+    opt = SparseGaussianAdam([{"params": [table], "lr": 1e-2}], lr=1e-2, eps=1e-15)
+    out = R.table_lookup(table, index)
+    (out - target).square().sum().backward()
+    grad, mask = R.table_gradient(2 * (out.detach() - target), index, 50)
+    assert torch.equal(grad, table.grad)
+    opt.step(row_mask=mask)
+    assert torch.equal(table.detach()[30:], start[30:])
+    named = torch.unique(index)
+    g = table.grad[named]
+    m, v = 0.1 * g, 0.001 * g * g
+    assert torch.allclose(table.detach()[named], start[named] - 1e-2 * m / (v.sqrt() + 1e-15), rtol=1e-5, atol=1e-6)
+
+
+@gpu
+def test_round_trip_through_groups(cuda):
+    n, k = 999, 3
+    g = R.group_rows(integers(n * k, 5, 0).reshape(n, k), 5)
+    x = torch.randint(-8, 9, (n, 33), device="cuda").float()
+    assert torch.equal(R.groups_to_rows(R.rows_to_groups(x, g), g), 3 * x)
+
+
+# ---- streams, graphs, devices ------------------------------------------------------------
+@gpu
+def test_captured_and_replayed(cuda):
+    """A whole step in a CUDA graph, replayed on new contents of its inputs, with an eager step between."""
+    def make(seed):
+        return dict(index=integers(5000, 301, seed, -1), x=normal((2500, 20), torch.float32, seed),
+                    table=normal((300, 20), torch.float32, seed + 1), up=normal((5000, 20), torch.float32, seed + 2),
+                    w=torch.rand(2500, 2, device="cuda"))
+
+    def step(s):
+        t = s["table"].detach().requires_grad_(True)
+        out = R.table_lookup(t, s["index"], 0.5)
+        dt, = torch.autograd.grad(out, t, s["up"])
+        g = R.group_rows(s["index"].reshape(2500, 2), 300)
+        x, w = s["x"].detach().requires_grad_(True), s["w"].detach().requires_grad_(True)
+        xs = R.rows_to_groups(x, g)
+        back = R.groups_to_rows(xs, g, w)
+        dx, dw = torch.autograd.grad(back, (x, w), s["up"][:2500])
+        return out, dt, g.order, g.slots, g.offsets, xs, back, dx, dw
+
+    static = make(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for seed in (10, 20):
+        new = make(seed)
+        expected = [t.clone() for t in step(new)]
+        for name, t in new.items():
+            static[name].copy_(t)
+        graph.replay()
+        for a, b in zip(outs, expected):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_two_streams_at_once(cuda):
+    index = [integers(200000, 5000, s, -1) for s in (1, 2)]
+    grad = [normal((200000, 12), torch.float32, s) for s in (3, 4)]
+    alone = [R.table_gradient(g, i, 5000)[0].clone() for g, i in zip(grad, index)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(R.table_gradient(grad[k], index[k], 5000)[0])
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(t, alone[k]) for t in got[k])
+
+
+@gpu
+def test_another_device_than_the_current_one(cuda):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    table = normal((10, 4), torch.float32, 0, "cuda:1")
+    index = torch.tensor([3, 3, 9], device="cuda:1")
+    assert torch.cuda.current_device() == 0
+    assert torch.equal(R.table_lookup(table, index), table[index])
+    with pytest.raises(ValueError):
+        R.table_lookup(table, index.to("cuda:0"))
+
+
+# ---- refusals -----------------------------------------------------------------------------
+def test_refusals_need_no_gpu():
+    cpu = torch.zeros(3, 4)
+    index = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA"):
+        R.table_lookup(cpu, index)
+    with pytest.raises(ValueError, match="CUDA"):
+        R.table_gradient(torch.zeros(2, 4), index, 3)
+    with pytest.raises(ValueError, match="CUDA"):
+        R.group_rows(index, 3)
+    with pytest.raises(TypeError, match="float32"):
+        R.table_lookup(cpu.double(), index)
+    with pytest.raises(TypeError, match="number"):
+        R.table_lookup(cpu, index, torch.ones(()))
+    with pytest.raises(ValueError, match="shape"):
+        R.table_gradient(torch.zeros(3, 4), index, 3)
+    with pytest.raises(ValueError, match="num_rows"):
+        R.table_gradient(torch.zeros(2, 4), index, -1)
+
+
+def test_c_abi_refusals_need_no_gpu():
+    """Bad arguments come back as a status before anything is launched."""
+    L = _lib.lib()
+    p = ctypes.c_void_p(256)   # never read: every call is refused
+
+    def lookup(table=p, rows=4, width=4, stride=4, dtype=0, index=p, bytes_=4, n=2, out=p):
+        return L.cvhrf_table_lookup(table, rows, width, stride, dtype, index, bytes_, n, 1.0, out, None)
+
+    for bad in (dict(table=None), dict(rows=-1), dict(rows=2 ** 31), dict(width=0), dict(width=2 ** 20 + 1),
+                dict(stride=-1), dict(dtype=3), dict(index=None), dict(bytes_=2), dict(n=-1), dict(out=None)):
+        assert lookup(**bad) == 1, bad
+    assert lookup(n=2 ** 30) == 4
+    assert lookup(n=0) == 0
+
+    need = L.cvhrf_table_gradient_workspace_bytes(1000, 10, 8)
+    assert need > 0 and L.cvhrf_table_gradient_workspace_bytes(-1, 10, 8) == 0
+
+    def gradient(grad=p, stride=8, dtype=0, width=8, index=p, bytes_=8, n=1000, out=p, rows=10, ws=p, nbytes=need):
+        return L.cvhrf_table_gradient(grad, stride, dtype, width, index, bytes_, n, 1.0, out, rows, None, ws, nbytes,
+                                      None)
+
+    for bad in (dict(grad=None), dict(stride=-1), dict(dtype=-1), dict(width=0), dict(index=None), dict(bytes_=1),
+                dict(n=-1), dict(out=None), dict(rows=-1)):
+        assert gradient(**bad) == 1, bad
+    assert gradient(ws=None) == 2 and gradient(nbytes=need - 1) == 2
+    assert gradient(n=2 ** 30) == 4
+
+    need = L.cvhrf_group_rows_workspace_bytes(1000, 5)
+
+    def group(index=p, bytes_=4, n=1000, groups=5, order=p, slots=p, offsets=p, ws=p, nbytes=need):
+        return L.cvhrf_group_rows(index, bytes_, n, groups, order, slots, offsets, ws, nbytes, None)
+
+    for bad in (dict(index=None), dict(bytes_=3), dict(n=-1), dict(groups=0), dict(order=None), dict(slots=None),
+                dict(offsets=None)):
+        assert group(**bad) == 1, bad
+    assert group(ws=None) == 2 and group(nbytes=need - 1) == 2 and group(n=2 ** 30) == 4
+
+    assert L.cvhrf_rows_to_groups(p, 4, 0, 2 ** 29, 2, 4, p, p, p, None) == 4
+    assert L.cvhrf_rows_to_groups(p, 4, 0, 5, 0, 4, p, p, p, None) == 1
+    assert L.cvhrf_rows_to_groups(p, 4, 0, 5, 1, 4, None, p, p, None) == 1
+    assert L.cvhrf_groups_to_rows(p, 4, 1, 5, 1, 4, p, p, 2, p, None) == 1     # weights of another 16-bit type
+    assert L.cvhrf_groups_to_rows(p, 4, 0, 5, 1, 4, p, None, 0, None, None) == 1
+    assert L.cvhrf_groups_to_rows_backward(p, 4, p, 4, 0, 5, 1, 4, p, p, None, 0, p, p, None) == 1
+    assert L.cvhrf_groups_to_rows_backward(p, 4, None, 4, 0, 5, 1, 4, p, p, p, 0, p, p, None) == 1
+
+
+@gpu
+def test_refusals_on_the_gpu(cuda):
+    table, index = torch.zeros(3, 4, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    for bad in (index.cpu(), ):
+        with pytest.raises(ValueError, match="index must be on"):
+            R.table_lookup(table, bad)
+    for bad in (index.to(torch.int16), index.float(), index.bool()):
+        with pytest.raises(TypeError, match="int32 or int64"):
+            R.table_lookup(table, bad)
+        with pytest.raises(TypeError, match="int32 or int64"):
+            R.group_rows(bad, 3)
+    with pytest.raises(ValueError, match="width"):
+        R.table_lookup(table[0], index)
+    with pytest.raises(ValueError, match="width"):
+        R.table_lookup(table[:, :0], index)
+    with pytest.raises(ValueError, match="num_groups"):
+        R.group_rows(index, 0)
+    with pytest.raises(ValueError, match="k >= 1"):
+        R.group_rows(index.reshape(1, 1, 2), 3)
+    g = R.group_rows(index, 3)
+    with pytest.raises(ValueError, match="2 rows"):
+        R.rows_to_groups(table, g)
+    with pytest.raises(ValueError, match="2 rows"):
+        R.groups_to_rows(table, g)
+    with pytest.raises(ValueError, match="weights must be"):
+        R.groups_to_rows(table[:2], g, torch.ones(2, 1, device="cuda"))
+    with pytest.raises(TypeError, match="weights must be"):
+        R.groups_to_rows(table[:2], g, torch.ones(2, device="cuda", dtype=torch.float16))
+
