@@ -8,14 +8,19 @@
 // (A look-back between tiles, as in scan_sort.cu, needs a cleared status array, one more
 // launch for the histogram, and a walk over the earlier tiles in L2 latency.)
 // The first pass reads the caller's indices as they are (4 or 8 bytes).
+//
+// Bound by latency: one block of 1024 threads per SM takes a chunk of up to 8192 keys in
+// registers, so a pass is a handful of dependent steps.  Up to 8192 keys in all, one block
+// does every pass in shared memory (small_sort_kernel, one launch).
 #include "row_groups.cuh"
 
 namespace cvhrf {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kItems = 4, kTile = kThreads * kItems;
-constexpr int kMaxChunks = 296;   // two blocks per SM
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kItems = 8, kTile = kThreads * kItems;
+constexpr int kMaxChunks = 148;   // one block per SM
 constexpr int kMaxRadix = 256;
+constexpr uint32_t kNone = 0xffffffffu;
 
 struct Source {
   const void* index;         // the caller's indices in the first pass
@@ -26,48 +31,63 @@ struct Source {
   int keep;
 };
 
-// Key of item i; false if it is left out.
-__device__ __forceinline__ bool source_key(const Source& s, uint32_t i, uint32_t& key) {
-  if (s.bytes == 0) {
-    key = s.keys[i];
-    return true;
-  }
+struct Target {
+  uint32_t* keys;      // null: not wanted
+  uint32_t* entries;
+  int* slots;          // cvhrf_group_rows: the place of each entry, -1 behind the last group
+  int* offsets;        // ... and where each of the `groups` groups begins, and the last one ends
+  int groups;
+  uint32_t* count;     // number of sorted items
+};
+
+// Key of item i, kNone if it is left out (keys are below 2^31).
+__device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
+  if (s.bytes == 0) return s.keys[i];
   const unsigned long long v = s.bytes == 4 ? (unsigned long long)(long long)((const int*)s.index)[i]
                                             : ((const unsigned long long*)s.index)[i];
-  const bool inside = v < s.rows;
-  key = inside ? (uint32_t)v : s.rows;
-  return inside || s.keep;
+  return v < s.rows ? (uint32_t)v : (s.keep ? s.rows : kNone);
 }
 
 // counts[chunk][digit] over the keys of each chunk.
 __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, const uint32_t* __restrict__ n_dev,
                                                                uint32_t chunk, int shift, int radix,
                                                                uint32_t* __restrict__ counts) {
-  __shared__ uint32_t h[kWarps][kMaxRadix];
+  constexpr int kCopies = 8;   // histograms, so that equal digits of different warps do not meet
+  __shared__ uint32_t h[kCopies][kMaxRadix];
   if (n_dev) n = min(n, *n_dev);
-  for (int i = threadIdx.x; i < kWarps * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < kCopies * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
-  const uint32_t mask = radix - 1;
-  for (uint32_t base = begin + warp * 32; base < end; base += kThreads) {
-    uint32_t key, d = 0xffffffffu;
-    if (base + lane < end && source_key(s, base + lane, key)) d = (key >> shift) & mask;
-    // one add per distinct digit of the warp: few groups would otherwise add to one word 32 times
-    const unsigned peers = __match_any_sync(0xffffffffu, d);
-    if (d != 0xffffffffu && (peers & ((1u << lane) - 1u)) == 0) h[warp][d] += __popc(peers);
-    __syncwarp();
+  uint32_t* mine = h[(threadIdx.x >> 5) % kCopies];
+  for (uint32_t tile = begin; tile < end; tile += kTile) {
+    uint32_t key[kItems];
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const uint32_t i = tile + r * kThreads + threadIdx.x;
+      key[r] = i < end ? source_key(s, i) : kNone;
+    }
+#pragma unroll
+    for (int r = 0; r < kItems; ++r)
+      if (key[r] != kNone) atomicAdd(&mine[(key[r] >> shift) & (radix - 1)], 1u);
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += kThreads) {
+  if (threadIdx.x < radix) {
     uint32_t c = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) c += h[w][d];
-    counts[(size_t)blockIdx.x * radix + d] = c;
+    for (int w = 0; w < kCopies; ++w) c += h[w][threadIdx.x];
+    counts[(size_t)blockIdx.x * radix + threadIdx.x] = c;
   }
 }
 
-// Exclusive scan over the 256 values of a block's first 256 threads; all threads call it.
+struct Shared {
+  uint32_t cnt[kWarps][kMaxRadix];
+  uint32_t key[kTile], entry[kTile];   // the tile in digit order
+  uint32_t base[kMaxRadix];            // place of the chunk's next key with this digit
+  uint32_t start[kMaxRadix];           // start of the digit inside the tile
+  uint32_t sh[9];
+};
+
+// Exclusive scan over the values of a block's first 256 threads; all threads call it.
 __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, uint32_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t inc = v;
@@ -78,15 +98,15 @@ __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, u
   }
   if (warp < 8 && lane == 31) sh[warp] = inc;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t run = 0;
+  if (warp == 0) {
+    uint32_t t = lane < 8 ? sh[lane] : 0u, run = t;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const uint32_t t = sh[w];
-      sh[w] = run;
-      run += t;
+    for (int o = 1; o < 8; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += u;
     }
-    sh[8] = run;
+    if (lane < 8) sh[lane] = run - t;
+    if (lane == 7) sh[8] = run;
   }
   __syncthreads();
   const uint32_t r = (warp < 8 ? sh[warp] : 0u) + inc - v;
@@ -95,114 +115,182 @@ __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, u
   return r;
 }
 
-struct Target {
-  uint32_t* keys;      // null: not wanted
-  uint32_t* entries;
-  int* slots;          // cvhrf_group_rows in one pass: the place of each entry, -1 behind the last group
-  int* offsets;        // ... and where each of the `groups` groups begins, and the last one ends
-  int groups;
-  uint32_t* count;     // number of sorted items
-};
+// Sorts one tile by a digit into sh.key / sh.entry.  Warp w holds the `rounds` x 32 keys from
+// w * rounds * 32 on (key[r] of lane l is the r * 32 + l-th of them; kNone: no key).  place[r]
+// becomes the key's place inside its digit's run.  Returns how many of digit threadIdx.x
+// there are; kept = keys in the tile.
+__device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[kItems], const uint32_t (&entry)[kItems],
+                                              uint32_t (&place)[kItems], int rounds, int shift, uint32_t mask,
+                                              uint32_t& kept) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < kWarps * kMaxRadix; i += kThreads) (&sh.cnt[0][0])[i] = 0;
+  __syncthreads();
+  const unsigned lt = (1u << lane) - 1u;
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    if (r >= rounds) break;
+    const uint32_t d = key[r] != kNone ? (key[r] >> shift) & mask : kNone;
+    const unsigned peers = __match_any_sync(0xffffffffu, d);
+    uint32_t before = 0;
+    if (d != kNone) before = sh.cnt[warp][d];
+    place[r] = before + __popc(peers & lt);
+    __syncwarp();
+    if (d != kNone && (peers & lt) == 0) sh.cnt[warp][d] = before + __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  uint32_t run = 0;
+  if (tid < kMaxRadix) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t c = sh.cnt[w][tid];
+      sh.cnt[w][tid] = run;
+      run += c;
+    }
+  }
+  const uint32_t start = scan_256(run, sh.sh, kept);
+  if (tid < kMaxRadix) sh.start[tid] = start;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    if (r >= rounds) break;
+    if (key[r] == kNone) continue;
+    const uint32_t d = (key[r] >> shift) & mask;
+    place[r] += sh.cnt[warp][d];
+    const uint32_t at = sh.start[d] + place[r];
+    sh.key[at] = key[r];
+    sh.entry[at] = entry[r];
+  }
+  __syncthreads();
+  return run;
+}
 
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
                                                                  const uint32_t* __restrict__ n_dev, uint32_t chunk,
                                                                  int shift, int radix,
                                                                  const uint32_t* __restrict__ counts, Target out) {
-  __shared__ uint32_t s_cnt[kWarps][kMaxRadix];
-  __shared__ uint32_t s_base[kMaxRadix];    // place of the chunk's next key with this digit
-  __shared__ uint32_t s_start[kMaxRadix];   // start of the digit inside the tile
-  __shared__ uint32_t s_key[kTile], s_entry[kTile];
-  __shared__ uint32_t sh[9];
+  extern __shared__ __align__(16) unsigned char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (n_dev) n = min(n, *n_dev);
-  // the matrix of counts: threads d and d + 256 add the even and the odd chunks of digit d
-  {
-    uint32_t before = 0, all = 0;
-    const int d = tid & 255;
-    if (d < radix) {
-#pragma unroll 8
-      for (int c = tid >> 8; c < (int)gridDim.x; c += 2) {
-        const uint32_t v = counts[(size_t)c * radix + d];
-        all += v;
-        before += c < (int)blockIdx.x ? v : 0u;
-      }
+  const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
+  const uint32_t mask = radix - 1;
+  uint32_t key[kItems], entry[kItems], place[kItems];
+  int rounds = 0;
+  auto load = [&](uint32_t tile) {
+    const uint32_t len = min(end - tile, (uint32_t)kTile);
+    rounds = (int)((len + kThreads - 1) / kThreads);   // equal runs for the warps
+    const uint32_t base = tile + warp * (32 * rounds) + lane;
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const uint32_t i = base + r * 32;
+      const bool in = r < rounds && i < end;
+      key[r] = in ? source_key(s, i) : kNone;
+      entry[r] = in ? (s.bytes ? i : s.entries[i]) : 0u;
     }
-    if (tid >= 256) s_cnt[0][d] = before, s_cnt[1][d] = all;
+  };
+  if (begin < end) load(begin);   // on its way while the matrix of counts is added up
+  // the matrix of counts: 16 shares of the chunks, four digits per thread
+  {
+    constexpr int kShares = 16, kLoads = (kMaxChunks + kShares - 1) / kShares;
+    const int quads = radix >> 2, share = tid / quads, q = tid - share * quads;
+    uint4* before4 = reinterpret_cast<uint4*>(sh.key);
+    uint4* all4 = reinterpret_cast<uint4*>(sh.entry);
+    if (share < kShares) {
+      uint4 v[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int c = share + i * kShares;
+        v[i] = c < (int)gridDim.x ? reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q] : make_uint4(0, 0, 0, 0);
+      }
+      uint4 before = make_uint4(0, 0, 0, 0), all = before;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        all.x += v[i].x, all.y += v[i].y, all.z += v[i].z, all.w += v[i].w;
+        if (share + i * kShares < (int)blockIdx.x)
+          before.x += v[i].x, before.y += v[i].y, before.z += v[i].z, before.w += v[i].w;
+      }
+      before4[share * quads + q] = before;
+      all4[share * quads + q] = all;
+    }
     __syncthreads();
-    if (tid < 256) before += s_cnt[0][d], all += s_cnt[1][d];
+    uint32_t before = 0, all = 0;
+    if (tid < radix) {
+#pragma unroll
+      for (int i = 0; i < kShares; ++i) before += sh.key[i * radix + tid], all += sh.entry[i * radix + tid];
+    }
     uint32_t total;
-    const uint32_t first = scan_256(tid < 256 ? all : 0u, sh, total);
-    if (tid < 256) s_base[d] = first + before;
+    const uint32_t first = scan_256(all, sh.sh, total);
+    if (tid < kMaxRadix) sh.base[tid] = first + before;
     if (blockIdx.x == 0 && tid == 0 && out.count) *out.count = total;
     if (blockIdx.x == 0 && out.offsets) {
-      if (tid < 256 && tid < out.groups) out.offsets[tid] = (int)first;
+      if (tid < out.groups) out.offsets[tid] = (int)first;
       if (tid == out.groups - 1) out.offsets[out.groups] = (int)(first + all);
     }
   }
-  const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
-  const uint32_t mask = radix - 1;
-  const unsigned lt = (1u << lane) - 1u;
   for (uint32_t tile = begin; tile < end; tile += kTile) {
-    for (int i = tid; i < kWarps * kMaxRadix; i += kThreads) (&s_cnt[0][0])[i] = 0;
-    __syncthreads();
-    // stable ranks inside the warp's run of 32 * kItems keys
-    const uint32_t base = tile + warp * (32 * kItems);
-    uint32_t key[kItems], rank[kItems], digit[kItems];
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const uint32_t i = base + r * 32 + lane;
-      uint32_t k = 0;
-      const bool in = i < end && source_key(s, i, k);
-      key[r] = k;
-      digit[r] = in ? (k >> shift) & mask : 0xffffffffu;
-    }
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const unsigned peers = __match_any_sync(0xffffffffu, digit[r]);
-      const bool in = digit[r] != 0xffffffffu;
-      uint32_t before = 0;
-      if (in) before = s_cnt[warp][digit[r]];
-      rank[r] = before + __popc(peers & lt);
-      __syncwarp();
-      if (in && (peers & lt) == 0) s_cnt[warp][digit[r]] = before + __popc(peers);
-      __syncwarp();
-    }
-    __syncthreads();
-    // per digit: where each warp's keys begin, then where the digit begins in the tile
-    uint32_t run = 0;
-    if (tid < 256) {
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t c = s_cnt[w][tid];
-        s_cnt[w][tid] = run;
-        run += c;
-      }
-    }
+    if (tile != begin) load(tile);
     uint32_t kept;
-    const uint32_t start = scan_256(run, sh, kept);
-    if (tid < 256) s_start[tid] = start;
-    __syncthreads();
+    const uint32_t run = sort_tile(sh, key, entry, place, rounds, shift, mask, kept);
+    if (out.slots) {   // first and only pass: the entries are the items in order
 #pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const uint32_t i = base + r * 32 + lane, d = digit[r];
-      if (d == 0xffffffffu) continue;
-      const uint32_t local = s_cnt[warp][d] + rank[r];
-      const uint32_t e = s.bytes ? i : s.entries[i];
-      s_key[s_start[d] + local] = key[r];
-      s_entry[s_start[d] + local] = e;
-      if (out.slots) out.slots[i] = key[r] < (uint32_t)out.groups ? (int)(s_base[d] + local) : -1;
+      for (int r = 0; r < kItems; ++r)
+        if (key[r] != kNone)
+          out.slots[entry[r]] =
+              key[r] < (uint32_t)out.groups ? (int)(sh.base[(key[r] >> shift) & mask] + place[r]) : -1;
     }
-    __syncthreads();
     // the tile is in digit order: each digit's keys go out as one run
     for (uint32_t i = tid; i < kept; i += kThreads) {
-      const uint32_t k = s_key[i], d = (k >> shift) & mask;
-      const uint32_t at = s_base[d] + i - s_start[d];
+      const uint32_t k = sh.key[i], d = (k >> shift) & mask;
+      const uint32_t at = sh.base[d] + i - sh.start[d];
       if (out.keys) out.keys[at] = k;
-      out.entries[at] = s_entry[i];
+      out.entries[at] = sh.entry[i];
     }
     __syncthreads();
-    if (tid < 256) s_base[tid] += run;
+    if (tid < kMaxRadix) sh.base[tid] += run;
     __syncthreads();
+  }
+}
+
+// All passes on up to kTile keys, in one block.
+__global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t n, int bits, int passes, Target out) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t key[kItems], entry[kItems], place[kItems];
+  uint32_t kept = n;
+  int done = 0;
+  for (int p = 0; p < passes; ++p) {
+    const int width = (bits - done + (passes - p) - 1) / (passes - p);
+    const int rounds = (int)((kept + kThreads - 1) / kThreads);
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const uint32_t i = warp * (32 * rounds) + r * 32 + lane;
+      const bool in = r < rounds && i < kept;
+      key[r] = !in ? kNone : p == 0 ? source_key(s, i) : sh.key[i];
+      entry[r] = !in ? 0u : p == 0 ? i : sh.entry[i];
+    }
+    __syncthreads();
+    sort_tile(sh, key, entry, place, rounds, done, (1u << width) - 1u, kept);
+    done += width;
+  }
+  for (uint32_t i = tid; i < kept; i += kThreads) {
+    const uint32_t k = sh.key[i], e = sh.entry[i];
+    if (out.keys) out.keys[i] = k;
+    out.entries[i] = e;
+    if (out.slots) out.slots[e] = k < (uint32_t)out.groups ? (int)i : -1;
+  }
+  if (tid == 0 && out.count) *out.count = kept;
+  if (out.offsets) {
+    for (long long g = tid; g <= out.groups; g += kThreads) {   // the first key of group g or a later one
+      uint32_t lo = 0, hi = kept;
+      while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (sh.key[mid] < (uint32_t)g) lo = mid + 1;
+        else hi = mid;
+      }
+      out.offsets[g] = (int)lo;
+    }
   }
 }
 
@@ -240,20 +328,32 @@ struct Chunks {
 };
 
 inline Chunks chunks_for(long long n) {
-  // a chunk has 1024 keys at least (two per thread), so small sorts stay on few blocks
-  long long c = (n + 1023) / 1024;
+  // a chunk has a key per thread at least
+  long long c = (n + kThreads - 1) / kThreads;
   if (c > kMaxChunks) c = kMaxChunks;
   if (c < 1) c = 1;
   const long long size = ((n + c - 1) / c + 31) / 32 * 32;
   return {(int)((n + size - 1) / (size > 0 ? size : 1)), (uint32_t)size};
 }
 
+inline int passes_for(int bits) { return (bits + 7) / 8; }
+
 int one_pass(const Source& src, long long n, const uint32_t* n_dev, int shift, int bits, uint32_t* counts, Target out,
              cudaStream_t st) {
   const Chunks c = chunks_for(n);
+  if (bits < 2) bits = 2;   // the counts are read four digits at a time
+  CVHRF_CUDA_TRY(cudaFuncSetAttribute(chunk_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)));
   chunk_count_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << bits, counts);
   CVHRF_LAUNCH_CHECK();
-  chunk_scatter_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << bits, counts, out);
+  chunk_scatter_kernel<<<c.count, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << bits,
+                                                                  counts, out);
+  CVHRF_LAUNCH_CHECK();
+  return CVHRF_OK;
+}
+
+int small_sort(const Source& src, long long n, int bits, Target out, cudaStream_t st) {
+  CVHRF_CUDA_TRY(cudaFuncSetAttribute(small_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)));
+  small_sort_kernel<<<1, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits, passes_for(bits), out);
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;
 }
@@ -271,8 +371,14 @@ int group_sort(const void* index, int index_bytes, long long n, long long rows, 
   uint32_t* k[2] = {counts + (size_t)kMaxChunks * kMaxRadix, nullptr};
   k[1] = k[0] + 2 * len;
   const int bits = bits_for((unsigned long long)rows + (keep_outside ? 1 : 0));
-  const int npass = (bits + 7) / 8;
+  const int npass = passes_for(bits);
   Source src{index, index_bytes, nullptr, nullptr, (uint32_t)rows, keep_outside ? 1 : 0};
+  *count_dev = count;
+  if (n <= kTile) {
+    *keys = k[0];
+    *entries = k[0] + len;
+    return small_sort(src, n, bits, Target{k[0], k[0] + len, nullptr, nullptr, 0, count}, st);
+  }
   int done = 0;
   for (int p = 0; p < npass; ++p) {
     const int width = (bits - done + (npass - p) - 1) / (npass - p);   // the bits left, shared evenly
@@ -285,7 +391,6 @@ int group_sort(const void* index, int index_bytes, long long n, long long rows, 
   }
   *keys = src.keys;
   *entries = src.entries;
-  *count_dev = count;
   return CVHRF_OK;
 }
 
@@ -310,12 +415,14 @@ extern "C" int cvhrf_group_rows(const void* index, int index_bytes, long long en
     return CVHRF_OK;
   }
   if (!workspace || workspace_bytes < cvhrf_group_rows_workspace_bytes(entries, groups)) return CVHRF_EWORKSPACE;
+  if ((uintptr_t)workspace & 15) return CVHRF_EINVAL;
   uint32_t* scratch = (uint32_t*)workspace;
-  if (groups < kMaxRadix) {   // one pass writes everything
-    const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)groups, 1};
-    const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr};
-    return one_pass(src, entries, nullptr, 0, bits_for((unsigned long long)groups + 1), scratch + 64, out, st);
-  }
+  const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)groups, 1};
+  const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr};
+  const int bits = bits_for((unsigned long long)groups + 1);
+  if (entries <= kTile) return small_sort(src, entries, bits, out, st);
+  // up to 255 groups (and the entries left out) one pass writes everything
+  if (groups < kMaxRadix) return one_pass(src, entries, nullptr, 0, bits, scratch + 64, out, st);
   const uint32_t *keys, *sorted, *count;
   const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, st, &keys, &sorted, &count);
   if (rc) return rc;

@@ -9,6 +9,7 @@
 // is owned by a power of two of lanes, up to a warp, that hold its columns, so a row of x or
 // dout is read once however many groups it goes to, and no two owners write to one place.
 // Bound by memory: each touches N + N k rows once.
+#include <type_traits>
 #include "row_groups.cuh"
 #include "row_types.cuh"
 
@@ -25,147 +26,329 @@ struct Moves {
   const int* used;      // (device) places that belong to a group; the rest is behind the last group
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> zero_pack() {
-  Pack<T, VEC> z;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) z.v[i] = from_float<T>(0.f);
-  return z;
-}
-
-// Zeros into the rows behind the last group, shared out between the owners (row n takes
-// every n-th of them, `choices` at most).
-template <typename T, int VEC>
-__device__ __forceinline__ void clear_behind(const Moves& m, long long row, int lane, T* __restrict__ out) {
+// Zeros into the rows behind the last group, shared out between the owners of the rows or the
+// entries (owner x of `owners` takes every `owners`-th of them).
+template <typename T, Layout L>
+__device__ __forceinline__ void clear_behind(const Moves& m, int used, long long x, long long owners, int lane,
+                                             T* __restrict__ out) {
+  using R = Row<T, L>;
   const long long places = m.n * m.choices;
-  for (long long p = *m.used + row; p < places; p += m.n)
-    for (int c = lane * VEC; c < m.width; c += m.lanes * VEC)
-      *(Pack<T, VEC>*)(out + p * m.width + c) = zero_pack<T, VEC>();
+  for (long long p = used + x; p < places; p += owners) {
+    T* to = out + p * m.width;
+    for (int e = lane * R::kVec - R::ahead(to); e < m.width; e += m.lanes * R::kVec)
+      R::store(to, e, m.width, zero_pack<T, L>());
+  }
 }
 
-template <typename T, int VEC>
+// Aligned rows: an owner has ROWS rows (owners apart, so that the owners of a block touch
+// neighbouring rows) with J packs of each in flight; each pack is read once and written once
+// per choice.
+template <typename T, int ROWS, int J>
 __global__ void __launch_bounds__(kThreads) rows_to_groups_kernel(Moves m, const T* __restrict__ x, long long stride,
                                                                   T* __restrict__ out) {
-  const long long row = (long long)blockIdx.x * (kThreads / m.lanes) + threadIdx.x / m.lanes;
-  const int lane = threadIdx.x & (m.lanes - 1);
-  if (row >= m.n) return;
-  const int* slots = m.slots + row * m.choices;
-  for (int c = lane * VEC; c < m.width; c += m.lanes * VEC) {
-    const Pack<T, VEC> p = *(const Pack<T, VEC>*)(x + row * stride + c);
-    for (int j = 0; j < m.choices; ++j) {
-      const int s = slots[j];
-      if (s >= 0) *(Pack<T, VEC>*)(out + (long long)s * m.width + c) = p;
-    }
-  }
-  clear_behind<T, VEC>(m, row, lane, out);
-}
-
-template <typename T, int VEC, typename W>
-__global__ void __launch_bounds__(kThreads) groups_to_rows_kernel(Moves m, const T* __restrict__ y, long long stride,
-                                                                  const W* __restrict__ weights,
-                                                                  T* __restrict__ out) {
-  const long long row = (long long)blockIdx.x * (kThreads / m.lanes) + threadIdx.x / m.lanes;
-  const int lane = threadIdx.x & (m.lanes - 1);
-  if (row >= m.n) return;
-  const int* slots = m.slots + row * m.choices;
-  for (int c = lane * VEC; c < m.width; c += m.lanes * VEC) {
-    float acc[VEC];
+  using R = Row<T, kAligned>;
+  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
+  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
+  const int used = *m.used;
+  for (int c0 = lane * R::kVec; c0 < m.width; c0 += step * J) {
+    uint4 p[ROWS][J];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (first + q * owners < m.n && c0 + j * step < m.width)
+          p[q][j] = *(const uint4*)(x + (first + q * owners) * stride + c0 + j * step);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      const long long row = first + q * owners;
+      if (row < m.n) {
 #pragma unroll 4
-    for (int j = 0; j < m.choices; ++j) {
-      const int s = slots[j];
-      if (s < 0) continue;   // whatever its weight holds
-      const Pack<T, VEC> p = *(const Pack<T, VEC>*)(y + (long long)s * stride + c);
-      const float w = weights ? to_float(weights[row * m.choices + j]) : 1.f;
+        for (int i = 0; i < m.choices; ++i) {
+          const int s = m.slots[row * m.choices + i];
+          if (s < 0) continue;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, to_float(p.v[i]), acc[i]);
-    }
-    Pack<T, VEC> o;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o.v[i] = from_float<T>(acc[i]);
-    *(Pack<T, VEC>*)(out + row * m.width + c) = o;
-  }
-}
-
-template <typename T, int VEC, typename W>
-__global__ void __launch_bounds__(kThreads) groups_to_rows_backward_kernel(
-    Moves m, const T* __restrict__ grad, long long grad_stride, const T* __restrict__ y, long long stride,
-    const W* __restrict__ weights, T* __restrict__ grad_y, W* __restrict__ grad_weights) {
-  const long long row = (long long)blockIdx.x * (kThreads / m.lanes) + threadIdx.x / m.lanes;
-  const int lane = threadIdx.x & (m.lanes - 1);
-  const bool live = row < m.n;
-  const int* slots = m.slots + row * m.choices;
-  for (int j = 0; j < m.choices; ++j) {
-    const int s = live ? slots[j] : -1;
-    float dot = 0.f;
-    if (s >= 0) {
-      const float w = weights ? to_float(weights[row * m.choices + j]) : 1.f;
-#pragma unroll 2
-      for (int c = lane * VEC; c < m.width; c += m.lanes * VEC) {
-        const Pack<T, VEC> g = *(const Pack<T, VEC>*)(grad + row * grad_stride + c);
-        if (grad_weights) {
-          const Pack<T, VEC> p = *(const Pack<T, VEC>*)(y + (long long)s * stride + c);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) dot = fmaf(to_float(g.v[i]), to_float(p.v[i]), dot);
-        }
-        if (grad_y) {
-          Pack<T, VEC> o;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) o.v[i] = from_float<T>(w * to_float(g.v[i]));
-          *(Pack<T, VEC>*)(grad_y + (long long)s * m.width + c) = o;
+          for (int j = 0; j < J; ++j)
+            if (c0 + j * step < m.width) *(uint4*)(out + (long long)s * m.width + c0 + j * step) = p[q][j];
         }
       }
     }
-    if (grad_weights) {
-      for (int o = m.lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if (live && lane == 0) grad_weights[row * m.choices + j] = from_float<W>(dot);
-    }
   }
-  if (live && grad_y) clear_behind<T, VEC>(m, row, lane, grad_y);
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q)
+    if (first + q * owners < m.n) clear_behind<T, kAligned>(m, used, first + q * owners, m.n, lane, out);
 }
 
-struct Launch {
-  Moves m;
-  unsigned blocks;
+// Other rows: packs follow the row that is written, which begins elsewhere for every choice,
+// so each owner copies ENTRIES entries (a row's choices are neighbours: its row is read from
+// DRAM once).
+template <typename T, Layout L, int ENTRIES>
+__global__ void __launch_bounds__(kThreads) entries_to_groups_kernel(Moves m, const T* __restrict__ x, Extent extent,
+                                                                     long long stride, T* __restrict__ out) {
+  using R = Row<T, L>;
+  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
+  const long long entries = m.n * m.choices;
+  const long long first = (long long)blockIdx.x * (owners * ENTRIES) + threadIdx.x / m.lanes;
+  const int used = *m.used;
+  const T* from[ENTRIES];
+  T* to[ENTRIES];
+  int e0[ENTRIES];
+#pragma unroll
+  for (int q = 0; q < ENTRIES; ++q) {
+    const long long e = first + q * owners;
+    const int s = e < entries ? m.slots[e] : -1;
+    from[q] = s >= 0 ? x + (long long)((uint32_t)e / (uint32_t)m.choices) * stride : nullptr;   // entries are below 2^30
+    to[q] = out + (long long)(s >= 0 ? s : 0) * m.width;
+    e0[q] = lane * R::kVec - R::ahead(to[q]);
+  }
+  for (int c = 0; c - (R::kVec - 1) < m.width; c += step) {
+    typename R::Raw p[ENTRIES];
+#pragma unroll
+    for (int q = 0; q < ENTRIES; ++q)
+      if (from[q] && e0[q] + c < m.width) p[q] = R::load(from[q], e0[q] + c, m.width, extent);
+#pragma unroll
+    for (int q = 0; q < ENTRIES; ++q)
+      if (from[q] && e0[q] + c < m.width) R::store(to[q], e0[q] + c, m.width, R::words(p[q]));
+  }
+#pragma unroll
+  for (int q = 0; q < ENTRIES; ++q)
+    if (first + q * owners < entries) clear_behind<T, L>(m, used, first + q * owners, entries, lane, out);
+}
+
+// The weights are float32 or of the rows' type.
+struct Weights {
+  const void* at;   // null: ones
+  bool same;        // of the rows' type
 };
 
-template <int VEC>
-Launch launch_for(long long n, int choices, int width, const int* slots, const int* used) {
-  const int packs = (width + VEC - 1) / VEC;
-  const int lanes = next_pow2(packs < 32 ? packs : 32);
-  const int rows = kThreads / lanes;
-  return {{n, choices, width, lanes, slots, used}, (unsigned)((n + rows - 1) / rows)};
+template <typename T>
+__device__ __forceinline__ float weight_at(const Weights& w, long long e) {
+  if (!w.at) return 1.f;
+  return w.same ? to_float(((const T*)w.at)[e]) : ((const float*)w.at)[e];
 }
 
-template <typename T, int VEC>
-int to_groups(const void* x, long long stride, long long n, int choices, int width, const int* slots, const int* used,
-              void* out, cudaStream_t st) {
-  const Launch l = launch_for<VEC>(n, choices, width, slots, used);
-  rows_to_groups_kernel<T, VEC><<<l.blocks, kThreads, 0, st>>>(l.m, (const T*)x, stride, (T*)out);
-  CVHRF_LAUNCH_CHECK();
-  return CVHRF_OK;
+// Slots and weights of CHOICES choices from i0 on of the owner's rows; a slot is -1 where
+// there is no entry or it is left out.
+template <typename T, int ROWS, int CHOICES>
+__device__ __forceinline__ void load_choices(const Moves& m, const Weights& weights, long long first, int owners, int i0,
+                                             int (&slot)[ROWS][CHOICES], float (&w)[ROWS][CHOICES]) {
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+    for (int i = 0; i < CHOICES; ++i) {
+      const long long row = first + q * owners, e = row * m.choices + i0 + i;
+      const bool in = row < m.n && i0 + i < m.choices;
+      slot[q][i] = in ? m.slots[e] : -1;
+      w[q][i] = in ? weight_at<T>(weights, e) : 0.f;
+    }
 }
 
-template <typename T, int VEC, typename W>
-int to_rows(const void* y, long long stride, long long n, int choices, int width, const int* slots,
-            const void* weights, void* out, cudaStream_t st) {
-  const Launch l = launch_for<VEC>(n, choices, width, slots, nullptr);
-  groups_to_rows_kernel<T, VEC, W><<<l.blocks, kThreads, 0, st>>>(l.m, (const T*)y, stride, (const W*)weights,
-                                                                 (T*)out);
-  CVHRF_LAUNCH_CHECK();
-  return CVHRF_OK;
+// An owner has one pack of CHOICES choices of each of ROWS rows in flight.
+template <typename T, Layout L, int ROWS, int CHOICES>
+__global__ void __launch_bounds__(kThreads, 4) groups_to_rows_kernel(Moves m, const T* __restrict__ y, Extent extent,
+                                                                     long long stride, Weights weights,
+                                                                     T* __restrict__ out) {
+  using R = Row<T, L>;
+  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
+  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
+  int slot[ROWS][CHOICES], e0[ROWS];
+  float w[ROWS][CHOICES];
+  load_choices<T>(m, weights, first, owners, 0, slot, w);
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q) e0[q] = lane * R::kVec - R::ahead(out + (first + q * owners) * m.width);
+  for (int c = 0; c - (L == kSpan ? R::kVec - 1 : 0) < m.width; c += step) {
+    float acc[ROWS][R::kVec];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int v = 0; v < R::kVec; ++v) acc[q][v] = 0.f;
+    for (int i0 = 0; i0 < m.choices; i0 += CHOICES) {
+      if (m.choices > CHOICES) load_choices<T>(m, weights, first, owners, i0, slot, w);
+      typename R::Raw p[ROWS][CHOICES];
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i)
+          if (slot[q][i] >= 0 && e0[q] + c < m.width)
+            p[q][i] = R::load(y + (long long)slot[q][i] * stride, e0[q] + c, m.width, extent);
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i)
+          if (slot[q][i] >= 0 && e0[q] + c < m.width) {   // an entry left out counts nothing, whatever its weight holds
+            float f[R::kVec];
+            R::floats(p[q][i], f);
+#pragma unroll
+            for (int v = 0; v < R::kVec; ++v) acc[q][v] = fmaf(w[q][i], f[v], acc[q][v]);
+          }
+    }
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+      if (first + q * owners < m.n && e0[q] + c < m.width)
+        R::store(out + (first + q * owners) * m.width, e0[q] + c, m.width, R::words(acc[q]));
+  }
 }
 
-template <typename T, int VEC, typename W>
-int to_rows_backward(const void* grad, long long grad_stride, const void* y, long long stride, long long n,
-                     int choices, int width, const int* slots, const int* used, const void* weights, void* grad_y,
-                     void* grad_weights, cudaStream_t st) {
-  const Launch l = launch_for<VEC>(n, choices, width, slots, used);
-  groups_to_rows_backward_kernel<T, VEC, W><<<l.blocks, kThreads, 0, st>>>(
-      l.m, (const T*)grad, grad_stride, (const T*)y, stride, (const W*)weights, (T*)grad_y, (W*)grad_weights);
-  CVHRF_LAUNCH_CHECK();
-  return CVHRF_OK;
+// Packs follow the row of grad_y that is written (with unaligned rows each choice's begins
+// elsewhere, so the row of grad is read again for it, from L1).
+template <typename T, Layout L, int ROWS, int CHOICES>
+__global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
+    Moves m, const T* __restrict__ grad, Extent grad_extent, long long grad_stride, const T* __restrict__ y,
+    Extent extent, long long stride, Weights weights, T* __restrict__ grad_y, void* __restrict__ grad_weights) {
+  using R = Row<T, L>;
+  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
+  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
+  for (int i0 = 0; i0 < m.choices; i0 += CHOICES) {
+    int slot[ROWS][CHOICES], e0[ROWS][CHOICES];
+    float w[ROWS][CHOICES], dot[ROWS][CHOICES];
+    load_choices<T>(m, weights, first, owners, i0, slot, w);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int i = 0; i < CHOICES; ++i) {
+        dot[q][i] = 0.f;
+        e0[q][i] = lane * R::kVec - (grad_y ? R::ahead(grad_y + (long long)slot[q][i] * m.width) : 0);
+      }
+    for (int c = 0; c - (L == kSpan ? R::kVec - 1 : 0) < m.width; c += step) {
+      typename R::Raw g[ROWS][L == kSpan ? CHOICES : 1], p[ROWS][CHOICES];
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+        const T* row = grad + (first + q * owners) * grad_stride;
+        if (L != kSpan && first + q * owners < m.n && e0[q][0] + c < m.width)
+          g[q][0] = R::load(row, e0[q][0] + c, m.width, grad_extent);
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i)
+          if (slot[q][i] >= 0 && e0[q][i] + c < m.width) {
+            if (L == kSpan) g[q][L == kSpan ? i : 0] = R::load(row, e0[q][i] + c, m.width, grad_extent);
+            if (grad_weights) p[q][i] = R::load(y + (long long)slot[q][i] * stride, e0[q][i] + c, m.width, extent);
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i) {
+          const int e = e0[q][i] + c;
+          if (slot[q][i] >= 0 && e < m.width) {
+            float f[R::kVec];
+            R::floats(g[q][L == kSpan ? i : 0], f);
+            if (grad_weights) {
+              float h[R::kVec];
+              R::floats(p[q][i], h);
+#pragma unroll
+              for (int v = 0; v < R::kVec; ++v)
+                if (L != kSpan || (e + v >= 0 && e + v < m.width)) dot[q][i] = fmaf(f[v], h[v], dot[q][i]);
+            }
+            if (grad_y) {
+#pragma unroll
+              for (int v = 0; v < R::kVec; ++v) f[v] *= w[q][i];
+              R::store(grad_y + (long long)slot[q][i] * m.width, e, m.width, R::words(f));
+            }
+          }
+        }
+    }
+    if (grad_weights) {
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i) {
+          float d = dot[q][i];
+          for (int o = m.lanes >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          const long long row = first + q * owners, e = row * m.choices + i0 + i;
+          if (lane == 0 && row < m.n && i0 + i < m.choices) {
+            if (weights.same) ((T*)grad_weights)[e] = from_float<T>(d);
+            else ((float*)grad_weights)[e] = d;
+          }
+        }
+    }
+  }
+  if (grad_y) {
+    const int used = *m.used;
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+      if (first + q * owners < m.n) clear_behind<T, L>(m, used, first + q * owners, m.n, lane, grad_y);
+  }
+}
+
+// Lanes that own a row of `packs` packs, and the blocks for `rows` rows per owner.
+inline int lanes_for(int packs) { return next_pow2(packs < 32 ? packs : 32); }
+inline unsigned blocks_for(long long n, int lanes, int rows) {
+  const int per_block = kThreads / lanes * rows;
+  return (unsigned)((n + per_block - 1) / per_block);
+}
+
+// Calls f<layout>(lanes) for rows that are all aligned, and for others by their width.
+template <typename T, typename F>
+int with_layout(bool aligned, int width, F f) {
+  if (aligned) return f(std::integral_constant<Layout, kAligned>(), lanes_for(packs_of<T, kAligned>(width)));
+  if (width >= kSpanWidth) return f(std::integral_constant<Layout, kSpan>(), lanes_for(packs_of<T, kSpan>(width)));
+  return f(std::integral_constant<Layout, kElement>(), lanes_for(width));
+}
+
+template <typename T>
+int to_groups(bool aligned, const void* x, long long stride, Moves m, void* out, cudaStream_t st) {
+  return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
+    constexpr Layout L = decltype(layout)::value;
+    m.lanes = lanes;
+    const T* from = (const T*)x;
+    if constexpr (L == kAligned) {
+      const int packs = packs_of<T, L>(m.width);
+      if (packs > 64) rows_to_groups_kernel<T, 1, 4><<<blocks_for(m.n, lanes, 1), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      else if (packs > 32) rows_to_groups_kernel<T, 2, 2><<<blocks_for(m.n, lanes, 2), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      else rows_to_groups_kernel<T, 4, 1><<<blocks_for(m.n, lanes, 4), kThreads, 0, st>>>(m, from, stride, (T*)out);
+    } else {
+      constexpr int kEntries = L == kSpan ? 2 : 4;
+      entries_to_groups_kernel<T, L, kEntries><<<blocks_for(m.n * m.choices, lanes, kEntries), kThreads, 0, st>>>(
+          m, from, extent_of(x, m.n, stride, m.width, sizeof(T)), stride, (T*)out);
+    }
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  });
+}
+
+template <typename T>
+int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weights, void* out, cudaStream_t st) {
+  return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
+    constexpr Layout L = decltype(layout)::value;
+    m.lanes = lanes;
+    const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
+#define CVHRF_LAUNCH(ROWS, CHOICES)                                                               \
+  groups_to_rows_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, lanes, ROWS), kThreads, 0, st>>>(  \
+      m, (const T*)y, extent, stride, weights, (T*)out)
+    if constexpr (L == kSpan) {   // twice the registers per pack
+      if (m.choices > 1) CVHRF_LAUNCH(1, 2);
+      else CVHRF_LAUNCH(2, 1);
+    } else {
+      if (m.choices > 2) CVHRF_LAUNCH(1, 4);
+      else if (m.choices > 1) CVHRF_LAUNCH(2, 2);
+      else CVHRF_LAUNCH(4, 1);
+    }
+#undef CVHRF_LAUNCH
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  });
+}
+
+template <typename T>
+int to_rows_backward(bool aligned, const void* grad, long long grad_stride, const void* y, long long stride, Moves m,
+                     Weights weights, void* grad_y, void* grad_weights, cudaStream_t st) {
+  return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
+    constexpr Layout L = decltype(layout)::value;
+    m.lanes = lanes;
+    const Extent grad_extent = extent_of(grad, m.n, grad_stride, m.width, sizeof(T));
+    const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
+#define CVHRF_LAUNCH(ROWS, CHOICES)                                                                        \
+  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, lanes, ROWS), kThreads, 0, st>>>(  \
+      m, (const T*)grad, grad_extent, grad_stride, (const T*)y, extent, stride, weights, (T*)grad_y, grad_weights)
+    if constexpr (L == kSpan) {   // four times: the pack of grad and of y
+      CVHRF_LAUNCH(1, 1);
+    } else {
+      if (m.choices > 2) CVHRF_LAUNCH(1, 4);
+      else if (m.choices > 1) CVHRF_LAUNCH(2, 2);
+      else CVHRF_LAUNCH(4, 1);
+    }
+#undef CVHRF_LAUNCH
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  });
 }
 
 int check_moves(int dtype, long long n, int choices, int width) {
@@ -174,18 +357,17 @@ int check_moves(int dtype, long long n, int choices, int width) {
   return CVHRF_OK;
 }
 
-// CALL<type, packed>(...) for the element type and whether rows move 16 bytes at a time
-#define CVHRF_ROW_DISPATCH(dtype, wide, CALL32, CALL32W, CALLB, CALLBW, CALLH, CALLHW) \
-  (dtype == CVHRF_F32    ? (wide ? CALL32W : CALL32)                                   \
-   : dtype == CVHRF_BF16 ? (wide ? CALLBW : CALLB)                                     \
-                         : (wide ? CALLHW : CALLH))
+template <typename F>
+int with_type(int dtype, F f) {
+  if (dtype == CVHRF_F32) return f(float());
+  if (dtype == CVHRF_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
 
 }  // namespace
 }  // namespace cvhrf
 
 using namespace cvhrf;
-using bf16 = __nv_bfloat16;
-using f16 = __half;
 
 extern "C" int cvhrf_rows_to_groups(const void* x, long long x_stride, int dtype, long long n, int choices, int width,
                                     const int* slots, const int* used, void* out, void* stream) {
@@ -194,12 +376,11 @@ extern "C" int cvhrf_rows_to_groups(const void* x, long long x_stride, int dtype
   if (x_stride < 0) return CVHRF_EINVAL;
   if (n == 0) return CVHRF_OK;
   if (!x || !slots || !used || !out) return CVHRF_EINVAL;
-  const bool wide = rows_16(x, x_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
-  cudaStream_t st = (cudaStream_t)stream;
-#define CVHRF_CALL(T, V) to_groups<T, V>(x, x_stride, n, choices, width, slots, used, out, st)
-  return CVHRF_ROW_DISPATCH(dtype, wide, CVHRF_CALL(float, 1), CVHRF_CALL(float, 4), CVHRF_CALL(bf16, 1),
-                            CVHRF_CALL(bf16, 8), CVHRF_CALL(f16, 1), CVHRF_CALL(f16, 8));
-#undef CVHRF_CALL
+  const bool aligned = rows_16(x, x_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
+  const Moves m{n, choices, width, 0, slots, used};
+  return with_type(dtype, [&](auto type) {
+    return to_groups<decltype(type)>(aligned, x, x_stride, m, out, (cudaStream_t)stream);
+  });
 }
 
 extern "C" int cvhrf_groups_to_rows(const void* y, long long y_stride, int dtype, long long n, int choices, int width,
@@ -210,14 +391,12 @@ extern "C" int cvhrf_groups_to_rows(const void* y, long long y_stride, int dtype
   if (y_stride < 0 || (weights && weights_dtype != CVHRF_F32 && weights_dtype != dtype)) return CVHRF_EINVAL;
   if (n == 0) return CVHRF_OK;
   if (!y || !slots || !out) return CVHRF_EINVAL;
-  const bool wide = rows_16(y, y_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
-  cudaStream_t st = (cudaStream_t)stream;
-#define CVHRF_CALL(T, V)                                                                                     \
-  (!weights || weights_dtype == CVHRF_F32 ? to_rows<T, V, float>(y, y_stride, n, choices, width, slots, weights, out, st) \
-                                          : to_rows<T, V, T>(y, y_stride, n, choices, width, slots, weights, out, st))
-  return CVHRF_ROW_DISPATCH(dtype, wide, CVHRF_CALL(float, 1), CVHRF_CALL(float, 4), CVHRF_CALL(bf16, 1),
-                            CVHRF_CALL(bf16, 8), CVHRF_CALL(f16, 1), CVHRF_CALL(f16, 8));
-#undef CVHRF_CALL
+  const bool aligned = rows_16(y, y_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
+  const Moves m{n, choices, width, 0, slots, nullptr};
+  const Weights w{weights, weights && weights_dtype == dtype};
+  return with_type(dtype, [&](auto type) {
+    return to_rows<decltype(type)>(aligned, y, y_stride, m, w, out, (cudaStream_t)stream);
+  });
 }
 
 extern "C" int cvhrf_groups_to_rows_backward(const void* grad, long long grad_stride, const void* y,
@@ -232,16 +411,12 @@ extern "C" int cvhrf_groups_to_rows_backward(const void* grad, long long grad_st
   if (n == 0 || (!grad_y && !grad_weights)) return CVHRF_OK;
   if (!grad || !slots || !used || (grad_weights && !y)) return CVHRF_EINVAL;
   const size_t elem = row_type_bytes(dtype);
-  const bool wide = rows_16(grad, grad_stride, width, elem) && (!grad_weights || rows_16(y, y_stride, width, elem)) &&
-                    ((uintptr_t)grad_y & 15) == 0;
-  cudaStream_t st = (cudaStream_t)stream;
-#define CVHRF_CALL(T, V)                                                                                        \
-  (!weights || weights_dtype == CVHRF_F32                                                                       \
-       ? to_rows_backward<T, V, float>(grad, grad_stride, y, y_stride, n, choices, width, slots, used, weights, \
-                                       grad_y, grad_weights, st)                                                \
-       : to_rows_backward<T, V, T>(grad, grad_stride, y, y_stride, n, choices, width, slots, used, weights,     \
-                                   grad_y, grad_weights, st))
-  return CVHRF_ROW_DISPATCH(dtype, wide, CVHRF_CALL(float, 1), CVHRF_CALL(float, 4), CVHRF_CALL(bf16, 1),
-                            CVHRF_CALL(bf16, 8), CVHRF_CALL(f16, 1), CVHRF_CALL(f16, 8));
-#undef CVHRF_CALL
+  const bool aligned = rows_16(grad, grad_stride, width, elem) &&
+                       (!grad_weights || rows_16(y, y_stride, width, elem)) && ((uintptr_t)grad_y & 15) == 0;
+  const Moves m{n, choices, width, 0, slots, used};
+  const Weights w{weights, weights && weights_dtype == dtype};
+  return with_type(dtype, [&](auto type) {
+    return to_rows_backward<decltype(type)>(aligned, grad, grad_stride, y, y_stride, m, w, grad_y, grad_weights,
+                                            (cudaStream_t)stream);
+  });
 }

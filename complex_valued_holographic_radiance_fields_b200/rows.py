@@ -26,8 +26,7 @@ reference, whose Gaussians own all their attributes, has no counterpart.
 """
 import torch
 
-from . import _lib
-from .profiling import timed
+from . import _lib, profiling
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
@@ -35,39 +34,45 @@ _MAX_ENTRIES = 2 ** 30 - 1
 _MAX_WIDTH = 2 ** 20
 
 
-def _call(name, device, *args):
-    """One libcvhrf call on `device` and its current stream."""
-    f = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = f(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(name, what, device, *args):
+    """One libcvhrf call on `device` and its current stream, timed as `what`."""
+    at = device.index
+    if profiling._active is not None or at != torch._C._cuda_getDevice():
+        with torch.cuda.device(device), profiling.timed(what):
+            rc = getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream)
     else:
-        with torch.cuda.device(device):
-            rc = f(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = getattr(_lib._lib or _lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(at))
     if rc:
         _lib.check(rc, name)
 
 
 def _rows(t, name):
-    """A 2-D tensor of rows whose elements are adjacent, and the elements between its rows."""
-    if t.dtype not in _TYPES:
+    """A 2-D tensor of rows whose elements are adjacent, its type's code, width and the
+    elements between its rows."""
+    code = _TYPES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dim() != 2 or not 1 <= t.shape[1] <= _MAX_WIDTH:
         raise ValueError(f"{name} must be rows x width with 1 <= width <= {_MAX_WIDTH}, got {tuple(t.shape)}")
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        t = t.contiguous()
-    return t, t.stride(0)
+    stride, one = t.stride()
+    width = t.shape[1]
+    if one != 1 and width > 1:
+        t, stride = t.contiguous(), width
+    return t, code, width, stride
 
 
-def _index(index, device, name="index"):
-    if index.dtype not in _INDEX_BYTES:
-        raise TypeError(f"{name} must be int32 or int64, got {index.dtype}")
+def _index(index, device):
+    nbytes = _INDEX_BYTES.get(index.dtype)
+    if nbytes is None:
+        raise TypeError(f"index must be int32 or int64, got {index.dtype}")
     if index.device != device:
-        raise ValueError(f"{name} must be on {device}, got {index.device}")
-    if index.numel() > _MAX_ENTRIES:
-        raise ValueError(f"{name} has {index.numel()} entries: {_MAX_ENTRIES} at most")
-    return index.contiguous()
+        raise ValueError(f"index must be on {device}, got {index.device}")
+    n = index.numel()
+    if n > _MAX_ENTRIES:
+        raise ValueError(f"index has {n} entries: {_MAX_ENTRIES} at most")
+    return index.contiguous(), nbytes, n
 
 
 def _scale(scale):
@@ -78,30 +83,29 @@ def _scale(scale):
 
 # ---- shared rows ----------------------------------------------------------------------
 def _lookup(table, index, scale):
-    table, stride = _rows(table, "table")
-    index = _index(index, table.device)
-    rows, width = table.shape
-    out = torch.empty(*index.shape, width, dtype=table.dtype, device=table.device)
-    with timed("table_lookup"):
-        _call("cvhrf_table_lookup", table.device, table.data_ptr(), rows, width, stride, _TYPES[table.dtype],
-              index.data_ptr(), _INDEX_BYTES[index.dtype], index.numel(), scale, out.data_ptr())
+    table, code, width, stride = _rows(table, "table")
+    device = table.device
+    index, nbytes, n = _index(index, device)
+    out = torch.empty((*index.shape, width), dtype=table.dtype, device=device)
+    _call("cvhrf_table_lookup", "table_lookup", device, table.data_ptr(), table.shape[0], width, stride, code,
+          index.data_ptr(), nbytes, n, scale, out.data_ptr())
     return out
 
 
 def _gradient(grad, index, num_rows, scale, with_mask):
-    width = grad.shape[-1]
-    grad, stride = _rows(grad.reshape(-1, width), "grad")
+    if grad.dim() != 2:
+        if not grad.shape or grad.shape[-1] < 1:
+            raise ValueError(f"grad must have rows of 1 element or more, got {tuple(grad.shape)}")
+        grad = grad.reshape(-1, grad.shape[-1])
+    grad, code, width, stride = _rows(grad, "grad")
     device = grad.device
-    index = _index(index, device)
-    n = index.numel()
-    out = torch.empty(num_rows, width, dtype=grad.dtype, device=device)
+    index, nbytes, n = _index(index, device)
+    out = torch.empty((num_rows, width), dtype=grad.dtype, device=device)
     mask = torch.empty(num_rows, dtype=torch.uint8, device=device) if with_mask else None
-    nbytes = _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with timed("table_gradient"):
-        _call("cvhrf_table_gradient", device, grad.data_ptr(), stride, _TYPES[grad.dtype], width, index.data_ptr(),
-              _INDEX_BYTES[index.dtype], n, scale, out.data_ptr(), num_rows, mask.data_ptr() if with_mask else None,
-              ws.data_ptr(), nbytes)
+    need = _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call("cvhrf_table_gradient", "table_gradient", device, grad.data_ptr(), stride, code, width, index.data_ptr(),
+          nbytes, n, scale, out.data_ptr(), num_rows, mask.data_ptr() if with_mask else None, ws.data_ptr(), need)
     return out, mask
 
 
@@ -128,18 +132,17 @@ def table_lookup(table, index, scale=1.0):
     return _lookup(table, index, scale)
 
 
-@torch.no_grad()
 def table_gradient(grad, index, num_rows, scale=1.0):
     """The gradient of ``table_lookup`` with respect to its table of `num_rows` rows: row v is
     scale times the sum of grad[t] over the entries with index[t] = v.  grad has the
     lookup's shape (*index.shape, D).  Returns (gradient (num_rows, D) in grad's type,
     row_mask (num_rows,) uint8: 1 where an entry names the row), so that
     ``SparseGaussianAdam.step(row_mask=row_mask)`` updates the rows that were used."""
-    if grad.dim() < 1 or grad.shape[:-1] != index.shape:
+    if grad.shape[:-1] != index.shape or not grad.shape:
         raise ValueError(f"grad must have the shape {tuple(index.shape)} and a row's width, got {tuple(grad.shape)}")
     if not 0 <= num_rows < 2 ** 31 - 1:
         raise ValueError(f"num_rows must be in [0, 2^31 - 1), got {num_rows}")
-    return _gradient(grad, index, num_rows, _scale(scale), True)
+    return _gradient(grad.detach(), index, num_rows, _scale(scale), True)
 
 
 # ---- rows by group --------------------------------------------------------------------
@@ -168,35 +171,37 @@ def group_rows(index, num_groups):
     if not 1 <= num_groups < 2 ** 31 - 1:
         raise ValueError(f"num_groups must be in [1, 2^31 - 1), got {num_groups}")
     device = index.device
-    index = _index(index, device)
-    n = index.numel()
+    shape = index.shape
+    index, nbytes, n = _index(index, device)
     order = torch.empty(n, dtype=torch.int32, device=device)
-    slots = torch.empty(index.shape, dtype=torch.int32, device=device)
+    slots = torch.empty(shape, dtype=torch.int32, device=device)
     offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
-    nbytes = _lib.lib().cvhrf_group_rows_workspace_bytes(n, num_groups)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with timed("group_rows"):
-        _call("cvhrf_group_rows", device, index.data_ptr(), _INDEX_BYTES[index.dtype], n, num_groups,
-              order.data_ptr(), slots.data_ptr(), offsets.data_ptr(), ws.data_ptr(), nbytes)
-    return RowGroups(order, slots, offsets, num_groups, index.shape[0], index.shape[1] if index.dim() == 2 else 1)
+    need = _lib.lib().cvhrf_group_rows_workspace_bytes(n, num_groups)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call("cvhrf_group_rows", "group_rows", device, index.data_ptr(), nbytes, n, num_groups, order.data_ptr(),
+          slots.data_ptr(), offsets.data_ptr(), ws.data_ptr(), need)
+    return RowGroups(order, slots, offsets, num_groups, shape[0], shape[1] if len(shape) == 2 else 1)
 
 
 def _to_groups(x, groups):
-    x, stride = _rows(x, "x")
-    out = torch.empty(groups.num_rows * groups.choices, x.shape[1], dtype=x.dtype, device=x.device)
-    with timed("rows_to_groups"):
-        _call("cvhrf_rows_to_groups", x.device, x.data_ptr(), stride, _TYPES[x.dtype], groups.num_rows,
-              groups.choices, x.shape[1], groups.slots.data_ptr(), groups._used(), out.data_ptr())
+    x, code, width, stride = _rows(x, "x")
+    device, n, k = x.device, groups.num_rows, groups.choices
+    out = torch.empty((n * k, width), dtype=x.dtype, device=device)
+    _call("cvhrf_rows_to_groups", "rows_to_groups", device, x.data_ptr(), stride, code, n, k, width,
+          groups.slots.data_ptr(), groups._used(), out.data_ptr())
     return out
 
 
+def _weights(weights):
+    return (None, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
+
+
 def _to_rows(y, groups, weights):
-    y, stride = _rows(y, "y")
-    out = torch.empty(groups.num_rows, y.shape[1], dtype=y.dtype, device=y.device)
-    with timed("groups_to_rows"):
-        _call("cvhrf_groups_to_rows", y.device, y.data_ptr(), stride, _TYPES[y.dtype], groups.num_rows,
-              groups.choices, y.shape[1], groups.slots.data_ptr(), None if weights is None else weights.data_ptr(),
-              0 if weights is None else _TYPES[weights.dtype], out.data_ptr())
+    y, code, width, stride = _rows(y, "y")
+    device, n = y.device, groups.num_rows
+    out = torch.empty((n, width), dtype=y.dtype, device=device)
+    _call("cvhrf_groups_to_rows", "groups_to_rows", device, y.data_ptr(), stride, code, n, groups.choices, width,
+          groups.slots.data_ptr(), *_weights(weights), out.data_ptr())
     return out
 
 
@@ -222,17 +227,16 @@ class GroupsToRows(torch.autograd.Function):
     def backward(ctx, grad):
         y, weights = ctx.saved_tensors
         groups = ctx.groups
-        grad, grad_stride = _rows(grad, "grad")
-        y, stride = _rows(y, "y")
+        grad, code, width, grad_stride = _rows(grad, "grad")
+        y, _, _, stride = _rows(y, "y")
+        device = y.device
         need_y, _, need_w = ctx.needs_input_grad
-        grad_y = torch.empty(y.shape, dtype=y.dtype, device=y.device) if need_y else None
+        grad_y = torch.empty(y.shape, dtype=y.dtype, device=device) if need_y else None
         grad_w = torch.empty_like(weights) if need_w else None
-        with timed("groups_to_rows_backward"):
-            _call("cvhrf_groups_to_rows_backward", y.device, grad.data_ptr(), grad_stride, y.data_ptr(), stride,
-                  _TYPES[y.dtype], groups.num_rows, groups.choices, y.shape[1], groups.slots.data_ptr(),
-                  groups._used(), None if weights is None else weights.data_ptr(),
-                  0 if weights is None else _TYPES[weights.dtype], grad_y.data_ptr() if need_y else None,
-                  grad_w.data_ptr() if need_w else None)
+        _call("cvhrf_groups_to_rows_backward", "groups_to_rows_backward", device, grad.data_ptr(), grad_stride,
+              y.data_ptr(), stride, code, groups.num_rows, groups.choices, width, groups.slots.data_ptr(),
+              groups._used(), *_weights(weights), grad_y.data_ptr() if need_y else None,
+              grad_w.data_ptr() if need_w else None)
         return grad_y, None, grad_w
 
 
