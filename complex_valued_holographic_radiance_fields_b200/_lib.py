@@ -5,6 +5,7 @@ loaded, every operator raises instead of falling back to another path.
 """
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -96,21 +97,14 @@ SIGNATURES = {
     "cvhrf_density_classify": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cvhrf_density_apply": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "cvhrf_opacity_regularization": (c_int, [c_void_p, c_int, c_float, c_void_p, c_void_p]),
-    "cvhrf_table_lookup": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_void_p, c_int, c_longlong,
-                                   c_float, c_void_p, c_void_p]),
+    "cvhrf_table_lookup": (c_int, [ctypes.c_char_p, c_void_p]),
     "cvhrf_table_gradient_workspace_bytes": (c_size_t, [c_longlong, c_longlong, c_int]),
-    "cvhrf_table_gradient": (c_int, [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_longlong, c_float,
-                                     c_void_p, c_longlong, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cvhrf_table_gradient": (c_int, [ctypes.c_char_p, c_void_p]),
     "cvhrf_group_rows_workspace_bytes": (c_size_t, [c_longlong, c_int]),
-    "cvhrf_group_rows": (c_int, [c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                                 c_size_t, c_void_p]),
-    "cvhrf_rows_to_groups": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
-                                     c_void_p, c_void_p]),
-    "cvhrf_groups_to_rows": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
-                                     c_int, c_void_p, c_void_p]),
-    "cvhrf_groups_to_rows_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_longlong, c_int,
-                                              c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
-                                              c_void_p]),
+    "cvhrf_group_rows": (c_int, [ctypes.c_char_p, c_void_p]),
+    "cvhrf_rows_to_groups": (c_int, [ctypes.c_char_p, c_void_p]),
+    "cvhrf_groups_to_rows": (c_int, [ctypes.c_char_p, c_void_p]),
+    "cvhrf_groups_to_rows_backward": (c_int, [ctypes.c_char_p, c_void_p]),
 }
 
 
@@ -157,6 +151,15 @@ class RasterScene(ctypes.Structure):
                [(n, c_float) for n in ("fx", "fy", "px", "py", "near_plane", "far_plane")] + \
                [(n, c_void_p) for n in ("cam_means", "z_vals", "quats", "scales", "colours", "phase", "opacities",
                                         "plane_probs", "view_matrix")]
+
+
+# Argument structs of the row operators (include/cvhrf.h), packed: their calls are short, and a
+# ctypes.Structure takes longer to fill than some of them to run.
+LOOKUP_ARGS = struct.Struct("@PPPqqqiiif")            # cvhrf_lookup_args
+GRADIENT_ARGS = struct.Struct("@PPPPPNqqqiiif")       # cvhrf_gradient_args
+GROUP_ARGS = struct.Struct("@PPPPPNqii")              # cvhrf_group_args
+MOVES_ARGS = struct.Struct("@PPPPPPqqiiii")            # cvhrf_moves_args
+MOVES_BACKWARD_ARGS = struct.Struct("@PPPPPPPPqqqiiii")  # cvhrf_moves_backward_args
 
 
 class CvhrfError(RuntimeError):

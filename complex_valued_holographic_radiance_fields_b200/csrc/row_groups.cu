@@ -1,10 +1,10 @@
 // Integer indices sorted stably by value (see row_groups.cuh), and cvhrf_group_rows.
 //
-// LSD radix sort, digits of at most 8 bits, the bits shared evenly between the passes.  A
-// pass is two launches: chunk_count_kernel counts the digits of each contiguous chunk of
-// keys into a chunk x digit matrix, and chunk_scatter_kernel reads that matrix, adds up
-// what lies before its own chunk, and writes each key to its place.  No block waits for
-// another one and nothing has to be cleared beforehand, so a sort is 2 launches per pass.
+// LSD radix sort, digits of at most 8 bits, the bits shared evenly between the passes.
+// chunk_count_kernel counts the first digits of each contiguous chunk of keys into a chunk x
+// digit matrix; each pass (chunk_scatter_kernel) reads its matrix, adds up what lies before
+// its own chunk, writes each key to its place, and counts the key's next digit for the chunk
+// it goes to.  No block waits for another one, and a sort is 1 launch more than its passes.
 // (A look-back between tiles, as in scan_sort.cu, needs a cleared status array, one more
 // launch for the histogram, and a walk over the earlier tiles in L2 latency.)
 // The first pass reads the caller's indices as they are (4 or 8 bytes).
@@ -13,6 +13,7 @@
 // registers, so a pass is a handful of dependent steps.  Up to 8192 keys in all, one block
 // does every pass in shared memory (small_sort_kernel, one launch).
 #include "row_groups.cuh"
+#include "row_types.cuh"
 
 namespace cvhrf {
 namespace {
@@ -38,6 +39,8 @@ struct Target {
   int* offsets;        // ... and where each of the `groups` groups begins, and the last one ends
   int groups;
   uint32_t* count;     // number of sorted items
+  uint32_t* next;      // where the next pass counts: chunk x next_radix; null: last pass
+  int next_shift, next_radix;
 };
 
 // Key of item i, kNone if it is left out (keys are below 2^31).
@@ -48,14 +51,16 @@ __device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
   return v < s.rows ? (uint32_t)v : (s.keep ? s.rows : kNone);
 }
 
-// counts[chunk][digit] over the keys of each chunk.
-__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, const uint32_t* __restrict__ n_dev,
-                                                               uint32_t chunk, int shift, int radix,
-                                                               uint32_t* __restrict__ counts) {
+// counts[chunk][digit] over the keys of each chunk; the `clear` words behind the matrix, where
+// the later passes count, are set to zero.
+__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, uint32_t chunk, int shift, int radix,
+                                                               uint32_t* __restrict__ counts, int clear) {
+  let_next_start();
   constexpr int kCopies = 8;   // histograms, so that equal digits of different warps do not meet
   __shared__ uint32_t h[kCopies][kMaxRadix];
-  if (n_dev) n = min(n, *n_dev);
   for (int i = threadIdx.x; i < kCopies * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < clear; i += gridDim.x * kThreads)
+    counts[(size_t)gridDim.x * radix + i] = 0;
   __syncthreads();
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   uint32_t* mine = h[(threadIdx.x >> 5) % kCopies];
@@ -120,8 +125,9 @@ __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, u
 // becomes the key's place inside its digit's run.  Returns how many of digit threadIdx.x
 // there are; kept = keys in the tile.
 __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[kItems], const uint32_t (&entry)[kItems],
-                                              uint32_t (&place)[kItems], int rounds, int shift, uint32_t mask,
+                                              uint32_t (&place)[kItems], int rounds, int shift, int width,
                                               uint32_t& kept) {
+  const uint32_t mask = (1u << width) - 1u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i < kWarps * kMaxRadix; i += kThreads) (&sh.cnt[0][0])[i] = 0;
   __syncthreads();
@@ -129,13 +135,20 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
 #pragma unroll
   for (int r = 0; r < kItems; ++r) {
     if (r >= rounds) break;
-    const uint32_t d = key[r] != kNone ? (key[r] >> shift) & mask : kNone;
-    const unsigned peers = __match_any_sync(0xffffffffu, d);
+    const bool in = key[r] != kNone;
+    const uint32_t d = (key[r] >> shift) & mask;
+    // the lanes with the same digit, bit by bit (__match_any_sync takes a step per distinct digit)
+    unsigned peers = __ballot_sync(0xffffffffu, in);
+    for (int b = 0; b < width; ++b) {
+      const bool one = (d >> b) & 1u;
+      const unsigned ones = __ballot_sync(0xffffffffu, one);
+      peers &= one ? ones : ~ones;
+    }
     uint32_t before = 0;
-    if (d != kNone) before = sh.cnt[warp][d];
+    if (in) before = sh.cnt[warp][d];
     place[r] = before + __popc(peers & lt);
     __syncwarp();
-    if (d != kNone && (peers & lt) == 0) sh.cnt[warp][d] = before + __popc(peers);
+    if (in && (peers & lt) == 0) sh.cnt[warp][d] = before + __popc(peers);
     __syncwarp();
   }
   __syncthreads();
@@ -172,6 +185,8 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  follow();
+  let_next_start();
   if (n_dev) n = min(n, *n_dev);
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   const uint32_t mask = radix - 1;
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
   for (uint32_t tile = begin; tile < end; tile += kTile) {
     if (tile != begin) load(tile);
     uint32_t kept;
-    const uint32_t run = sort_tile(sh, key, entry, place, rounds, shift, mask, kept);
+    const uint32_t run = sort_tile(sh, key, entry, place, rounds, shift, 31 - __clz(radix), kept);
     if (out.slots) {   // first and only pass: the entries are the items in order
 #pragma unroll
       for (int r = 0; r < kItems; ++r)
@@ -245,6 +260,7 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
       const uint32_t at = sh.base[d] + i - sh.start[d];
       if (out.keys) out.keys[at] = k;
       out.entries[at] = sh.entry[i];
+      if (out.next) atomicAdd(&out.next[(size_t)(at / chunk) * out.next_radix + ((k >> out.next_shift) & (out.next_radix - 1))], 1u);
     }
     __syncthreads();
     if (tid < kMaxRadix) sh.base[tid] += run;
@@ -257,6 +273,7 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  let_next_start();
   uint32_t key[kItems], entry[kItems], place[kItems];
   uint32_t kept = n;
   int done = 0;
@@ -271,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
       entry[r] = !in ? 0u : p == 0 ? i : sh.entry[i];
     }
     __syncthreads();
-    sort_tile(sh, key, entry, place, rounds, done, (1u << width) - 1u, kept);
+    sort_tile(sh, key, entry, place, rounds, done, width, kept);
     done += width;
   }
   for (uint32_t i = tid; i < kept; i += kThreads) {
@@ -299,6 +316,7 @@ __global__ void __launch_bounds__(256) places_kernel(const uint32_t* __restrict_
                                                      const uint32_t* __restrict__ entries, uint32_t n, int groups,
                                                      int* __restrict__ order, int* __restrict__ slots,
                                                      int* __restrict__ offsets) {
+  follow();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i < n) {
     const uint32_t e = entries[i];
@@ -338,21 +356,43 @@ inline Chunks chunks_for(long long n) {
 
 inline int passes_for(int bits) { return (bits + 7) / 8; }
 
-int one_pass(const Source& src, long long n, const uint32_t* n_dev, int shift, int bits, uint32_t* counts, Target out,
-             cudaStream_t st) {
+// All passes over the low `bits` bits.  The last one writes `out`; the ones before it go to and
+// fro between the two buffers of keys and entries at `buffers` (of `len` words each).
+int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* buffers, size_t len, uint32_t* count,
+                Target out, cudaStream_t st) {
+  static std::atomic<unsigned long long> allowed{0};
+  CVHRF_CUDA_TRY(allow_shared(chunk_scatter_kernel, sizeof(Shared), allowed));
   const Chunks c = chunks_for(n);
-  if (bits < 2) bits = 2;   // the counts are read four digits at a time
-  CVHRF_CUDA_TRY(cudaFuncSetAttribute(chunk_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)));
-  chunk_count_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << bits, counts);
+  const int passes = passes_for(bits);
+  int shift[5] = {0}, radix[4];
+  for (int p = 0; p < passes; ++p) {
+    int width = (bits - shift[p] + (passes - p) - 1) / (passes - p);   // the bits left, shared evenly
+    if (width < 2) width = 2;   // the counts are read four digits at a time
+    radix[p] = 1 << width;
+    shift[p + 1] = shift[p] + width;
+  }
+  int clear = 0;
+  for (int p = 1; p < passes; ++p) clear += c.count * radix[p];
+  chunk_count_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, c.size, 0, radix[0], counts, clear);
   CVHRF_LAUNCH_CHECK();
-  chunk_scatter_kernel<<<c.count, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << bits,
-                                                                  counts, out);
-  CVHRF_LAUNCH_CHECK();
+  for (int p = 0; p < passes; ++p) {
+    uint32_t* to = buffers + (p & 1) * 2 * len;
+    uint32_t* next = counts + (size_t)c.count * radix[p];
+    Target t = out;
+    if (p + 1 < passes) t = Target{to, to + len, nullptr, nullptr, 0, nullptr, next, shift[p + 1], radix[p + 1]};
+    t.count = p == 0 ? count : nullptr;
+    CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count), kThreads, sizeof(Shared), st, src, (uint32_t)n,
+                                p == 0 ? nullptr : count, c.size, shift[p], radix[p], counts, t));
+    count_launch(1);
+    src = Source{nullptr, 0, to, to + len, src.rows, 1};
+    counts = next;
+  }
   return CVHRF_OK;
 }
 
 int small_sort(const Source& src, long long n, int bits, Target out, cudaStream_t st) {
-  CVHRF_CUDA_TRY(cudaFuncSetAttribute(small_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)));
+  static std::atomic<unsigned long long> allowed{0};
+  CVHRF_CUDA_TRY(allow_shared(small_sort_kernel, sizeof(Shared), allowed));
   small_sort_kernel<<<1, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits, passes_for(bits), out);
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;
@@ -360,38 +400,28 @@ int small_sort(const Source& src, long long n, int bits, Target out, cudaStream_
 
 }  // namespace
 
-// scratch: count (64 words), counts matrix, two buffers of keys and entries
-size_t group_sort_words(long long n) { return 64 + (size_t)kMaxChunks * kMaxRadix + 4 * (align_up((size_t)n, 64)); }
+// scratch: count (64 words), the passes' matrices of counts, two buffers of keys and entries
+// (up to kTile keys only the result, of exactly that many)
+constexpr size_t kCountWords = 4 * (size_t)kMaxChunks * kMaxRadix;
+size_t group_sort_words(long long n) {
+  const size_t len = align_up((size_t)n, 64);
+  return n <= kTile ? 64 + 2 * len : 64 + kCountWords + 4 * len;
+}
 
 int group_sort(const void* index, int index_bytes, long long n, long long rows, bool keep_outside, uint32_t* scratch,
                cudaStream_t st, const uint32_t** keys, const uint32_t** entries, const uint32_t** count_dev) {
   uint32_t* count = scratch;
-  uint32_t* counts = scratch + 64;
-  const size_t len = align_up((size_t)n, 64);
-  uint32_t* k[2] = {counts + (size_t)kMaxChunks * kMaxRadix, nullptr};
-  k[1] = k[0] + 2 * len;
-  const int bits = bits_for((unsigned long long)rows + (keep_outside ? 1 : 0));
-  const int npass = passes_for(bits);
-  Source src{index, index_bytes, nullptr, nullptr, (uint32_t)rows, keep_outside ? 1 : 0};
   *count_dev = count;
-  if (n <= kTile) {
-    *keys = k[0];
-    *entries = k[0] + len;
-    return small_sort(src, n, bits, Target{k[0], k[0] + len, nullptr, nullptr, 0, count}, st);
-  }
-  int done = 0;
-  for (int p = 0; p < npass; ++p) {
-    const int width = (bits - done + (npass - p) - 1) / (npass - p);   // the bits left, shared evenly
-    uint32_t* to = k[p & 1];
-    Target out{to, to + len, nullptr, nullptr, 0, p == 0 ? count : nullptr};
-    const int rc = one_pass(src, n, p == 0 ? nullptr : count, done, width, counts, out, st);
-    if (rc) return rc;
-    src = Source{nullptr, 0, to, to + len, (uint32_t)rows, 1};
-    done += width;
-  }
-  *keys = src.keys;
-  *entries = src.entries;
-  return CVHRF_OK;
+  const size_t len = align_up((size_t)n, 64);
+  const int bits = bits_for((unsigned long long)rows + (keep_outside ? 1 : 0));
+  const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)rows, keep_outside ? 1 : 0};
+  uint32_t* buffers = scratch + 64 + (n <= kTile ? 0 : kCountWords);
+  uint32_t* to = buffers + (n <= kTile ? 0 : ((passes_for(bits) - 1) & 1) * 2 * len);
+  *keys = to;
+  *entries = to + len;
+  const Target out{to, to + len, nullptr, nullptr, 0, count, nullptr, 0, 0};
+  if (n <= kTile) return small_sort(src, n, bits, out, st);
+  return sort_chunks(src, n, bits, scratch + 64, buffers, len, count, out, st);
 }
 
 }  // namespace cvhrf
@@ -399,12 +429,13 @@ int group_sort(const void* index, int index_bytes, long long n, long long rows, 
 using namespace cvhrf;
 
 extern "C" size_t cvhrf_group_rows_workspace_bytes(long long entries, int groups) {
-  if (entries < 0 || entries > kGroupMaxEntries || groups < 1) return 0;
+  if (entries <= kTile || entries > kGroupMaxEntries || groups < 1) return 0;   // a small sort needs none
   return group_sort_words(entries) * sizeof(uint32_t);
 }
 
-extern "C" int cvhrf_group_rows(const void* index, int index_bytes, long long entries, int groups, int* order,
-                                int* slots, int* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int cvhrf_group_rows(const cvhrf_group_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const auto [index, order, slots, offsets, workspace, workspace_bytes, entries, groups, index_bytes] = *args;
   if (entries < 0 || groups < 1 || groups > 0x7ffffffe || (index_bytes != 4 && index_bytes != 8) || !offsets)
     return CVHRF_EINVAL;
   if (entries > 0 && (!index || !order || !slots)) return CVHRF_EINVAL;
@@ -414,21 +445,22 @@ extern "C" int cvhrf_group_rows(const void* index, int index_bytes, long long en
     CVHRF_CUDA_TRY(cudaMemsetAsync(offsets, 0, ((size_t)groups + 1) * sizeof(int), st));
     return CVHRF_OK;
   }
-  if (!workspace || workspace_bytes < cvhrf_group_rows_workspace_bytes(entries, groups)) return CVHRF_EWORKSPACE;
+  const size_t need = cvhrf_group_rows_workspace_bytes(entries, groups);
+  if (need && (!workspace || workspace_bytes < need)) return CVHRF_EWORKSPACE;
   if ((uintptr_t)workspace & 15) return CVHRF_EINVAL;
   uint32_t* scratch = (uint32_t*)workspace;
   const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)groups, 1};
-  const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr};
+  const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr, nullptr, 0, 0};
   const int bits = bits_for((unsigned long long)groups + 1);
   if (entries <= kTile) return small_sort(src, entries, bits, out, st);
   // up to 255 groups (and the entries left out) one pass writes everything
-  if (groups < kMaxRadix) return one_pass(src, entries, nullptr, 0, bits, scratch + 64, out, st);
+  if (groups < kMaxRadix) return sort_chunks(src, entries, bits, scratch + 64, nullptr, 0, scratch, out, st);
   const uint32_t *keys, *sorted, *count;
   const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, st, &keys, &sorted, &count);
   if (rc) return rc;
   const long long most = entries > (long long)groups + 1 ? entries : (long long)groups + 1;
-  places_kernel<<<(unsigned)((most + 255) / 256), 256, 0, st>>>(keys, sorted, (uint32_t)entries, groups, order, slots,
-                                                               offsets);
-  CVHRF_LAUNCH_CHECK();
+  CVHRF_CUDA_TRY(launch_after(places_kernel, dim3((unsigned)((most + 255) / 256)), 256, 0, st, keys, sorted,
+                              (uint32_t)entries, groups, order, slots, offsets));
+  count_launch(1);
   return CVHRF_OK;
 }

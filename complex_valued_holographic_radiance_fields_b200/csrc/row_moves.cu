@@ -11,6 +11,7 @@
 // Bound by memory: each touches N + N k rows once.
 #include <type_traits>
 #include "row_groups.cuh"
+#include "row_tiles.cuh"
 #include "row_types.cuh"
 
 namespace cvhrf {
@@ -21,7 +22,7 @@ constexpr int kThreads = 256;
 struct Moves {
   long long n;          // rows
   int choices, width;
-  int lanes;            // lanes that own a row
+  int lanes, owners;    // lanes that own a row, owners in a block
   const int* slots;     // n x choices
   const int* used;      // (device) places that belong to a group; the rest is behind the last group
 };
@@ -31,13 +32,8 @@ struct Moves {
 template <typename T, Layout L>
 __device__ __forceinline__ void clear_behind(const Moves& m, int used, long long x, long long owners, int lane,
                                              T* __restrict__ out) {
-  using R = Row<T, L>;
   const long long places = m.n * m.choices;
-  for (long long p = used + x; p < places; p += owners) {
-    T* to = out + p * m.width;
-    for (int e = lane * R::kVec - R::ahead(to); e < m.width; e += m.lanes * R::kVec)
-      R::store(to, e, m.width, zero_pack<T, L>());
-  }
+  for (long long p = used + x; p < places; p += owners) clear_row<T, L>(out + p * m.width, m.width, lane, m.lanes);
 }
 
 // Aligned rows: an owner has ROWS rows (owners apart, so that the owners of a block touch
@@ -47,8 +43,10 @@ template <typename T, int ROWS, int J>
 __global__ void __launch_bounds__(kThreads) rows_to_groups_kernel(Moves m, const T* __restrict__ x, long long stride,
                                                                   T* __restrict__ out) {
   using R = Row<T, kAligned>;
-  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
-  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
+  const Owner o = Owner::of(m.lanes);
+  const int owners = m.owners, lane = o.lane, step = m.lanes * R::kVec;
+  const long long first = (long long)blockIdx.x * (owners * ROWS) + o.index;
+  if (!o.live) return;
   const int used = *m.used;
   for (int c0 = lane * R::kVec; c0 < m.width; c0 += step * J) {
     uint4 p[ROWS][J];
@@ -85,33 +83,82 @@ template <typename T, Layout L, int ENTRIES>
 __global__ void __launch_bounds__(kThreads) entries_to_groups_kernel(Moves m, const T* __restrict__ x, Extent extent,
                                                                      long long stride, T* __restrict__ out) {
   using R = Row<T, L>;
-  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
+  const Owner o = Owner::of(m.lanes);
+  const int owners = m.owners, lane = o.lane;
   const long long entries = m.n * m.choices;
-  const long long first = (long long)blockIdx.x * (owners * ENTRIES) + threadIdx.x / m.lanes;
+  const long long first = (long long)blockIdx.x * (owners * ENTRIES) + o.index;
+  if (!o.live) return;
   const int used = *m.used;
+  bool inside = true;
   const T* from[ENTRIES];
   T* to[ENTRIES];
-  int e0[ENTRIES];
+  Edges edges[ENTRIES];
 #pragma unroll
   for (int q = 0; q < ENTRIES; ++q) {
     const long long e = first + q * owners;
     const int s = e < entries ? m.slots[e] : -1;
-    from[q] = s >= 0 ? x + (long long)((uint32_t)e / (uint32_t)m.choices) * stride : nullptr;   // entries are below 2^30
+    from[q] = x + (long long)((uint32_t)e / (uint32_t)m.choices) * stride;   // entries are below 2^30
     to[q] = out + (long long)(s >= 0 ? s : 0) * m.width;
-    e0[q] = lane * R::kVec - R::ahead(to[q]);
+    edges[q] = Edges::of<R>(to[q], m.width);
+    if (s < 0) edges[q].packs = edges[q].count = 0;
+    else inside = inside && extent.inside(from[q], m.width);
   }
-  for (int c = 0; c - (R::kVec - 1) < m.width; c += step) {
+  for (int k = lane; k < packs_of<T, L>(m.width); k += m.lanes) {
     typename R::Raw p[ENTRIES];
+    if (inside) {
+#pragma unroll
+      for (int q = 0; q < ENTRIES; ++q)
+        if (k < edges[q].packs) p[q] = R::load(from[q] + edges[q].head + k * R::kVec);
+    } else {
+#pragma unroll
+      for (int q = 0; q < ENTRIES; ++q)
+        if (k < edges[q].packs) p[q] = R::load_elements(from[q] + edges[q].head + k * R::kVec);
+    }
 #pragma unroll
     for (int q = 0; q < ENTRIES; ++q)
-      if (from[q] && e0[q] + c < m.width) p[q] = R::load(from[q], e0[q] + c, m.width, extent);
-#pragma unroll
-    for (int q = 0; q < ENTRIES; ++q)
-      if (from[q] && e0[q] + c < m.width) R::store(to[q], e0[q] + c, m.width, R::words(p[q]));
+      if (k < edges[q].packs) R::store(to[q] + edges[q].head + k * R::kVec, R::words(p[q]));
   }
 #pragma unroll
-  for (int q = 0; q < ENTRIES; ++q)
+  for (int q = 0; q < ENTRIES; ++q) {
+    if (L == kSpan)
+      for (int i = lane; i < edges[q].count; i += m.lanes) to[q][edges[q].edge(i)] = from[q][edges[q].edge(i)];
     if (first + q * owners < entries) clear_behind<T, L>(m, used, first + q * owners, entries, lane, out);
+  }
+}
+
+// ... gathered into runs of places.
+struct Places {
+  const int* order;     // the entry at each place
+  const int* used;
+  int choices;
+  __device__ __forceinline__ long long row(long long place) const {   // -1: behind the last group
+    return place < *used ? (long long)((uint32_t)order[place] / (uint32_t)choices) : -1;   // entries are below 2^30
+  }
+};
+
+template <typename T, bool WIDE, int ROWS, int J>
+__global__ void __launch_bounds__(kTileThreads) rows_to_groups_tile_kernel(Places places, long long count, int tile,
+                                                                           int width, const T* __restrict__ x,
+                                                                           long long stride, T* __restrict__ out) {
+  gather_tile<T, false, WIDE, ROWS, J>(
+      [&](long long p) -> const T* {
+        const long long n = places.row(p);
+        return n >= 0 ? x + n * stride : nullptr;
+      },
+      count, tile, width, 1.f, out);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) rows_to_groups_flat_kernel(Places places, long long count, int tile,
+                                                                           uint32_t reciprocal, int width,
+                                                                           const T* __restrict__ x, long long stride,
+                                                                           T* __restrict__ out) {
+  gather_flat<T, false>(
+      [&](long long p) -> const T* {
+        const long long n = places.row(p);
+        return n >= 0 ? x + n * stride : nullptr;
+      },
+      count, tile, reciprocal, width, 1.f, out);
 }
 
 // The weights are float32 or of the rows' type.
@@ -148,14 +195,26 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_kernel(Moves m, co
                                                                      long long stride, Weights weights,
                                                                      T* __restrict__ out) {
   using R = Row<T, L>;
-  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
-  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
-  int slot[ROWS][CHOICES], e0[ROWS];
+  const Owner o = Owner::of(m.lanes);
+  const int owners = m.owners, lane = o.lane;
+  const long long first = (long long)blockIdx.x * (owners * ROWS) + o.index;
+  if (!o.live) return;
+  int slot[ROWS][CHOICES];
   float w[ROWS][CHOICES];
+  Edges edges[ROWS];
   load_choices<T>(m, weights, first, owners, 0, slot, w);
+  bool inside = true;
 #pragma unroll
-  for (int q = 0; q < ROWS; ++q) e0[q] = lane * R::kVec - R::ahead(out + (first + q * owners) * m.width);
-  for (int c = 0; c - (L == kSpan ? R::kVec - 1 : 0) < m.width; c += step) {
+  for (int q = 0; q < ROWS; ++q) {
+    edges[q] = Edges::of<R>(out + (first + q * owners) * m.width, m.width);
+    if (first + q * owners >= m.n) edges[q].packs = edges[q].count = 0;
+    if (L == kSpan && extent.checked)
+      for (int i = 0; i < m.choices; ++i) {
+        const int s = first + q * owners < m.n ? m.slots[(first + q * owners) * m.choices + i] : -1;
+        if (s >= 0) inside = inside && extent.inside(y + (long long)s * stride, m.width);
+      }
+  }
+  for (int k = lane; k < packs_of<T, L>(m.width); k += m.lanes) {
     float acc[ROWS][R::kVec];
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
@@ -164,17 +223,21 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_kernel(Moves m, co
     for (int i0 = 0; i0 < m.choices; i0 += CHOICES) {
       if (m.choices > CHOICES) load_choices<T>(m, weights, first, owners, i0, slot, w);
       typename R::Raw p[ROWS][CHOICES];
+      auto load = [&](auto read) {
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+          for (int i = 0; i < CHOICES; ++i)
+            if (slot[q][i] >= 0 && k < edges[q].packs)
+              p[q][i] = read(y + (long long)slot[q][i] * stride + edges[q].head + k * R::kVec);
+      };
+      if (L != kSpan || inside) load([](const T* at) { return R::load(at); });
+      else load([](const T* at) { return R::load_elements(at); });
 #pragma unroll
       for (int q = 0; q < ROWS; ++q)
 #pragma unroll
         for (int i = 0; i < CHOICES; ++i)
-          if (slot[q][i] >= 0 && e0[q] + c < m.width)
-            p[q][i] = R::load(y + (long long)slot[q][i] * stride, e0[q] + c, m.width, extent);
-#pragma unroll
-      for (int q = 0; q < ROWS; ++q)
-#pragma unroll
-        for (int i = 0; i < CHOICES; ++i)
-          if (slot[q][i] >= 0 && e0[q] + c < m.width) {   // an entry left out counts nothing, whatever its weight holds
+          if (slot[q][i] >= 0 && k < edges[q].packs) {   // an entry left out counts nothing, whatever its weight holds
             float f[R::kVec];
             R::floats(p[q][i], f);
 #pragma unroll
@@ -183,9 +246,155 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_kernel(Moves m, co
     }
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
-      if (first + q * owners < m.n && e0[q] + c < m.width)
-        R::store(out + (first + q * owners) * m.width, e0[q] + c, m.width, R::words(acc[q]));
+      if (k < edges[q].packs)
+        R::store(out + (first + q * owners) * m.width + edges[q].head + k * R::kVec, R::words(acc[q]));
   }
+  if (L == kSpan) {
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      const long long row = first + q * owners;
+      for (int i = lane; i < edges[q].count; i += m.lanes) {
+        const int e = edges[q].edge(i);
+        float acc = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < m.choices; ++j) {
+          const int s = m.slots[row * m.choices + j];
+          if (s >= 0) acc = fmaf(weight_at<T>(weights, row * m.choices + j), to_float(y[(long long)s * stride + e]), acc);
+        }
+        out[row * m.width + e] = from_float<T>(acc);
+      }
+    }
+  }
+}
+
+// Rows that are not aligned, up to 4 KB: a warp puts its rows into the block's tile, two choices
+// of J elements per lane in flight.  Its slots and weights are 32 at a time, one per lane.
+template <typename T, bool WIDE, int J>
+__global__ void __launch_bounds__(kTileThreads) groups_to_rows_tile_kernel(long long rows, int choices, int tile,
+                                                                           int width, const int* __restrict__ slots,
+                                                                           const T* __restrict__ y, long long stride,
+                                                                           Weights weights, T* __restrict__ out) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  T* buf = reinterpret_cast<T*>(raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = tile / kTileWarps;
+  const long long first = (long long)blockIdx.x * tile;
+  const int n = (int)min((long long)tile, rows - first), r0 = warp * each, mine = max(0, min(each, n - r0));
+  const long long e0 = (first + r0) * choices;
+  const int entries = mine * choices;   // of this warp
+  int chunk = -32;
+  unsigned long long my_row = 0;
+  float my_weight = 0.f;
+  auto entry = [&](int e, const T*& row, float& w) {   // the same entry for the whole warp
+    if (e < chunk || e >= chunk + 32) {
+      chunk = e & ~31;
+      const int i = chunk + lane, s = i < entries ? slots[e0 + i] : -1;
+      my_row = (unsigned long long)(uintptr_t)(s >= 0 ? y + (long long)s * stride : reinterpret_cast<const T*>(g_zero_row));
+      my_weight = s >= 0 ? weight_at<T>(weights, e0 + i) : 0.f;   // left out: whatever its weight holds
+    }
+    row = reinterpret_cast<const T*>((uintptr_t)shuffle(my_row, e & 31)) + lane;
+    w = __shfl_sync(0xffffffffu, my_weight, e & 31);
+  };
+  for (int r = 0; r < mine; ++r) {
+    T* to = buf + (r0 + r) * width + lane;
+    for (int c = 0; c < width; c += 32 * J) {
+      const int left = width - lane - c;
+      float acc[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] = 0.f;
+      for (int i = 0; i < choices; i += 2) {
+        const T *a, *b;
+        float wa, wb = 0.f;
+        entry(r * choices + i, a, wa);
+        if (i + 1 < choices) entry(r * choices + i + 1, b, wb);
+        else b = reinterpret_cast<const T*>(g_zero_row) + lane;
+        T va[J], vb[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (32 * j < left) va[j] = a[c + 32 * j], vb[j] = b[c + 32 * j];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (32 * j < left) acc[j] = fmaf(wb, to_float(vb[j]), fmaf(wa, to_float(va[j]), acc[j]));
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (32 * j < left) to[c + 32 * j] = from_float<T>(acc[j]);
+      if (!WIDE) break;
+    }
+  }
+  send_tile(buf, n, width, out + first * width);
+}
+
+// ... and its gradient, by places: dy[p] = w dout[n], dw = <dout[n], y[p]> for the entry at p.
+template <typename T, bool WIDE, int ROWS, int J>
+__global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_tile_kernel(
+    Places places, long long count, int tile, int width, const T* __restrict__ grad, long long grad_stride,
+    const T* __restrict__ y, long long stride, Weights weights, T* __restrict__ grad_y,
+    void* __restrict__ grad_weights) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  T* buf = reinterpret_cast<T*>(raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = tile / kTileWarps;
+  const long long first = (long long)blockIdx.x * tile;
+  const int n = (int)min((long long)tile, count - first), r0 = warp * each;
+  const T* zeros = reinterpret_cast<const T*>(g_zero_row);
+  const T *grad_row = zeros, *y_row = zeros;
+  float weight = 0.f, my_dot = 0.f;
+  int entry = -1;
+  if (lane < each && r0 + lane < n) {
+    const long long p = first + r0 + lane, row = places.row(p);
+    entry = places.order[p];
+    if (row >= 0) {
+      grad_row = grad + row * grad_stride;
+      y_row = y + p * stride;
+      weight = weight_at<T>(weights, entry);
+    }
+  }
+  for (int r = 0; r < each; r += ROWS) {
+    const T *g[ROWS], *h[ROWS];
+    float w[ROWS], dot[ROWS];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      const int src = (r + q) & 31;
+      g[q] = reinterpret_cast<const T*>((uintptr_t)shuffle((unsigned long long)(uintptr_t)grad_row, src)) + lane;
+      h[q] = reinterpret_cast<const T*>((uintptr_t)shuffle((unsigned long long)(uintptr_t)y_row, src)) + lane;
+      w[q] = __shfl_sync(0xffffffffu, weight, src);
+      dot[q] = 0.f;
+    }
+    for (int c = 0; c < width; c += 32 * J) {
+      const int left = width - lane - c;
+      T vg[ROWS][J], vh[ROWS][J];
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (32 * j < left) {
+            vg[q][j] = g[q][c + 32 * j];
+            if (grad_weights) vh[q][j] = h[q][c + 32 * j];
+          }
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (32 * j < left) {
+            const float f = to_float(vg[q][j]);
+            if (grad_weights) dot[q] = fmaf(f, to_float(vh[q][j]), dot[q]);
+            if (grad_y && r + q < each) buf[(r0 + r + q) * width + lane + c + 32 * j] = from_float<T>(w[q] * f);
+          }
+      if (!WIDE) break;
+    }
+    if (grad_weights) {
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], o);
+        if (lane == r + q) my_dot = dot[q];
+      }
+    }
+  }
+  if (grad_weights && entry >= 0) {
+    if (weights.same) ((T*)grad_weights)[entry] = from_float<T>(my_dot);
+    else ((float*)grad_weights)[entry] = my_dot;
+  }
+  if (grad_y) send_tile(buf, n, width, grad_y + first * width);
 }
 
 // Packs follow the row of grad_y that is written (with unaligned rows each choice's begins
@@ -195,55 +404,77 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
     Moves m, const T* __restrict__ grad, Extent grad_extent, long long grad_stride, const T* __restrict__ y,
     Extent extent, long long stride, Weights weights, T* __restrict__ grad_y, void* __restrict__ grad_weights) {
   using R = Row<T, L>;
-  const int owners = kThreads / m.lanes, lane = threadIdx.x & (m.lanes - 1), step = m.lanes * R::kVec;
-  const long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / m.lanes;
+  constexpr bool kShared = L != kSpan;   // one pack of grad for all choices
+  const Owner o = Owner::of(m.lanes);
+  const int owners = m.owners, lane = o.lane;
+  // lanes without an owner stay for the shuffles, behind the last row
+  const long long first = o.live ? (long long)blockIdx.x * (owners * ROWS) + o.index : m.n;
   for (int i0 = 0; i0 < m.choices; i0 += CHOICES) {
-    int slot[ROWS][CHOICES], e0[ROWS][CHOICES];
+    int slot[ROWS][CHOICES];
     float w[ROWS][CHOICES], dot[ROWS][CHOICES];
+    Edges edges[ROWS][CHOICES];
     load_choices<T>(m, weights, first, owners, i0, slot, w);
+    bool inside = true;
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
 #pragma unroll
       for (int i = 0; i < CHOICES; ++i) {
         dot[q][i] = 0.f;
-        e0[q][i] = lane * R::kVec - (grad_y ? R::ahead(grad_y + (long long)slot[q][i] * m.width) : 0);
+        edges[q][i] = Edges::of<R>((grad_y ? grad_y : grad) + (long long)max(slot[q][i], 0) * m.width, m.width);
+        if (L == kSpan && slot[q][i] >= 0)
+          inside = inside && grad_extent.inside(grad + (first + q * owners) * grad_stride, m.width) &&
+                   (!grad_weights || extent.inside(y + (long long)slot[q][i] * stride, m.width));
       }
-    for (int c = 0; c - (L == kSpan ? R::kVec - 1 : 0) < m.width; c += step) {
-      typename R::Raw g[ROWS][L == kSpan ? CHOICES : 1], p[ROWS][CHOICES];
+    for (int k = lane; k < packs_of<T, L>(m.width); k += m.lanes) {
+      typename R::Raw g[ROWS][kShared ? 1 : CHOICES], p[ROWS][CHOICES];
+      auto load = [&](auto read) {
 #pragma unroll
-      for (int q = 0; q < ROWS; ++q) {
-        const T* row = grad + (first + q * owners) * grad_stride;
-        if (L != kSpan && first + q * owners < m.n && e0[q][0] + c < m.width)
-          g[q][0] = R::load(row, e0[q][0] + c, m.width, grad_extent);
+        for (int q = 0; q < ROWS; ++q) {
+          const T* row = grad + (first + q * owners) * grad_stride;
+          if (kShared && first + q * owners < m.n) g[q][0] = read(row + k * R::kVec);
 #pragma unroll
-        for (int i = 0; i < CHOICES; ++i)
-          if (slot[q][i] >= 0 && e0[q][i] + c < m.width) {
-            if (L == kSpan) g[q][L == kSpan ? i : 0] = R::load(row, e0[q][i] + c, m.width, grad_extent);
-            if (grad_weights) p[q][i] = R::load(y + (long long)slot[q][i] * stride, e0[q][i] + c, m.width, extent);
-          }
-      }
+          for (int i = 0; i < CHOICES; ++i)
+            if (slot[q][i] >= 0 && k < edges[q][i].packs) {
+              const int e = edges[q][i].head + k * R::kVec;
+              if (!kShared) g[q][kShared ? 0 : i] = read(row + e);
+              if (grad_weights) p[q][i] = read(y + (long long)slot[q][i] * stride + e);
+            }
+        }
+      };
+      if (L != kSpan || inside) load([](const T* at) { return R::load(at); });
+      else load([](const T* at) { return R::load_elements(at); });
 #pragma unroll
       for (int q = 0; q < ROWS; ++q)
 #pragma unroll
-        for (int i = 0; i < CHOICES; ++i) {
-          const int e = e0[q][i] + c;
-          if (slot[q][i] >= 0 && e < m.width) {
+        for (int i = 0; i < CHOICES; ++i)
+          if (slot[q][i] >= 0 && k < edges[q][i].packs) {
             float f[R::kVec];
-            R::floats(g[q][L == kSpan ? i : 0], f);
+            R::floats(g[q][kShared ? 0 : i], f);
             if (grad_weights) {
               float h[R::kVec];
               R::floats(p[q][i], h);
 #pragma unroll
-              for (int v = 0; v < R::kVec; ++v)
-                if (L != kSpan || (e + v >= 0 && e + v < m.width)) dot[q][i] = fmaf(f[v], h[v], dot[q][i]);
+              for (int v = 0; v < R::kVec; ++v) dot[q][i] = fmaf(f[v], h[v], dot[q][i]);
             }
             if (grad_y) {
 #pragma unroll
               for (int v = 0; v < R::kVec; ++v) f[v] *= w[q][i];
-              R::store(grad_y + (long long)slot[q][i] * m.width, e, m.width, R::words(f));
+              R::store(grad_y + (long long)slot[q][i] * m.width + edges[q][i].head + k * R::kVec, R::words(f));
             }
           }
-        }
+    }
+    if (L == kSpan) {
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < CHOICES; ++i)
+          if (slot[q][i] >= 0)
+            for (int j = lane; j < edges[q][i].count; j += m.lanes) {
+              const int e = edges[q][i].edge(j);
+              const float f = to_float(grad[(first + q * owners) * grad_stride + e]);
+              if (grad_weights) dot[q][i] = fmaf(f, to_float(y[(long long)slot[q][i] * stride + e]), dot[q][i]);
+              if (grad_y) grad_y[(long long)slot[q][i] * m.width + e] = from_float<T>(w[q][i] * f);
+            }
     }
     if (grad_weights) {
 #pragma unroll
@@ -251,7 +482,14 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
 #pragma unroll
         for (int i = 0; i < CHOICES; ++i) {
           float d = dot[q][i];
-          for (int o = m.lanes >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if ((m.lanes & (m.lanes - 1)) == 0) {
+            for (int x = m.lanes >> 1; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+          } else {   // lanes beside one another: halve what is left, an odd one waits for its turn
+            for (int left = m.lanes; left > 1; left = (left + 1) >> 1) {
+              const float other = __shfl_down_sync(0xffffffffu, d, (left + 1) >> 1);
+              if (lane < left >> 1) d += other;
+            }
+          }
           const long long row = first + q * owners, e = row * m.choices + i0 + i;
           if (lane == 0 && row < m.n && i0 + i < m.choices) {
             if (weights.same) ((T*)grad_weights)[e] = from_float<T>(d);
@@ -268,10 +506,8 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
   }
 }
 
-// Lanes that own a row of `packs` packs, and the blocks for `rows` rows per owner.
-inline int lanes_for(int packs) { return next_pow2(packs < 32 ? packs : 32); }
-inline unsigned blocks_for(long long n, int lanes, int rows) {
-  const int per_block = kThreads / lanes * rows;
+inline unsigned blocks_for(long long n, int owners, int rows) {
+  const long long per_block = (long long)owners * rows;
   return (unsigned)((n + per_block - 1) / per_block);
 }
 
@@ -284,19 +520,44 @@ int with_layout(bool aligned, int width, F f) {
 }
 
 template <typename T>
-int to_groups(bool aligned, const void* x, long long stride, Moves m, void* out, cudaStream_t st) {
+int to_groups(bool aligned, const void* x, long long stride, Moves m, const int* order, void* out, cudaStream_t st) {
+  const Places places{order, m.used, m.choices};
+  const long long count = m.n * m.choices;
+  if (!aligned && flat_fits(m.width, out)) {
+    const int tile = flat_rows(m.width, sizeof(T));
+    rows_to_groups_flat_kernel<T><<<(unsigned)((count + tile - 1) / tile), kTileThreads, 0, st>>>(
+        places, count, tile, flat_reciprocal(m.width), m.width, (const T*)x, stride, (T*)out);
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
+  if (!aligned && tile_fits(m.width, sizeof(T), out)) {
+    const int tile = tile_rows(count, m.width, sizeof(T));
+    const unsigned blocks = (unsigned)((count + tile - 1) / tile);
+    const size_t shared = (size_t)tile * m.width * sizeof(T);
+#define CVHRF_LAUNCH(WIDE, ROWS, J)                                                        \
+  rows_to_groups_tile_kernel<T, WIDE, ROWS, J><<<blocks, kTileThreads, shared, st>>>(      \
+      places, count, tile, m.width, (const T*)x, stride, (T*)out)
+    if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
+    else if (m.width > 64) CVHRF_LAUNCH(false, 2, 4);
+    else if (m.width > 32) CVHRF_LAUNCH(false, 4, 2);
+    else CVHRF_LAUNCH(false, 8, 1);
+#undef CVHRF_LAUNCH
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
   return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
     constexpr Layout L = decltype(layout)::value;
     m.lanes = lanes;
+    m.owners = owners_of(kThreads, lanes);
     const T* from = (const T*)x;
     if constexpr (L == kAligned) {
       const int packs = packs_of<T, L>(m.width);
-      if (packs > 64) rows_to_groups_kernel<T, 1, 4><<<blocks_for(m.n, lanes, 1), kThreads, 0, st>>>(m, from, stride, (T*)out);
-      else if (packs > 32) rows_to_groups_kernel<T, 2, 2><<<blocks_for(m.n, lanes, 2), kThreads, 0, st>>>(m, from, stride, (T*)out);
-      else rows_to_groups_kernel<T, 4, 1><<<blocks_for(m.n, lanes, 4), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      if (packs > 64) rows_to_groups_kernel<T, 1, 4><<<blocks_for(m.n, m.owners, 1), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      else if (packs > 32) rows_to_groups_kernel<T, 2, 2><<<blocks_for(m.n, m.owners, 2), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      else rows_to_groups_kernel<T, 4, 1><<<blocks_for(m.n, m.owners, 4), kThreads, 0, st>>>(m, from, stride, (T*)out);
     } else {
       constexpr int kEntries = L == kSpan ? 2 : 4;
-      entries_to_groups_kernel<T, L, kEntries><<<blocks_for(m.n * m.choices, lanes, kEntries), kThreads, 0, st>>>(
+      entries_to_groups_kernel<T, L, kEntries><<<blocks_for(m.n * m.choices, m.owners, kEntries), kThreads, 0, st>>>(
           m, from, extent_of(x, m.n, stride, m.width, sizeof(T)), stride, (T*)out);
     }
     CVHRF_LAUNCH_CHECK();
@@ -306,20 +567,36 @@ int to_groups(bool aligned, const void* x, long long stride, Moves m, void* out,
 
 template <typename T>
 int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weights, void* out, cudaStream_t st) {
+  if (!aligned && m.width > kFlatWidth && tile_fits(m.width, sizeof(T), out)) {
+    const int tile = tile_rows(m.n, m.width, sizeof(T));
+    const unsigned blocks = (unsigned)((m.n + tile - 1) / tile);
+    const size_t shared = (size_t)tile * m.width * sizeof(T);
+#define CVHRF_LAUNCH(WIDE, J)                                                          \
+  groups_to_rows_tile_kernel<T, WIDE, J><<<blocks, kTileThreads, shared, st>>>(        \
+      m.n, m.choices, tile, m.width, m.slots, (const T*)y, stride, weights, (T*)out)
+    if (m.width > 128) CVHRF_LAUNCH(true, 8);
+    else if (m.width > 64) CVHRF_LAUNCH(false, 4);
+    else if (m.width > 32) CVHRF_LAUNCH(false, 2);
+    else CVHRF_LAUNCH(false, 1);
+#undef CVHRF_LAUNCH
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
   return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
     constexpr Layout L = decltype(layout)::value;
     m.lanes = lanes;
+    m.owners = owners_of(kThreads, lanes);
     const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
 #define CVHRF_LAUNCH(ROWS, CHOICES)                                                               \
-  groups_to_rows_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, lanes, ROWS), kThreads, 0, st>>>(  \
+  groups_to_rows_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, m.owners, ROWS), kThreads, 0, st>>>(  \
       m, (const T*)y, extent, stride, weights, (T*)out)
     if constexpr (L == kSpan) {   // twice the registers per pack
       if (m.choices > 1) CVHRF_LAUNCH(1, 2);
-      else CVHRF_LAUNCH(2, 1);
+      else CVHRF_LAUNCH(1, 1);
     } else {
       if (m.choices > 2) CVHRF_LAUNCH(1, 4);
-      else if (m.choices > 1) CVHRF_LAUNCH(2, 2);
-      else CVHRF_LAUNCH(4, 1);
+      else if (m.choices > 1) CVHRF_LAUNCH(1, 2);
+      else CVHRF_LAUNCH(2, 1);
     }
 #undef CVHRF_LAUNCH
     CVHRF_LAUNCH_CHECK();
@@ -329,21 +606,39 @@ int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weig
 
 template <typename T>
 int to_rows_backward(bool aligned, const void* grad, long long grad_stride, const void* y, long long stride, Moves m,
-                     Weights weights, void* grad_y, void* grad_weights, cudaStream_t st) {
+                     const int* order, Weights weights, void* grad_y, void* grad_weights, cudaStream_t st) {
+  if (!aligned && m.width > kFlatWidth && tile_fits(m.width, sizeof(T), grad_y)) {
+    const Places places{order, m.used, m.choices};
+    const long long count = m.n * m.choices;
+    const int tile = tile_rows(count, m.width, sizeof(T));
+    const unsigned blocks = (unsigned)((count + tile - 1) / tile);
+    const size_t shared = (size_t)tile * m.width * sizeof(T);
+#define CVHRF_LAUNCH(WIDE, ROWS, J)                                                               \
+  groups_to_rows_backward_tile_kernel<T, WIDE, ROWS, J><<<blocks, kTileThreads, shared, st>>>(    \
+      places, count, tile, m.width, (const T*)grad, grad_stride, (const T*)y, stride, weights, (T*)grad_y, grad_weights)
+    if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
+    else if (m.width > 64) CVHRF_LAUNCH(false, 1, 4);
+    else if (m.width > 32) CVHRF_LAUNCH(false, 2, 2);
+    else CVHRF_LAUNCH(false, 4, 1);
+#undef CVHRF_LAUNCH
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
   return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
     constexpr Layout L = decltype(layout)::value;
     m.lanes = lanes;
+    m.owners = owners_of(kThreads, lanes);
     const Extent grad_extent = extent_of(grad, m.n, grad_stride, m.width, sizeof(T));
     const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
 #define CVHRF_LAUNCH(ROWS, CHOICES)                                                                        \
-  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, lanes, ROWS), kThreads, 0, st>>>(  \
+  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, m.owners, ROWS), kThreads, 0, st>>>(  \
       m, (const T*)grad, grad_extent, grad_stride, (const T*)y, extent, stride, weights, (T*)grad_y, grad_weights)
     if constexpr (L == kSpan) {   // four times: the pack of grad and of y
       CVHRF_LAUNCH(1, 1);
     } else {
       if (m.choices > 2) CVHRF_LAUNCH(1, 4);
-      else if (m.choices > 1) CVHRF_LAUNCH(2, 2);
-      else CVHRF_LAUNCH(4, 1);
+      else if (m.choices > 1) CVHRF_LAUNCH(1, 2);
+      else CVHRF_LAUNCH(2, 1);
     }
 #undef CVHRF_LAUNCH
     CVHRF_LAUNCH_CHECK();
@@ -369,54 +664,55 @@ int with_type(int dtype, F f) {
 
 using namespace cvhrf;
 
-extern "C" int cvhrf_rows_to_groups(const void* x, long long x_stride, int dtype, long long n, int choices, int width,
-                                    const int* slots, const int* used, void* out, void* stream) {
-  const int rc = check_moves(dtype, n, choices, width);
+extern "C" int cvhrf_rows_to_groups(const cvhrf_moves_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const cvhrf_moves_args a = *args;
+  const int rc = check_moves(a.dtype, a.n, a.choices, a.width);
   if (rc) return rc;
-  if (x_stride < 0) return CVHRF_EINVAL;
-  if (n == 0) return CVHRF_OK;
-  if (!x || !slots || !used || !out) return CVHRF_EINVAL;
-  const bool aligned = rows_16(x, x_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
-  const Moves m{n, choices, width, 0, slots, used};
-  return with_type(dtype, [&](auto type) {
-    return to_groups<decltype(type)>(aligned, x, x_stride, m, out, (cudaStream_t)stream);
+  if (a.stride < 0) return CVHRF_EINVAL;
+  if (a.n == 0) return CVHRF_OK;
+  if (!a.from || !a.order || !a.slots || !a.used || !a.to) return CVHRF_EINVAL;
+  const bool aligned = rows_16(a.from, a.stride, a.width, row_type_bytes(a.dtype)) && ((uintptr_t)a.to & 15) == 0;
+  const Moves m{a.n, a.choices, a.width, 0, 0, a.slots, a.used};
+  return with_type(a.dtype, [&](auto type) {
+    return to_groups<decltype(type)>(aligned, a.from, a.stride, m, a.order, a.to, (cudaStream_t)stream);
   });
 }
 
-extern "C" int cvhrf_groups_to_rows(const void* y, long long y_stride, int dtype, long long n, int choices, int width,
-                                    const int* slots, const void* weights, int weights_dtype, void* out,
-                                    void* stream) {
-  const int rc = check_moves(dtype, n, choices, width);
+extern "C" int cvhrf_groups_to_rows(const cvhrf_moves_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const cvhrf_moves_args a = *args;
+  const int rc = check_moves(a.dtype, a.n, a.choices, a.width);
   if (rc) return rc;
-  if (y_stride < 0 || (weights && weights_dtype != CVHRF_F32 && weights_dtype != dtype)) return CVHRF_EINVAL;
-  if (n == 0) return CVHRF_OK;
-  if (!y || !slots || !out) return CVHRF_EINVAL;
-  const bool aligned = rows_16(y, y_stride, width, row_type_bytes(dtype)) && ((uintptr_t)out & 15) == 0;
-  const Moves m{n, choices, width, 0, slots, nullptr};
-  const Weights w{weights, weights && weights_dtype == dtype};
-  return with_type(dtype, [&](auto type) {
-    return to_rows<decltype(type)>(aligned, y, y_stride, m, w, out, (cudaStream_t)stream);
+  if (a.stride < 0 || (a.weights && a.weights_dtype != CVHRF_F32 && a.weights_dtype != a.dtype)) return CVHRF_EINVAL;
+  if (a.n == 0) return CVHRF_OK;
+  if (!a.from || !a.slots || !a.to) return CVHRF_EINVAL;
+  const bool aligned = rows_16(a.from, a.stride, a.width, row_type_bytes(a.dtype)) && ((uintptr_t)a.to & 15) == 0;
+  const Moves m{a.n, a.choices, a.width, 0, 0, a.slots, nullptr};
+  const Weights w{a.weights, a.weights && a.weights_dtype == a.dtype};
+  return with_type(a.dtype, [&](auto type) {
+    return to_rows<decltype(type)>(aligned, a.from, a.stride, m, w, a.to, (cudaStream_t)stream);
   });
 }
 
-extern "C" int cvhrf_groups_to_rows_backward(const void* grad, long long grad_stride, const void* y,
-                                             long long y_stride, int dtype, long long n, int choices, int width,
-                                             const int* slots, const int* used, const void* weights,
-                                             int weights_dtype, void* grad_y, void* grad_weights, void* stream) {
-  const int rc = check_moves(dtype, n, choices, width);
+extern "C" int cvhrf_groups_to_rows_backward(const cvhrf_moves_backward_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const cvhrf_moves_backward_args a = *args;
+  const int rc = check_moves(a.dtype, a.n, a.choices, a.width);
   if (rc) return rc;
-  if (grad_stride < 0 || y_stride < 0 || (weights && weights_dtype != CVHRF_F32 && weights_dtype != dtype) ||
-      (grad_weights && !weights))
+  if (a.grad_stride < 0 || a.y_stride < 0 ||
+      (a.weights && a.weights_dtype != CVHRF_F32 && a.weights_dtype != a.dtype) || (a.grad_weights && !a.weights))
     return CVHRF_EINVAL;
-  if (n == 0 || (!grad_y && !grad_weights)) return CVHRF_OK;
-  if (!grad || !slots || !used || (grad_weights && !y)) return CVHRF_EINVAL;
-  const size_t elem = row_type_bytes(dtype);
-  const bool aligned = rows_16(grad, grad_stride, width, elem) &&
-                       (!grad_weights || rows_16(y, y_stride, width, elem)) && ((uintptr_t)grad_y & 15) == 0;
-  const Moves m{n, choices, width, 0, slots, used};
-  const Weights w{weights, weights && weights_dtype == dtype};
-  return with_type(dtype, [&](auto type) {
-    return to_rows_backward<decltype(type)>(aligned, grad, grad_stride, y, y_stride, m, w, grad_y, grad_weights,
-                                            (cudaStream_t)stream);
+  if (a.n == 0 || (!a.grad_y && !a.grad_weights)) return CVHRF_OK;
+  if (!a.grad || !a.order || !a.slots || !a.used || (a.grad_weights && !a.y)) return CVHRF_EINVAL;
+  const size_t elem = row_type_bytes(a.dtype);
+  const bool aligned = rows_16(a.grad, a.grad_stride, a.width, elem) &&
+                       (!a.grad_weights || rows_16(a.y, a.y_stride, a.width, elem)) && ((uintptr_t)a.grad_y & 15) == 0;
+  const Moves m{a.n, a.choices, a.width, 0, 0, a.slots, a.used};
+  const Weights w{a.weights, a.weights && a.weights_dtype == a.dtype};
+  return with_type(a.dtype, [&](auto type) {
+    return to_rows_backward<decltype(type)>(aligned, a.grad, a.grad_stride, a.y, a.y_stride, m, a.order, w,
+                                            a.grad_y,
+                                            a.grad_weights, (cudaStream_t)stream);
   });
 }

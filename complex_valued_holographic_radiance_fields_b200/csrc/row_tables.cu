@@ -16,6 +16,8 @@
 // between blocks by table_join_kernel.  The order of every sum is fixed, so results repeat.
 #include "row_groups.cuh"
 #include "row_types.cuh"
+#include "row_tiles.cuh"
+#include "row_words.cuh"
 
 namespace cvhrf {
 namespace {
@@ -28,20 +30,22 @@ __device__ __forceinline__ long long table_row(const void* index, int bytes, lon
   return (unsigned long long)v < (unsigned long long)rows ? v : -1;
 }
 
-// A row is owned by a power of two of lanes, up to a warp.  An owner has ROWS rows in flight
-// (J packs of each at a time), the owners of a block neighbouring rows; blocks walk over the
+// Aligned rows.  A row is owned by up to a warp of lanes; an owner has ROWS rows in flight (J
+// packs of each at a time), the owners of a block neighbouring rows.  Blocks walk over the
 // entries, and the indices of the next rows are read while these rows are on their way:
 // without that a row waits for two trips to memory, one after the other.
-template <typename T, Layout L, int ROWS, int J>
-__global__ void __launch_bounds__(kThreads, 4) table_lookup_kernel(const T* __restrict__ table, Extent extent,
-                                                                   long long rows, int width, long long stride,
+template <typename T, int ROWS, int J>
+__global__ void __launch_bounds__(kThreads, 4) table_lookup_kernel(const T* __restrict__ table, long long rows,
+                                                                   int width, long long stride,
                                                                    const void* __restrict__ index, int index_bytes,
-                                                                   long long entries, int lanes, float scale,
-                                                                   T* __restrict__ out) {
-  using R = Row<T, L>;
-  const int owners = kThreads / lanes, lane = threadIdx.x & (lanes - 1), step = lanes * R::kVec;
+                                                                   long long entries, int lanes, int owners,
+                                                                   float scale, T* __restrict__ out) {
+  using R = Row<T, kAligned>;
+  const Owner o = Owner::of(lanes);
+  const int step = lanes * R::kVec;
+  if (!o.live) return;
   const long long walk = (long long)gridDim.x * owners * ROWS;
-  long long first = (long long)blockIdx.x * (owners * ROWS) + threadIdx.x / lanes;
+  long long first = (long long)blockIdx.x * (owners * ROWS) + o.index;
   long long v[ROWS];
   auto load_index = [&](long long from) {
 #pragma unroll
@@ -53,89 +57,154 @@ __global__ void __launch_bounds__(kThreads, 4) table_lookup_kernel(const T* __re
   load_index(first);
   for (; first < entries; first += walk) {
     const T* from[ROWS];
-    T* to[ROWS];
-    int e0[ROWS];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      from[k] = v[k] >= 0 ? table + v[k] * stride : nullptr;
-      to[k] = out + (first + k * owners) * width;
-      e0[k] = lane * R::kVec - R::ahead(to[k]);
-    }
+    for (int k = 0; k < ROWS; ++k) from[k] = v[k] >= 0 ? table + v[k] * stride : nullptr;
     bool next = true;
-    for (int c = 0; c - (L == kSpan ? R::kVec - 1 : 0) < width; c += step * J) {
+    for (int c = o.lane * R::kVec; c < width; c += step * J) {
       typename R::Raw p[ROWS][J];
 #pragma unroll
       for (int k = 0; k < ROWS; ++k)
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (from[k] && e0[k] + c + j * step < width) p[k][j] = R::load(from[k], e0[k] + c + j * step, width, extent);
+          if (from[k] && c + j * step < width) p[k][j] = R::load(from[k] + c + j * step);
       if (next) load_index(first + walk);
       next = false;
 #pragma unroll
       for (int k = 0; k < ROWS; ++k)
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (first + k * owners < entries && e0[k] + c + j * step < width) {
-            if (from[k]) {
-              float f[R::kVec];
-              R::floats(p[k][j], f);
+          if (first + k * owners < entries && c + j * step < width) {
+            float f[R::kVec];
+            R::floats(p[k][j], f);
 #pragma unroll
-              for (int i = 0; i < R::kVec; ++i) f[i] *= scale;
-              R::store(to[k], e0[k] + c + j * step, width, R::words(f));
-            } else {
-              R::store(to[k], e0[k] + c + j * step, width, zero_pack<T, L>());
-            }
+            for (int i = 0; i < R::kVec; ++i) f[i] *= scale;
+            R::store(out + (first + k * owners) * width + c + j * step, from[k] ? R::words(f) : zero_words());
           }
     }
   }
 }
 
-template <typename T, Layout L, int ROWS, int J>
+// Rows that are not aligned, up to 4 KB.
+template <typename T, bool WIDE, int ROWS, int J>
+__global__ void __launch_bounds__(kTileThreads) table_lookup_tile_kernel(const T* __restrict__ table, long long rows,
+                                                                         int width, long long stride,
+                                                                         const void* __restrict__ index,
+                                                                         int index_bytes, long long entries, int tile,
+                                                                         float scale, T* __restrict__ out) {
+  gather_tile<T, true, WIDE, ROWS, J>(
+      [&](long long t) -> const T* {
+        const long long v = table_row(index, index_bytes, t, rows);
+        return v >= 0 ? table + v * stride : nullptr;
+      },
+      entries, tile, width, scale, out);
+}
+
+template <typename T, bool WIDE, int ROWS, int J>
+int launch_lookup_tile(const void* table, long long rows, int width, long long stride, const void* index,
+                       int index_bytes, long long entries, float scale, void* out, cudaStream_t st) {
+  const int tile = tile_rows(entries, width, sizeof(T));
+  table_lookup_tile_kernel<T, WIDE, ROWS, J>
+      <<<(unsigned)((entries + tile - 1) / tile), kTileThreads, (size_t)tile * width * sizeof(T), st>>>(
+          (const T*)table, rows, width, stride, index, index_bytes, entries, tile, scale, (T*)out);
+  CVHRF_LAUNCH_CHECK();
+  return CVHRF_OK;
+}
+
+// ... of a few elements.
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) table_lookup_flat_kernel(const T* __restrict__ table, long long rows,
+                                                                         int width, long long stride,
+                                                                         const void* __restrict__ index,
+                                                                         int index_bytes, long long entries, int tile,
+                                                                         uint32_t reciprocal, float scale,
+                                                                         T* __restrict__ out) {
+  gather_flat<T, true>(
+      [&](long long t) -> const T* {
+        const long long v = table_row(index, index_bytes, t, rows);
+        return v >= 0 ? table + v * stride : nullptr;
+      },
+      entries, tile, reciprocal, width, scale, out);
+}
+
+// ... and wider ones, or an output that does not begin on 16 bytes.
+template <typename T, int LANES, int FLIGHT, int J>
+__global__ void __launch_bounds__(kWordThreads) table_lookup_words_kernel(const T* __restrict__ table, Source4 source,
+                                                                          long long rows, int width,
+                                                                          const void* __restrict__ index,
+                                                                          int index_bytes, long long entries,
+                                                                          int rounds, int lanes, float scale,
+                                                                          T* __restrict__ out) {
+  copy_rows<T, true, LANES, FLIGHT, J>(
+      [&](long long e, int& from, int& to) {
+        from = (int)table_row(index, index_bytes, e, rows);
+        to = (int)e;
+      },
+      entries, rounds, lanes, width, table, source, scale, out);
+}
+
+template <typename T, int LANES, int FLIGHT, int J>
+int launch_lookup_words(const void* table, long long rows, int width, long long stride, const void* index,
+                        int index_bytes, long long entries, float scale, void* out, cudaStream_t st) {
+  const int lanes = word_lanes(words_of<T>(width)), owners = 32 / lanes, rounds = rounds_for(entries, owners, FLIGHT);
+  table_lookup_words_kernel<T, LANES, FLIGHT, J><<<word_blocks(entries, rounds, owners), kWordThreads, 0, st>>>(
+      (const T*)table, source4_of(table, rows, stride, width, sizeof(T)), rows, width, index, index_bytes, entries,
+      rounds, lanes, scale, (T*)out);
+  CVHRF_LAUNCH_CHECK();
+  return CVHRF_OK;
+}
+
+template <typename T, int ROWS, int J>
 int launch_lookup(const void* table, long long rows, int width, long long stride, const void* index, int index_bytes,
                   long long entries, int lanes, float scale, void* out, cudaStream_t st) {
   static const int resident = [] {
     int blocks = 0;
     const cudaError_t e =
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, table_lookup_kernel<T, L, ROWS, J>, kThreads, 0);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, table_lookup_kernel<T, ROWS, J>, kThreads, 0);
     return e == cudaSuccess && blocks > 0 ? blocks : 4;
   }();
-  const long long per_block = kThreads / lanes * ROWS, blocks = (entries + per_block - 1) / per_block;
+  const int owners = owners_of(kThreads, lanes);
+  const long long per_block = (long long)owners * ROWS, blocks = (entries + per_block - 1) / per_block;
   const long long most = 148 * resident;
-  table_lookup_kernel<T, L, ROWS, J><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, st>>>(
-      (const T*)table, extent_of(table, rows, stride, width, sizeof(T)), rows, width, stride, index, index_bytes,
-      entries, lanes, scale, (T*)out);
+  table_lookup_kernel<T, ROWS, J><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, st>>>(
+      (const T*)table, rows, width, stride, index, index_bytes, entries, lanes, owners, scale, (T*)out);
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;
-}
-
-template <typename T, Layout L>
-int lookup_rows(const void* table, long long rows, int width, long long stride, const void* index, int index_bytes,
-                long long entries, float scale, void* out, cudaStream_t st) {
-  const int packs = packs_of<T, L>(width), lanes = next_pow2(packs < 32 ? packs : 32);
-  if constexpr (L == kSpan) {   // twice the registers per pack
-    if (packs > 32)
-      return launch_lookup<T, L, 1, 2>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
-    return launch_lookup<T, L, 2, 1>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
-  } else {
-    if (packs > 64)
-      return launch_lookup<T, L, 1, 4>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
-    if (packs > 32)
-      return launch_lookup<T, L, 2, 2>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
-    return launch_lookup<T, L, 4, 1>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
-  }
 }
 
 template <typename T>
 int lookup(const void* table, long long rows, int width, long long stride, const void* index, int index_bytes,
            long long entries, float scale, void* out, cudaStream_t st) {
-  if (rows_16(table, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0)
-    return lookup_rows<T, kAligned>(table, rows, width, stride, index, index_bytes, entries, scale, out, st);
-  if (width >= kSpanWidth)
-    return lookup_rows<T, kSpan>(table, rows, width, stride, index, index_bytes, entries, scale, out, st);
-  // rows of one element per lane: a warp's worth of lanes at most, so one step
-  const int lanes = next_pow2(width);
-  return launch_lookup<T, kElement, 4, 1>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out,
-                                          st);
+  if (rows_16(table, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0) {
+    const int packs = packs_of<T, kAligned>(width), lanes = lanes_for(packs);
+    if (packs > 64)
+      return launch_lookup<T, 1, 4>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
+    if (packs > 32)
+      return launch_lookup<T, 2, 2>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
+    return launch_lookup<T, 4, 1>(table, rows, width, stride, index, index_bytes, entries, lanes, scale, out, st);
+  }
+  if (flat_fits(width, out)) {
+    const int tile = flat_rows(width, sizeof(T));
+    table_lookup_flat_kernel<T><<<(unsigned)((entries + tile - 1) / tile), kTileThreads, 0, st>>>(
+        (const T*)table, rows, width, stride, index, index_bytes, entries, tile, flat_reciprocal(width), scale,
+        (T*)out);
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
+  if (tile_fits(width, sizeof(T), out)) {
+#define CVHRF_LOOKUP_TILE(WIDE, ROWS, J) \
+  launch_lookup_tile<T, WIDE, ROWS, J>(table, rows, width, stride, index, index_bytes, entries, scale, out, st)
+    if (width > 128) return CVHRF_LOOKUP_TILE(true, 1, 8);
+    if (width > 64) return CVHRF_LOOKUP_TILE(false, 2, 4);
+    if (width > 32) return CVHRF_LOOKUP_TILE(false, 4, 2);
+    return CVHRF_LOOKUP_TILE(false, 8, 1);
+#undef CVHRF_LOOKUP_TILE
+  }
+  const int words = words_of<T>(width);
+  if (words > 64)
+    return launch_lookup_words<T, 32, 2, 4>(table, rows, width, stride, index, index_bytes, entries, scale, out, st);
+  if (words >= 32)
+    return launch_lookup_words<T, 32, 4, 2>(table, rows, width, stride, index, index_bytes, entries, scale, out, st);
+  return launch_lookup_words<T, 0, 4, 1>(table, rows, width, stride, index, index_bytes, entries, scale, out, st);
 }
 
 // ---- gradient -------------------------------------------------------------------------
@@ -157,7 +226,7 @@ struct Gradient {
   const uint32_t* count;     // how many
   long long stride;          // elements between the rows of grad
   int rows, width;
-  int lanes;                 // lanes of a unit (a power of two up to 32)
+  int lanes, units;          // lanes of a unit (up to 32), units of a block
   int items;                 // items of a unit
   float scale;
   uint8_t* mask;             // may be null
@@ -187,15 +256,16 @@ constexpr size_t gradient_shared() {   // staged entries, heads and tails (units
 
 // Units of `lanes` lanes; a lane holds one pack of columns; blockIdx.y: column tile.
 template <typename T, Layout L>
-__global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, const T* __restrict__ grad, Extent extent,
+__global__ void __launch_bounds__(kThreads, 4) table_gradient_kernel(Gradient g, const T* __restrict__ grad, Extent extent,
                                                                   T* __restrict__ out, Joins joins) {
   using R = Row<T, L>;
   constexpr int VEC = R::kVec;
   constexpr int kBatch = L == kSpan ? 4 : 8;   // rows of grad in flight per unit
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t s_bound[2];
-  const int lanes = g.lanes, units = kThreads / lanes;
-  const int unit = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+  const int lanes = g.lanes, units = g.units;
+  const int unit = threadIdx.x / lanes, lane = threadIdx.x - unit * lanes;
+  const bool live = unit < units;   // a few threads are left over where the lanes do not divide them
   const int tile_width = lanes * VEC;
   uint32_t* keys = reinterpret_cast<uint32_t*>(raw);
   uint32_t* entries = keys + kBlockItems;
@@ -204,6 +274,8 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   int* head_row = reinterpret_cast<int*>(tails + kThreads * VEC);
   int* tail_row = head_row + kThreads;
   int* tail_begun = tail_row + kThreads;
+  follow();
+  let_next_start();
   const uint32_t n = *g.count;
   const long long total = (long long)n + g.rows;
   // the block's share of the merge, its entries brought into shared memory
@@ -222,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   }
   __syncthreads();
   // the unit's share, places counted from `first`
-  const long long d0 = min(b0 + (long long)unit * g.items, b1), d1 = min(d0 + g.items, b1);
+  const long long d0 = live ? min(b0 + (long long)unit * g.items, b1) : b1, d1 = min(d0 + g.items, b1);
   uint32_t p0, p1;
   {
     auto search = [&](long long d) {
@@ -241,8 +313,11 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   const uint32_t r1 = (uint32_t)(d1 - first - p1);
   // whether row r has entries in earlier units
   bool begun_before = d0 < d1 && (p0 > 0 ? keys[p0 - 1] : before_first) == r;
-  const int col = blockIdx.y * tile_width + lane * VEC;   // the lane's first column
-  const bool in = col < g.width;
+  // the lane's first column; a last pack that would end behind the row is moved back into it
+  // (its first columns are then the lane's before, added up twice and written twice, alike)
+  const int first_col = blockIdx.y * tile_width + lane * VEC;
+  const bool in = live && first_col < g.width;
+  const int col = L == kSpan ? min(first_col, g.width - VEC) : first_col;
   float acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
@@ -253,10 +328,13 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   auto write = [&](uint32_t row, float (&sum)[VEC]) {   // columns of a row that may begin anywhere
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[i] *= g.scale;
-    T* to = out + (long long)row * g.width;
-    if (in) {
-      if (L == kSpan && R::ahead(to) != 0) R::store_by_element(to, col, g.width, R::words(sum));
-      else R::store(to, col, g.width, R::words(sum));
+    if (!in) return;
+    T* to = out + (long long)row * g.width + col;
+    if (L == kSpan && ((uintptr_t)to & 15)) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) to[i] = from_float<T>(sum[i]);
+    } else {
+      R::store(to, R::words(sum));
     }
   };
 
@@ -266,15 +344,10 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
 #pragma unroll
       for (int i = 0; i < VEC; ++i) my_heads[i] = acc[i];
     } else {
-      if (any) {
+      if (any || L != kSpan) {
         write(r, acc);
-      } else {
-        // zeros may be shifted: whole packs wherever the row begins, one more at its end
-        T* to = out + (long long)r * g.width;
-        const int e = col - R::ahead(to);
-        if (e < g.width) R::store(to, e, g.width, zero_pack<T, L>());
-        if (L == kSpan && lane == lanes - 1 && blockIdx.y + 1 == gridDim.y && e + VEC < g.width)
-          R::store(to, e + VEC, g.width, zero_pack<T, L>());
+      } else if (r % gridDim.y == blockIdx.y) {   // the tiles share the rows without entries
+        clear_row<T, L>(out + (long long)r * g.width, g.width, lane, lanes);
       }
       if (g.mask && lane == 0 && blockIdx.y == 0) g.mask[r] = any;
     }
@@ -285,11 +358,34 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
     ++r;
   };
 
+  // the rows of the next batches are called into L2 ahead of their loads, which costs no registers
+  const int tile_bytes = (int)sizeof(T) * min(tile_width, g.width - (int)blockIdx.y * tile_width);
+  const int lines = (tile_bytes + 127) / 128 + (L == kAligned ? 0 : 1);
+  auto call = [&](uint32_t from) {
+    for (int i = lane; i < kBatch * lines; i += lanes) {
+      const int b = i / lines, at = min((i - b * lines) * 128, tile_bytes - (int)sizeof(T));
+      if (from + b < p1)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(
+            grad + (long long)entries[from + b] * g.stride + blockIdx.y * tile_width) + at));
+    }
+  };
+  if (live) call(p0 + kBatch);
   for (uint32_t p = p0; p < p1; p += kBatch) {
+    if (live) call(p + 2 * kBatch);
     typename R::Raw v[kBatch];
+    auto load = [&](auto read) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (p + b < p1 && in) v[b] = R::load(grad + (long long)entries[p + b] * g.stride, col, g.width, extent);
+      for (int b = 0; b < kBatch; ++b)
+        if (p + b < p1 && in) v[b] = read(grad + (long long)entries[p + b] * g.stride + col);
+    };
+    bool inside = true;
+    if (L == kSpan && extent.checked) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (p + b < p1) inside = inside && extent.inside(grad + (long long)entries[p + b] * g.stride, g.width);
+    }
+    if (L != kSpan || inside) load([](const T* at) { return R::load(at); });
+    else load([](const T* at) { return R::load_elements(at); });
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
       if (p + b < p1) {
@@ -312,7 +408,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
 #pragma unroll
     for (int i = 0; i < VEC; ++i) my_tails[i] = acc[i];
   }
-  if (lane == 0) {
+  if (live && lane == 0) {
     head_row[unit] = my_head;
     tail_row[unit] = open ? (int)r : -1;
     tail_begun[unit] = open && !begun_before;
@@ -337,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
       unfinished = true;
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (col + i < g.width) joins.head[(long long)blockIdx.x * g.width + col + i] = sum[i];
+        if (in) joins.head[(long long)blockIdx.x * g.width + col + i] = sum[i];
       if (lane == 0 && blockIdx.y == 0) joins.head_row[blockIdx.x] = my_head;
     }
   }
@@ -358,7 +454,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (col + i < g.width) joins.tail[(long long)blockIdx.x * g.width + col + i] = sum[i];
+        if (in) joins.tail[(long long)blockIdx.x * g.width + col + i] = sum[i];
     }
     if (lane == 0 && blockIdx.y == 0) {
       joins.tail_row[blockIdx.x] = row;
@@ -374,6 +470,7 @@ __global__ void __launch_bounds__(kThreads) table_join_kernel(Joins joins, int w
                                                               T* __restrict__ out, uint8_t* __restrict__ mask) {
   __shared__ float part[kThreads];
   __shared__ int s_first;
+  follow();
   const int block = blockIdx.x, row = joins.head_row[block];
   if (row < 0) return;
   // the chain of open tails of this row: it begins at the nearest block where the row begins
@@ -407,7 +504,8 @@ constexpr int kMinItems = 8;        // items of a unit at least, or the searches
 // Most blocks a gradient can have (x dimension): its joins' rows.
 inline long long most_blocks(long long n, long long rows) {
   const long long total = n + rows, fewest = 8 * kMinItems;   // 8 units at least in a block
-  const long long full = (total + kBlockItems - 1) / kBlockItems + 148 * 8;
+  constexpr long long share = kBlockItems - kThreads;       // of a block whose units do not divide kBlockItems
+  const long long full = (total + share - 1) / share + 148 * 8;
   const long long tiny = (total + fewest - 1) / fewest;
   return full < tiny ? full : tiny;
 }
@@ -424,8 +522,8 @@ int launch_gradient(Gradient g, long long n, const void* grad, void* out, float*
     return e == cudaSuccess && blocks > 0 ? (blocks < 8 ? blocks : 8) : 2;
   }();
   const int packs = (g.width + VEC - 1) / VEC;
-  g.lanes = next_pow2(packs < 32 ? packs : 32);
-  const int units = kThreads / g.lanes, tile_width = g.lanes * VEC;
+  g.lanes = packs < 32 ? packs : 32;
+  const int units = g.units = kThreads / g.lanes, tile_width = g.lanes * VEC;
   const int tiles = (g.width + tile_width - 1) / tile_width;
   // equal blocks that fill the SMs a whole number of times
   const long long total = n + g.rows;
@@ -443,24 +541,23 @@ int launch_gradient(Gradient g, long long n, const void* grad, void* out, float*
   joins.head_row = (int*)(joins.tail + blocks * g.width);
   joins.tail_row = joins.head_row + blocks;
   joins.tail_begun = joins.tail_row + blocks;
-  table_gradient_kernel<T, L><<<dim3((unsigned)blocks, tiles), kThreads, shared, st>>>(
-      g, (const T*)grad, extent_of(grad, n, g.stride, g.width, sizeof(T)), (T*)out, joins);
-  CVHRF_LAUNCH_CHECK();
+  CVHRF_CUDA_TRY(launch_after(table_gradient_kernel<T, L>, dim3((unsigned)blocks, tiles), kThreads, shared, st, g,
+                              (const T*)grad, extent_of(grad, n, g.stride, g.width, sizeof(T)), (T*)out, joins));
+  count_launch(1);
   if (blocks == 1) return CVHRF_OK;
   const int columns = next_pow2(g.width < kThreads ? g.width : kThreads);
-  table_join_kernel<T><<<dim3((unsigned)blocks, (g.width + columns - 1) / columns), kThreads, 0, st>>>(
-      joins, g.width, columns, g.scale, (T*)out, g.mask);
-  CVHRF_LAUNCH_CHECK();
+  CVHRF_CUDA_TRY(launch_after(table_join_kernel<T>, dim3((unsigned)blocks, (g.width + columns - 1) / columns), kThreads,
+                              0, st, joins, g.width, columns, g.scale, (T*)out, g.mask));
+  count_launch(1);
   return CVHRF_OK;
 }
 
-// Units of the smallest power of two of lanes that holds a row, a warp at most; wider rows are
-// cut into tiles.
+// Units of as many lanes as a row has packs, a warp at most; wider rows are cut into tiles.
 template <typename T>
 int gradient(const void* grad, long long stride, int width, long long n, long long rows, float scale, void* out,
              uint8_t* mask, const uint32_t* keys, const uint32_t* entries, const uint32_t* count, float* joins,
              cudaStream_t st) {
-  const Gradient g{keys, entries, count, stride, (int)rows, width, 0, 0, scale, mask};
+  const Gradient g{keys, entries, count, stride, (int)rows, width, 0, 0, 0, scale, mask};
   if (rows_16(grad, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0)
     return launch_gradient<T, kAligned>(g, n, grad, out, joins, st);
   if (width >= kSpanWidth) return launch_gradient<T, kSpan>(g, n, grad, out, joins, st);
@@ -475,9 +572,9 @@ constexpr int kMaxWidth = 1 << 20;
 
 using namespace cvhrf;
 
-extern "C" int cvhrf_table_lookup(const void* table, long long rows, int width, long long row_stride, int dtype,
-                                  const void* index, int index_bytes, long long entries, float scale, void* out,
-                                  void* stream) {
+extern "C" int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const auto [table, index, out, rows, row_stride, entries, width, dtype, index_bytes, scale] = *args;
   if (!row_type_ok(dtype) || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth || row_stride < 0 ||
       (index_bytes != 4 && index_bytes != 8) || entries < 0)
     return CVHRF_EINVAL;
@@ -499,9 +596,10 @@ extern "C" size_t cvhrf_table_gradient_workspace_bytes(long long entries, long l
          (size_t)most_blocks(entries, rows) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int));
 }
 
-extern "C" int cvhrf_table_gradient(const void* grad, long long grad_stride, int dtype, int width, const void* index,
-                                    int index_bytes, long long entries, float scale, void* grad_table, long long rows,
-                                    uint8_t* row_mask, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* stream) {
+  if (!args) return CVHRF_EINVAL;
+  const auto [grad, index, grad_table, row_mask, workspace, workspace_bytes, grad_stride, entries, rows, width, dtype,
+              index_bytes, scale] = *args;
   if (!row_type_ok(dtype) || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth || grad_stride < 0 ||
       (index_bytes != 4 && index_bytes != 8) || entries < 0)
     return CVHRF_EINVAL;

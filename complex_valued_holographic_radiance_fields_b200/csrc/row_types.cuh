@@ -4,13 +4,12 @@
 //   kAligned  every row begins on 16 bytes and is a multiple of 16 bytes long: a pack is 16 bytes
 //             of the row, one load or store.
 //   kSpan     rows begin anywhere (an odd width, a slice).  Packs are 16-byte aligned on the side
-//             that is written, so that stores stay whole; the first and the last pack of a row
-//             are partial and stored by element.  A pack's elements lie in two aligned 16-byte
-//             words of the row that is read, which are shifted together.  By element, a warp needs
-//             4 (float32) or 8 (16 bits) times the instructions, and was bound by them: 141 us
-//             against 55 us for 1M rows of 59 floats.
+//             that is written, so that stores stay whole; the elements before the first and
+//             behind the last boundary (the edges) are moved one per lane.  A pack's elements lie
+//             in two aligned 16-byte words of the row that is read, which are shifted together.
 //   kElement  rows of a few elements: one element per lane (a span would be all edges).
 #pragma once
+#include <atomic>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -31,16 +30,23 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 
 enum Layout { kAligned, kSpan, kElement };
 
-// A tensor that is read: its first byte and the byte behind its last one.  A 16-byte word that
-// is not wholly inside is read by element.
+// A tensor that is read.  Where it does not begin and end on 16 bytes, the words at its ends are
+// not wholly inside, and the rows that touch them are read by element (Row::load_elements).
 struct Extent {
-  const char* begin;
-  const char* end;
+  const char* begin;   // its first byte
+  const char* end;     // the byte behind its last one
+  bool checked;
+  template <typename T>
+  __device__ __forceinline__ bool inside(const T* row, int width) const {
+    return !checked || (reinterpret_cast<const char*>(row) - 15 >= begin &&
+                        reinterpret_cast<const char*>(row + width) + 15 <= end);
+  }
 };
 
 inline Extent extent_of(const void* p, long long rows, long long stride, int width, size_t elem) {
   const char* b = (const char*)p;
-  return {b, rows > 0 ? b + ((rows - 1) * stride + width) * (long long)elem : b};
+  const char* e = rows > 0 ? b + ((rows - 1) * stride + width) * (long long)elem : b;
+  return {b, e, (((uintptr_t)b | (uintptr_t)e) & 15) != 0};
 }
 
 __device__ __forceinline__ uint4 zero_words() { return make_uint4(0u, 0u, 0u, 0u); }
@@ -87,9 +93,8 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// How packs of a row are read and written.  A pack is named by its first element `e` of the
-// row; it may begin before the row or end behind it (kSpan), what lies outside is undefined
-// when read and not written.
+// How packs of a row are read and written.  A pack is named by its first element of the row and
+// lies wholly inside it.
 template <typename T, Layout L>
 struct Row {
   static constexpr int kVec = 16 / (int)sizeof(T);
@@ -97,35 +102,40 @@ struct Row {
     uint4 a, b;
     uint32_t shift;
   };
-  // elements by which the written row is ahead of a 16-byte boundary
-  static __device__ __forceinline__ int ahead(const T* row) {
-    return L == kSpan ? (int)(((uintptr_t)row & 15) / sizeof(T)) : 0;
+  // elements of a row before its first boundary of 16 bytes
+  static __device__ __forceinline__ int head(const T* row, int width) {
+    if (L != kSpan) return 0;
+    const int ahead = (int)(((uintptr_t)row & 15) / sizeof(T));
+    return min(ahead ? kVec - ahead : 0, width);
   }
-  static __device__ __forceinline__ Raw load(const T* row, int e, int width, const Extent& x) {
+  static __device__ __forceinline__ Raw load(const T* from) {
     Raw r;
     if (L == kAligned) {
-      r.a = *reinterpret_cast<const uint4*>(row + e);
+      r.a = *reinterpret_cast<const uint4*>(from);
       return r;
     }
-    const char* p = reinterpret_cast<const char*>(row) + (long long)e * (int)sizeof(T);
+    const char* p = reinterpret_cast<const char*>(from);
     r.shift = (uint32_t)((uintptr_t)p & 15);
-    const char* at = p - r.shift;
-    if (at >= x.begin && at + 32 <= x.end) {
-      r.a = *reinterpret_cast<const uint4*>(at);
-      r.b = r.shift ? *reinterpret_cast<const uint4*>(at + 16) : zero_words();
-    } else {   // at the tensor's ends
-      r.shift = 0;
-      r.a = zero_words();
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
+    p -= r.shift;
+    r.a = *reinterpret_cast<const uint4*>(p);
+    // the word with the pack's last element (the same one again if the pack is aligned)
+    r.b = *reinterpret_cast<const uint4*>(p + (r.shift ? 16 : 0));
+    return r;
+  }
+  static __device__ __noinline__ uint4 load_words(const T* from) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (e + i >= 0 && e + i < width) {
-          if (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t*>(row)[e + i];
-          else w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[e + i] << ((i & 1) * 16);
-        }
-      r.a = make_uint4(w[0], w[1], w[2], w[3]);
-      r.b = zero_words();
+    for (int i = 0; i < kVec; ++i) {
+      if (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
+      else w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(from)[i] << ((i & 1) * 16);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ Raw load_elements(const T* from) {
+    Raw r;
+    r.a = load_words(from);
+    r.b = r.a;
+    r.shift = 0;
     return r;
   }
   static __device__ __forceinline__ uint4 words(const Raw& r) {
@@ -146,22 +156,7 @@ struct Row {
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
   }
-  static __device__ __forceinline__ void store(T* row, int e, int width, uint4 w) {
-    if (L == kAligned || (e >= 0 && e + kVec <= width)) {
-      *reinterpret_cast<uint4*>(row + e) = w;
-    } else {
-      store_by_element(row, e, width, w);
-    }
-  }
-  static __device__ __forceinline__ void store_by_element(T* row, int e, int width, uint4 w) {
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (e + i >= 0 && e + i < width) {
-        if (sizeof(T) == 4) reinterpret_cast<uint32_t*>(row)[e + i] = x[i];
-        else reinterpret_cast<uint16_t*>(row)[e + i] = (uint16_t)(x[i >> 1] >> ((i & 1) * 16));
-      }
-  }
+  static __device__ __forceinline__ void store(T* to, uint4 w) { *reinterpret_cast<uint4*>(to) = w; }
   static __device__ __forceinline__ void floats(const Raw& r, float (&f)[kVec]) { unpack(words(r), f, (const T*)nullptr); }
   static __device__ __forceinline__ uint4 words(const float (&f)[kVec]) { return pack(f, (const T*)nullptr); }
 };
@@ -170,13 +165,29 @@ template <typename T>
 struct Row<T, kElement> {
   static constexpr int kVec = 1;
   using Raw = T;
-  static __device__ __forceinline__ int ahead(const T*) { return 0; }
-  static __device__ __forceinline__ Raw load(const T* row, int e, int, const Extent&) { return row[e]; }
+  static __device__ __forceinline__ int head(const T*, int) { return 0; }
+  static __device__ __forceinline__ Raw load(const T* from) { return *from; }
+  static __device__ __forceinline__ Raw load_elements(const T* from) { return *from; }
   static __device__ __forceinline__ T words(const Raw& r) { return r; }
-  static __device__ __forceinline__ void store(T* row, int e, int, T w) { row[e] = w; }
-  static __device__ __forceinline__ void store_by_element(T* row, int e, int, T w) { row[e] = w; }
+  static __device__ __forceinline__ void store(T* to, T w) { *to = w; }
   static __device__ __forceinline__ void floats(const Raw& r, float (&f)[1]) { f[0] = to_float(r); }
   static __device__ __forceinline__ T words(const float (&f)[1]) { return from_float<T>(f[0]); }
+};
+
+// Where a row's whole packs begin (after `head` elements) and how many there are, and the `count`
+// elements outside them: edge(i) for i < count.
+struct Edges {
+  int head, packs, count, width;
+  template <typename R, typename T>
+  static __device__ __forceinline__ Edges of(const T* row, int width) {
+    Edges e;
+    e.head = R::head(row, width);
+    e.packs = (width - e.head) / R::kVec;
+    e.count = width - e.packs * R::kVec;
+    e.width = width;
+    return e;
+  }
+  __device__ __forceinline__ int edge(int i) const { return i < head ? i : width - count + i; }
 };
 
 template <typename T, Layout L>
@@ -185,11 +196,20 @@ __device__ __forceinline__ auto zero_pack() {
   else return zero_words();
 }
 
-// Packs that cover a row wherever it begins.
+// Zeros into a row.
 template <typename T, Layout L>
-__host__ __device__ constexpr int packs_of(int width) {
-  constexpr int vec = 16 / (int)sizeof(T);
-  return L == kElement ? width : L == kAligned ? width / vec : (width + vec - 1) / vec + 1;
+__device__ __forceinline__ void clear_row(T* row, int width, int lane, int lanes) {
+  using R = Row<T, L>;
+  const Edges e = Edges::of<R>(row, width);
+  for (int q = lane; q < e.packs; q += lanes) R::store(row + e.head + q * R::kVec, zero_pack<T, L>());
+  if (L == kSpan)
+    for (int i = lane; i < e.count; i += lanes) row[e.edge(i)] = from_float<T>(0.f);
+}
+
+// Whole packs of a row at most.
+template <typename T, Layout L>
+constexpr int packs_of(int width) {
+  return width / Row<T, L>::kVec;
 }
 
 inline size_t row_type_bytes(int dtype) { return dtype == CVHRF_F32 ? 4 : 2; }
@@ -208,5 +228,57 @@ inline bool rows_16(const void* p, long long stride, int width, size_t elem) {
 
 // A span's edges are up to two packs' worth of single elements, so it pays from this many on.
 constexpr int kSpanWidth = 32;
+
+// Rows are owned by `lanes` neighbouring lanes of a warp (not a power of two: rows of 5 packs
+// would leave 3 of 8 lanes idle); a warp has 32 / lanes owners.
+struct Owner {
+  int index, lane;   // the owner in its block, the lane in its owner
+  bool live;
+  static __device__ __forceinline__ Owner of(int lanes) {
+    const int in_warp = threadIdx.x & 31, each = 32 / lanes, o = in_warp / lanes;
+    return {(int)(threadIdx.x >> 5) * each + o, in_warp - o * lanes, o < each};
+  }
+};
+inline int owners_of(int threads, int lanes) { return threads / 32 * (32 / lanes); }
+// A row's lanes: its packs, a warp at most, or half of one where that leaves fewer idle.
+inline int lanes_for(int packs) {
+  if (packs <= 32) return packs < 1 ? 1 : packs;
+  return (packs + 31) / 32 * 2 > (packs + 15) / 16 ? 16 : 32;
+}
+
+// ---- launches that follow one another ----------------------------------------------------
+// A kernel launched with launch_after may start while the one before it ends; it calls
+// follow() before it touches memory, which waits until that one is done and its writes seen.
+__device__ __forceinline__ void follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// ... and the one before it says early that the next one may start.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <typename K>
+inline cudaError_t allow_shared(K* kernel, size_t bytes, std::atomic<unsigned long long>& devices) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (devices.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 }  // namespace cvhrf

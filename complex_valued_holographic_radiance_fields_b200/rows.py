@@ -24,6 +24,8 @@ call can be captured in a CUDA graph.  Every step runs in libcvhrf (cvhrf_table_
 cvhrf_table_gradient, cvhrf_group_rows, cvhrf_rows_to_groups, cvhrf_groups_to_rows); the
 reference, whose Gaussians own all their attributes, has no counterpart.
 """
+import functools
+
 import torch
 
 from . import _lib, profiling
@@ -34,16 +36,27 @@ _MAX_ENTRIES = 2 ** 30 - 1
 _MAX_WIDTH = 2 ** 20
 
 
-def _call(name, what, device, *args):
+def _call(name, what, device, args):
     """One libcvhrf call on `device` and its current stream, timed as `what`."""
+    f = getattr(_lib._lib or _lib.lib(), name)
     at = device.index
     if profiling._active is not None or at != torch._C._cuda_getDevice():
         with torch.cuda.device(device), profiling.timed(what):
-            rc = getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = f(args, torch.cuda.current_stream(device).cuda_stream)
     else:
-        rc = getattr(_lib._lib or _lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(at))
+        rc = f(args, torch._C._cuda_getCurrentRawStream(at))
     if rc:
         _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=256)
+def _gradient_workspace(n, num_rows, width):
+    return _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
+
+
+@functools.lru_cache(maxsize=256)
+def _group_workspace(n, num_groups):
+    return _lib.lib().cvhrf_group_rows_workspace_bytes(n, num_groups)
 
 
 def _rows(t, name):
@@ -87,8 +100,8 @@ def _lookup(table, index, scale):
     device = table.device
     index, nbytes, n = _index(index, device)
     out = torch.empty((*index.shape, width), dtype=table.dtype, device=device)
-    _call("cvhrf_table_lookup", "table_lookup", device, table.data_ptr(), table.shape[0], width, stride, code,
-          index.data_ptr(), nbytes, n, scale, out.data_ptr())
+    _call("cvhrf_table_lookup", "table_lookup", device, _lib.LOOKUP_ARGS.pack(
+        table.data_ptr(), index.data_ptr(), out.data_ptr(), table.shape[0], stride, n, width, code, nbytes, scale))
     return out
 
 
@@ -102,10 +115,11 @@ def _gradient(grad, index, num_rows, scale, with_mask):
     index, nbytes, n = _index(index, device)
     out = torch.empty((num_rows, width), dtype=grad.dtype, device=device)
     mask = torch.empty(num_rows, dtype=torch.uint8, device=device) if with_mask else None
-    need = _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
+    need = _gradient_workspace(n, num_rows, width)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call("cvhrf_table_gradient", "table_gradient", device, grad.data_ptr(), stride, code, width, index.data_ptr(),
-          nbytes, n, scale, out.data_ptr(), num_rows, mask.data_ptr() if with_mask else None, ws.data_ptr(), need)
+    _call("cvhrf_table_gradient", "table_gradient", device, _lib.GRADIENT_ARGS.pack(
+        grad.data_ptr(), index.data_ptr(), out.data_ptr(), mask.data_ptr() if with_mask else 0, ws.data_ptr(), need,
+        stride, n, num_rows, width, code, nbytes, scale))
     return out, mask
 
 
@@ -166,42 +180,42 @@ def group_rows(index, num_groups):
     group.  Entries outside [0, num_groups) come behind the last group and have slot -1."""
     if not index.is_cuda:
         raise ValueError("index must be a CUDA tensor")
-    if index.dim() not in (1, 2) or (index.dim() == 2 and index.shape[1] < 1):
-        raise ValueError(f"index must be (N,) or (N, k) with k >= 1, got {tuple(index.shape)}")
+    shape = index.shape
+    choices = 1 if len(shape) == 1 else shape[1] if len(shape) == 2 else 0
+    if choices < 1:
+        raise ValueError(f"index must be (N,) or (N, k) with k >= 1, got {tuple(shape)}")
     if not 1 <= num_groups < 2 ** 31 - 1:
         raise ValueError(f"num_groups must be in [1, 2^31 - 1), got {num_groups}")
     device = index.device
-    shape = index.shape
     index, nbytes, n = _index(index, device)
     order = torch.empty(n, dtype=torch.int32, device=device)
     slots = torch.empty(shape, dtype=torch.int32, device=device)
     offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
-    need = _lib.lib().cvhrf_group_rows_workspace_bytes(n, num_groups)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call("cvhrf_group_rows", "group_rows", device, index.data_ptr(), nbytes, n, num_groups, order.data_ptr(),
-          slots.data_ptr(), offsets.data_ptr(), ws.data_ptr(), need)
-    return RowGroups(order, slots, offsets, num_groups, shape[0], shape[1] if len(shape) == 2 else 1)
+    need = _group_workspace(n, num_groups)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call("cvhrf_group_rows", "group_rows", device, _lib.GROUP_ARGS.pack(
+        index.data_ptr(), order.data_ptr(), slots.data_ptr(), offsets.data_ptr(), ws.data_ptr() if need else 0, need,
+        n, num_groups, nbytes))
+    return RowGroups(order, slots, offsets, num_groups, shape[0], choices)
 
 
 def _to_groups(x, groups):
     x, code, width, stride = _rows(x, "x")
     device, n, k = x.device, groups.num_rows, groups.choices
     out = torch.empty((n * k, width), dtype=x.dtype, device=device)
-    _call("cvhrf_rows_to_groups", "rows_to_groups", device, x.data_ptr(), stride, code, n, k, width,
-          groups.slots.data_ptr(), groups._used(), out.data_ptr())
+    _call("cvhrf_rows_to_groups", "rows_to_groups", device, _lib.MOVES_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), groups.order.data_ptr(), groups.slots.data_ptr(), groups._used(), 0, n, stride, k,
+        width, code, 0))
     return out
-
-
-def _weights(weights):
-    return (None, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
 
 
 def _to_rows(y, groups, weights):
     y, code, width, stride = _rows(y, "y")
     device, n = y.device, groups.num_rows
     out = torch.empty((n, width), dtype=y.dtype, device=device)
-    _call("cvhrf_groups_to_rows", "groups_to_rows", device, y.data_ptr(), stride, code, n, groups.choices, width,
-          groups.slots.data_ptr(), *_weights(weights), out.data_ptr())
+    w, w_code = (0, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
+    _call("cvhrf_groups_to_rows", "groups_to_rows", device, _lib.MOVES_ARGS.pack(
+        y.data_ptr(), out.data_ptr(), 0, groups.slots.data_ptr(), 0, w, n, stride, groups.choices, width, code, w_code))
     return out
 
 
@@ -233,10 +247,11 @@ class GroupsToRows(torch.autograd.Function):
         need_y, _, need_w = ctx.needs_input_grad
         grad_y = torch.empty(y.shape, dtype=y.dtype, device=device) if need_y else None
         grad_w = torch.empty_like(weights) if need_w else None
-        _call("cvhrf_groups_to_rows_backward", "groups_to_rows_backward", device, grad.data_ptr(), grad_stride,
-              y.data_ptr(), stride, code, groups.num_rows, groups.choices, width, groups.slots.data_ptr(),
-              groups._used(), *_weights(weights), grad_y.data_ptr() if need_y else None,
-              grad_w.data_ptr() if need_w else None)
+        w, w_code = (0, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
+        _call("cvhrf_groups_to_rows_backward", "groups_to_rows_backward", device, _lib.MOVES_BACKWARD_ARGS.pack(
+            grad.data_ptr(), y.data_ptr(), groups.order.data_ptr(), groups.slots.data_ptr(), groups._used(), w,
+            grad_y.data_ptr() if need_y else 0, grad_w.data_ptr() if need_w else 0, groups.num_rows, grad_stride,
+            stride, groups.choices, width, code, w_code))
         return grad_y, None, grad_w
 
 

@@ -543,6 +543,10 @@ int cvhrf_hologram_field_backward(const void* holo, int C, long long n, const fl
 /* ---- rows shared by many entries, and rows sorted by group ------------------- */
 /*
  * Element types of rows.  Sums are float32 whatever the type; a result is rounded once.
+ * Rows read may be any `stride` elements apart (0: one row for all), rows written are
+ * contiguous.  Workspaces are aligned to 16 bytes.  Entries are below 2^30, a row is at
+ * most 2^20 elements.  No counterpart in the reference, whose Gaussians own all their
+ * attributes.
  */
 #define CVHRF_F32 0
 #define CVHRF_BF16 1
@@ -550,54 +554,94 @@ int cvhrf_hologram_field_backward(const void* holo, int C, long long n, const fl
 /*
  * Lookup of table rows (a codebook of attributes that many Gaussians share):
  *   out[t] = scale * table[index[t]],  t < entries
- * table: rows x width of type `dtype`, `row_stride` elements between rows; out: entries x
- * width, contiguous.  index: int32 or int64 (index_bytes 4 or 8).  An index outside
- * [0, rows) gives a row of zeros.  entries < 2^30, width <= 2^20.  No counterpart in the
- * reference, whose Gaussians own all their attributes.
+ * table: rows x width of type `dtype`; index: int32 or int64 (index_bytes 4 or 8).  An
+ * index outside [0, rows) gives a row of zeros.
  */
-int cvhrf_table_lookup(const void* table, long long rows, int width, long long row_stride, int dtype,
-                       const void* index, int index_bytes, long long entries, float scale, void* out, void* stream);
+typedef struct {
+  const void* table;
+  const void* index;
+  void* out;
+  long long rows, row_stride, entries;
+  int width, dtype, index_bytes;
+  float scale;
+} cvhrf_lookup_args;
+int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream);
 /*
  * Its gradient: grad_table[v] = scale * sum of grad[t] over the entries with index[t] = v
- * (zeros where there is none), every row written; row_mask[v] (optional, may be null) = 1
- * where there is one, the mask cvhrf_sparse_adam_masked takes.  The order of the sums is
- * fixed (the entries' order, joined between blocks in a fixed order): results repeat bit
- * for bit.  An entry whose index is outside [0, rows) is left out and its row not read.
+ * (zeros where there is none), every row written; row_mask[v] (may be null) = 1 where
+ * there is one, the mask cvhrf_sparse_adam_masked takes.  The order of the sums is fixed
+ * (the entries' order, joined between blocks in a fixed order): results repeat bit for
+ * bit.  An entry whose index is outside [0, rows) is left out and its row not read.
  */
+typedef struct {
+  const void* grad;
+  const void* index;
+  void* grad_table;
+  uint8_t* row_mask;
+  void* workspace;
+  size_t workspace_bytes;
+  long long grad_stride, entries, rows;
+  int width, dtype, index_bytes;
+  float scale;
+} cvhrf_gradient_args;
 size_t cvhrf_table_gradient_workspace_bytes(long long entries, long long rows, int width);
-int cvhrf_table_gradient(const void* grad, long long grad_stride, int dtype, int width, const void* index,
-                         int index_bytes, long long entries, float scale, void* grad_table, long long rows,
-                         uint8_t* row_mask, void* workspace, size_t workspace_bytes, void* stream);
+int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* stream);
 /*
  * The entries of an index array sorted stably by value (the group: a depth plane, an owner):
  * order[p] = the entry at place p, slots[e] = the place of entry e, offsets[g] = where group
  * g begins (groups + 1 values; the last is where the last group ends).  Entries whose value
- * is outside [0, groups) follow behind the last group and have slot -1.
+ * is outside [0, groups) follow behind the last group and have slot -1.  The workspace query
+ * returns 0 where none is needed.
  */
+typedef struct {
+  const void* index;
+  int* order;
+  int* slots;
+  int* offsets;
+  void* workspace;
+  size_t workspace_bytes;
+  long long entries;
+  int groups, index_bytes;
+} cvhrf_group_args;
 size_t cvhrf_group_rows_workspace_bytes(long long entries, int groups);
-int cvhrf_group_rows(const void* index, int index_bytes, long long entries, int groups, int* order, int* slots,
-                     int* offsets, void* workspace, size_t workspace_bytes, void* stream);
+int cvhrf_group_rows(const cvhrf_group_args* args, void* stream);
 /*
  * Rows to their groups and back.  Row n has `choices` entries n * choices + j with places
- * slots[n * choices + j]; used = (device) the number of places that belong to a group
- * (offsets + groups of cvhrf_group_rows).
- *   cvhrf_rows_to_groups:  out[slot] = x[n]  (n * choices rows; those from *used on are zeros)
- *   cvhrf_groups_to_rows:  out[n] = sum_j weights[n, j] y[slots[n, j]]  (float32 sum; entries
- *     left out count nothing; weights null: ones).  Without weights it is the gradient of
- *     cvhrf_rows_to_groups.
+ * slots[n * choices + j], order is cvhrf_group_rows' other way round; used = (device) the
+ * number of places that belong to a group (offsets + groups of cvhrf_group_rows).
+ *   cvhrf_rows_to_groups:  to[slot] = from[n]  (n * choices rows; those from *used on are zeros)
+ *   cvhrf_groups_to_rows:  to[n] = sum_j weights[n, j] from[slots[n, j]]  (float32 sum; entries
+ *     left out count nothing; weights null: ones; order and used are not read).  Without weights it is the
+ *     gradient of cvhrf_rows_to_groups.
  *   cvhrf_groups_to_rows_backward: grad_y[slot] = weights[n, j] grad[n] (rows from *used on:
  *     zeros), grad_weights[n, j] = <grad[n], y[slot]> (0 where left out); either may be null.
- * weights are float32 or of type `dtype`, n x choices, contiguous; x, y and grad take a row
- * stride, outputs are contiguous.
+ * weights are float32 or of type `dtype`, n x choices, contiguous.
  */
-int cvhrf_rows_to_groups(const void* x, long long x_stride, int dtype, long long n, int choices, int width,
-                         const int* slots, const int* used, void* out, void* stream);
-int cvhrf_groups_to_rows(const void* y, long long y_stride, int dtype, long long n, int choices, int width,
-                         const int* slots, const void* weights, int weights_dtype, void* out, void* stream);
-int cvhrf_groups_to_rows_backward(const void* grad, long long grad_stride, const void* y, long long y_stride,
-                                  int dtype, long long n, int choices, int width, const int* slots, const int* used,
-                                  const void* weights, int weights_dtype, void* grad_y, void* grad_weights,
-                                  void* stream);
+typedef struct {
+  const void* from;
+  void* to;
+  const int* order;
+  const int* slots;
+  const int* used;
+  const void* weights;
+  long long n, stride;
+  int choices, width, dtype, weights_dtype;
+} cvhrf_moves_args;
+typedef struct {
+  const void* grad;
+  const void* y;
+  const int* order;
+  const int* slots;
+  const int* used;
+  const void* weights;
+  void* grad_y;
+  void* grad_weights;
+  long long n, grad_stride, y_stride;
+  int choices, width, dtype, weights_dtype;
+} cvhrf_moves_backward_args;
+int cvhrf_rows_to_groups(const cvhrf_moves_args* args, void* stream);
+int cvhrf_groups_to_rows(const cvhrf_moves_args* args, void* stream);
+int cvhrf_groups_to_rows_backward(const cvhrf_moves_backward_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,8 @@ used), a product by u, and the rounding to t by eps(t) / 2 of the value (or half
 subnormal).  No constant beyond these is added, except 1 + 2^-10 for the terms of second order.
 """
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -500,13 +502,17 @@ def test_refusals_need_no_gpu():
 def test_c_abi_refusals_need_no_gpu():
     """Bad arguments come back as a status before anything is launched."""
     L = _lib.lib()
-    p = ctypes.c_void_p(256)   # never read: every call is refused
+    p = 256   # never read: every call is refused
+    for f in (L.cvhrf_table_lookup, L.cvhrf_table_gradient, L.cvhrf_group_rows, L.cvhrf_rows_to_groups,
+              L.cvhrf_groups_to_rows, L.cvhrf_groups_to_rows_backward):
+        assert f(None, None) == 1
 
-    def lookup(table=p, rows=4, width=4, stride=4, dtype=0, index=p, bytes_=4, n=2, out=p):
-        return L.cvhrf_table_lookup(table, rows, width, stride, dtype, index, bytes_, n, 1.0, out, None)
+    def lookup(table=p, index=p, out=p, rows=4, stride=4, n=2, width=4, dtype=0, nbytes=4):
+        return L.cvhrf_table_lookup(_lib.LOOKUP_ARGS.pack(table, index, out, rows, stride, n, width, dtype, nbytes, 1.0),
+                                    None)
 
-    for bad in (dict(table=None), dict(rows=-1), dict(rows=2 ** 31), dict(width=0), dict(width=2 ** 20 + 1),
-                dict(stride=-1), dict(dtype=3), dict(index=None), dict(bytes_=2), dict(n=-1), dict(out=None)):
+    for bad in (dict(table=0), dict(rows=-1), dict(rows=2 ** 31), dict(width=0), dict(width=2 ** 20 + 1),
+                dict(stride=-1), dict(dtype=3), dict(index=0), dict(nbytes=2), dict(n=-1), dict(out=0)):
         assert lookup(**bad) == 1, bad
     assert lookup(n=2 ** 30) == 4
     assert lookup(n=0) == 0
@@ -514,33 +520,63 @@ def test_c_abi_refusals_need_no_gpu():
     need = L.cvhrf_table_gradient_workspace_bytes(1000, 10, 8)
     assert need > 0 and L.cvhrf_table_gradient_workspace_bytes(-1, 10, 8) == 0
 
-    def gradient(grad=p, stride=8, dtype=0, width=8, index=p, bytes_=8, n=1000, out=p, rows=10, ws=p, nbytes=need):
-        return L.cvhrf_table_gradient(grad, stride, dtype, width, index, bytes_, n, 1.0, out, rows, None, ws, nbytes,
-                                      None)
+    def gradient(grad=p, index=p, out=p, ws=p, need=need, stride=8, n=1000, rows=10, width=8, dtype=0, nbytes=8):
+        return L.cvhrf_table_gradient(_lib.GRADIENT_ARGS.pack(grad, index, out, 0, ws, need, stride, n, rows, width,
+                                                              dtype, nbytes, 1.0), None)
 
-    for bad in (dict(grad=None), dict(stride=-1), dict(dtype=-1), dict(width=0), dict(index=None), dict(bytes_=1),
-                dict(n=-1), dict(out=None), dict(rows=-1)):
+    for bad in (dict(grad=0), dict(stride=-1), dict(dtype=-1), dict(width=0), dict(index=0), dict(nbytes=1),
+                dict(n=-1), dict(out=0), dict(rows=-1), dict(ws=264)):
         assert gradient(**bad) == 1, bad
-    assert gradient(ws=None) == 2 and gradient(nbytes=need - 1) == 2
+    assert gradient(ws=0) == 2 and gradient(need=need - 1) == 2
     assert gradient(n=2 ** 30) == 4
 
-    need = L.cvhrf_group_rows_workspace_bytes(1000, 5)
+    need = L.cvhrf_group_rows_workspace_bytes(10000, 5)
+    assert need > 0 and L.cvhrf_group_rows_workspace_bytes(100, 5) == 0
 
-    def group(index=p, bytes_=4, n=1000, groups=5, order=p, slots=p, offsets=p, ws=p, nbytes=need):
-        return L.cvhrf_group_rows(index, bytes_, n, groups, order, slots, offsets, ws, nbytes, None)
+    def group(index=p, order=p, slots=p, offsets=p, ws=p, need=need, n=10000, groups=5, nbytes=4):
+        return L.cvhrf_group_rows(_lib.GROUP_ARGS.pack(index, order, slots, offsets, ws, need, n, groups, nbytes), None)
 
-    for bad in (dict(index=None), dict(bytes_=3), dict(n=-1), dict(groups=0), dict(order=None), dict(slots=None),
-                dict(offsets=None)):
+    for bad in (dict(index=0), dict(nbytes=3), dict(n=-1), dict(groups=0), dict(order=0), dict(slots=0),
+                dict(offsets=0), dict(ws=264)):
         assert group(**bad) == 1, bad
-    assert group(ws=None) == 2 and group(nbytes=need - 1) == 2 and group(n=2 ** 30) == 4
+    assert group(ws=0) == 2 and group(need=need - 1) == 2 and group(n=2 ** 30) == 4
 
-    assert L.cvhrf_rows_to_groups(p, 4, 0, 2 ** 29, 2, 4, p, p, p, None) == 4
-    assert L.cvhrf_rows_to_groups(p, 4, 0, 5, 0, 4, p, p, p, None) == 1
-    assert L.cvhrf_rows_to_groups(p, 4, 0, 5, 1, 4, None, p, p, None) == 1
-    assert L.cvhrf_groups_to_rows(p, 4, 1, 5, 1, 4, p, p, 2, p, None) == 1     # weights of another 16-bit type
-    assert L.cvhrf_groups_to_rows(p, 4, 0, 5, 1, 4, p, None, 0, None, None) == 1
-    assert L.cvhrf_groups_to_rows_backward(p, 4, p, 4, 0, 5, 1, 4, p, p, None, 0, p, p, None) == 1
-    assert L.cvhrf_groups_to_rows_backward(p, 4, None, 4, 0, 5, 1, 4, p, p, p, 0, p, p, None) == 1
+    def moves(f, a=p, to=p, order=p, slots=p, used=p, w=0, n=5, stride=4, k=1, width=4, dtype=0, w_dtype=0):
+        return f(_lib.MOVES_ARGS.pack(a, to, order, slots, used, w, n, stride, k, width, dtype, w_dtype), None)
+
+    for f in (L.cvhrf_rows_to_groups, L.cvhrf_groups_to_rows):
+        for bad in (dict(a=0), dict(to=0), dict(slots=0), dict(n=-1), dict(stride=-1), dict(k=0), dict(width=0),
+                    dict(dtype=5)):
+            assert moves(f, **bad) == 1, bad
+        assert moves(f, n=2 ** 29, k=2) == 4
+    assert moves(L.cvhrf_rows_to_groups, used=0) == 1 and moves(L.cvhrf_rows_to_groups, order=0) == 1
+    assert moves(L.cvhrf_groups_to_rows, w=p, dtype=1, w_dtype=2) == 1      # weights of another 16-bit type
+
+    def backward(grad=p, y=p, order=p, slots=p, used=p, w=p, dy=p, dw=p, dtype=0, w_dtype=0):
+        return L.cvhrf_groups_to_rows_backward(_lib.MOVES_BACKWARD_ARGS.pack(
+            grad, y, order, slots, used, w, dy, dw, 5, 4, 4, 1, 4, dtype, w_dtype), None)
+
+    for bad in (dict(grad=0), dict(y=0), dict(order=0), dict(slots=0), dict(used=0), dict(w=0), dict(dtype=2, w_dtype=1)):
+        assert backward(**bad) == 1, bad
+    assert backward(dy=0, dw=0) == 0                                        # nothing asked for
+
+
+def test_argument_structs_match_the_header():
+    """The packed layouts have the sizes a C compiler gives the structs."""
+    sizes = {}
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "cvhrf.h")).read()
+    for body, name in re.findall(r"typedef struct \{([^{}]*)\} (cvhrf_\w+_args);", src):
+        fields = []
+        for line in body.strip().splitlines():
+            kind, names = re.match(r"\s*((?:const )?(?:long long|\w+)\s?\*?)\s*(.*);", line).groups()
+            c = (ctypes.c_void_p if "*" in kind else
+                 {"long long": ctypes.c_longlong, "int": ctypes.c_int, "float": ctypes.c_float,
+                  "size_t": ctypes.c_size_t}[kind.strip()])
+            fields += [(f.strip(), c) for f in names.split(",")]
+        sizes[name] = ctypes.sizeof(type(name, (ctypes.Structure,), {"_fields_": fields}))
+    assert sizes == {"cvhrf_lookup_args": _lib.LOOKUP_ARGS.size, "cvhrf_gradient_args": _lib.GRADIENT_ARGS.size,
+                     "cvhrf_group_args": _lib.GROUP_ARGS.size, "cvhrf_moves_args": _lib.MOVES_ARGS.size,
+                     "cvhrf_moves_backward_args": _lib.MOVES_BACKWARD_ARGS.size}
 
 
 @gpu
