@@ -43,6 +43,30 @@ struct Target {
   int next_shift, next_radix;
 };
 
+// A launch's share of Zeros: its blocks from `first_block` on write the zeros.
+struct Fill {
+  Zeros z;
+  int first_block, part, parts;
+};
+
+__device__ __forceinline__ void fill_zeros(const Fill& f) {
+  const int block = blockIdx.x - f.first_block, blocks = gridDim.x - f.first_block;
+  for (int k = 0; k < 2; ++k) {
+    char* at = (char*)f.z.at[k];
+    const unsigned long long head = min((unsigned long long)(-(long long)(uintptr_t)at & 15), f.z.bytes[k]);
+    const unsigned long long words = (f.z.bytes[k] - head) >> 4, tail = head + (words << 4);
+    if (f.part == 0 && block == 0) {   // the ends that are not whole words
+      for (unsigned long long i = threadIdx.x; i < head; i += kThreads) at[i] = 0;
+      for (unsigned long long i = tail + threadIdx.x; i < f.z.bytes[k]; i += kThreads) at[i] = 0;
+    }
+    uint4* w = reinterpret_cast<uint4*>(at + head);
+    const unsigned long long begin = words * f.part / f.parts, end = words * (f.part + 1) / f.parts;
+    for (unsigned long long i = begin + (unsigned long long)block * kThreads + threadIdx.x; i < end;
+         i += (unsigned long long)blocks * kThreads)
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // Key of item i, kNone if it is left out (keys are below 2^31).
 __device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
   if (s.bytes == 0) return s.keys[i];
@@ -54,13 +78,15 @@ __device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
 // counts[chunk][digit] over the keys of each chunk; the `clear` words behind the matrix, where
 // the later passes count, are set to zero.
 __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, uint32_t chunk, int shift, int radix,
-                                                               uint32_t* __restrict__ counts, int clear) {
+                                                               uint32_t* __restrict__ counts, int clear, Fill fill) {
   let_next_start();
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
+  const uint32_t chunks = fill.first_block;
   constexpr int kCopies = 8;   // histograms, so that equal digits of different warps do not meet
   __shared__ uint32_t h[kCopies][kMaxRadix];
   for (int i = threadIdx.x; i < kCopies * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
-  for (int i = blockIdx.x * kThreads + threadIdx.x; i < clear; i += gridDim.x * kThreads)
-    counts[(size_t)gridDim.x * radix + i] = 0;
+  for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < (uint32_t)clear; i += chunks * kThreads)
+    counts[(size_t)chunks * radix + i] = 0;
   __syncthreads();
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   uint32_t* mine = h[(threadIdx.x >> 5) % kCopies];
@@ -181,12 +207,15 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
                                                                  const uint32_t* __restrict__ n_dev, uint32_t chunk,
                                                                  int shift, int radix,
-                                                                 const uint32_t* __restrict__ counts, Target out) {
+                                                                 const uint32_t* __restrict__ counts, Target out,
+                                                                 Fill fill) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   follow();
   let_next_start();
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
+  const int chunks = fill.first_block;
   if (n_dev) n = min(n, *n_dev);
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   const uint32_t mask = radix - 1;
@@ -216,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int c = share + i * kShares;
-        v[i] = c < (int)gridDim.x ? reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q] : make_uint4(0, 0, 0, 0);
+        v[i] = c < chunks ? reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q] : make_uint4(0, 0, 0, 0);
       }
       uint4 before = make_uint4(0, 0, 0, 0), all = before;
 #pragma unroll
@@ -269,11 +298,13 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
 }
 
 // All passes on up to kTile keys, in one block.
-__global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t n, int bits, int passes, Target out) {
+__global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t n, int bits, int passes, Target out,
+                                                              Fill fill) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   let_next_start();
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
   uint32_t key[kItems], entry[kItems], place[kItems];
   uint32_t kept = n;
   int done = 0;
@@ -356,10 +387,16 @@ inline Chunks chunks_for(long long n) {
 
 inline int passes_for(int bits) { return (bits + 7) / 8; }
 
+// Blocks for zeros beside a launch: 64 KB each at least, one per SM at most.
+inline int fill_blocks(const Zeros& z, int parts) {
+  const unsigned long long b = ((z.bytes[0] + z.bytes[1]) / parts + 65535) / 65536;
+  return (int)(b < 148 ? b : 148);
+}
+
 // All passes over the low `bits` bits.  The last one writes `out`; the ones before it go to and
 // fro between the two buffers of keys and entries at `buffers` (of `len` words each).
 int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* buffers, size_t len, uint32_t* count,
-                Target out, cudaStream_t st) {
+                Target out, const Zeros& zeros, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed{0};
   CVHRF_CUDA_TRY(allow_shared(chunk_scatter_kernel, sizeof(Shared), allowed));
   const Chunks c = chunks_for(n);
@@ -373,7 +410,9 @@ int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* b
   }
   int clear = 0;
   for (int p = 1; p < passes; ++p) clear += c.count * radix[p];
-  chunk_count_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, c.size, 0, radix[0], counts, clear);
+  const int parts = passes + 1, more = fill_blocks(zeros, parts);
+  chunk_count_kernel<<<c.count + more, kThreads, 0, st>>>(src, (uint32_t)n, c.size, 0, radix[0], counts, clear,
+                                                          Fill{zeros, c.count, 0, parts});
   CVHRF_LAUNCH_CHECK();
   for (int p = 0; p < passes; ++p) {
     uint32_t* to = buffers + (p & 1) * 2 * len;
@@ -381,8 +420,9 @@ int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* b
     Target t = out;
     if (p + 1 < passes) t = Target{to, to + len, nullptr, nullptr, 0, nullptr, next, shift[p + 1], radix[p + 1]};
     t.count = p == 0 ? count : nullptr;
-    CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count), kThreads, sizeof(Shared), st, src, (uint32_t)n,
-                                p == 0 ? nullptr : count, c.size, shift[p], radix[p], counts, t));
+    CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count + more), kThreads, sizeof(Shared), st, src,
+                                (uint32_t)n, p == 0 ? nullptr : count, c.size, shift[p], radix[p], counts, t,
+                                Fill{zeros, c.count, p + 1, parts}));
     count_launch(1);
     src = Source{nullptr, 0, to, to + len, src.rows, 1};
     counts = next;
@@ -390,10 +430,12 @@ int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* b
   return CVHRF_OK;
 }
 
-int small_sort(const Source& src, long long n, int bits, Target out, cudaStream_t st) {
+int small_sort(const Source& src, long long n, int bits, Target out, const Zeros& zeros, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed{0};
   CVHRF_CUDA_TRY(allow_shared(small_sort_kernel, sizeof(Shared), allowed));
-  small_sort_kernel<<<1, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits, passes_for(bits), out);
+  small_sort_kernel<<<1 + fill_blocks(zeros, 1), kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits,
+                                                                                 passes_for(bits), out,
+                                                                                 Fill{zeros, 1, 0, 1});
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;
 }
@@ -409,7 +451,8 @@ size_t group_sort_words(long long n) {
 }
 
 int group_sort(const void* index, int index_bytes, long long n, long long rows, bool keep_outside, uint32_t* scratch,
-               cudaStream_t st, const uint32_t** keys, const uint32_t** entries, const uint32_t** count_dev) {
+               const Zeros& zeros, cudaStream_t st, const uint32_t** keys, const uint32_t** entries,
+               const uint32_t** count_dev) {
   uint32_t* count = scratch;
   *count_dev = count;
   const size_t len = align_up((size_t)n, 64);
@@ -420,8 +463,8 @@ int group_sort(const void* index, int index_bytes, long long n, long long rows, 
   *keys = to;
   *entries = to + len;
   const Target out{to, to + len, nullptr, nullptr, 0, count, nullptr, 0, 0};
-  if (n <= kTile) return small_sort(src, n, bits, out, st);
-  return sort_chunks(src, n, bits, scratch + 64, buffers, len, count, out, st);
+  if (n <= kTile) return small_sort(src, n, bits, out, zeros, st);
+  return sort_chunks(src, n, bits, scratch + 64, buffers, len, count, out, zeros, st);
 }
 
 }  // namespace cvhrf
@@ -452,11 +495,12 @@ extern "C" int cvhrf_group_rows(const cvhrf_group_args* args, void* stream) {
   const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)groups, 1};
   const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr, nullptr, 0, 0};
   const int bits = bits_for((unsigned long long)groups + 1);
-  if (entries <= kTile) return small_sort(src, entries, bits, out, st);
+  const Zeros none{};
+  if (entries <= kTile) return small_sort(src, entries, bits, out, none, st);
   // up to 255 groups (and the entries left out) one pass writes everything
-  if (groups < kMaxRadix) return sort_chunks(src, entries, bits, scratch + 64, nullptr, 0, scratch, out, st);
+  if (groups < kMaxRadix) return sort_chunks(src, entries, bits, scratch + 64, nullptr, 0, scratch, out, none, st);
   const uint32_t *keys, *sorted, *count;
-  const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, st, &keys, &sorted, &count);
+  const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, none, st, &keys, &sorted, &count);
   if (rc) return rc;
   const long long most = entries > (long long)groups + 1 ? entries : (long long)groups + 1;
   CVHRF_CUDA_TRY(launch_after(places_kernel, dim3((unsigned)((most + 255) / 256)), 256, 0, st, keys, sorted,

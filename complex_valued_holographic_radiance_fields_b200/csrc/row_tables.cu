@@ -6,14 +6,12 @@
 // Both are bound by memory: the lookup reads the distinct rows and writes T rows; the
 // gradient reads T rows and writes V.
 //
-// The gradient sorts the entries by row (row_groups.cu) and merges the sorted list with the
-// list of row ends 0 .. V-1: an item is either an entry (add its row) or a row end (write the
-// sum, zeros for a row without entries, and start the next).  Every unit of lanes takes an
-// equal share of the T + V items, found by one binary search on its diagonal of the merge, so
-// neither a row with very many entries nor a long stretch of rows with none holds up a block,
-// and the table is written once without being cleared first.  A row whose entries lie in
-// several units is joined in the order of the units: inside a block through shared memory,
-// between blocks by table_join_kernel.  The order of every sum is fixed, so results repeat.
+// The gradient sorts the entries by row (row_groups.cu), which also sets the table to zero
+// beside its own work, and adds up runs of entries with the same row.  Every unit of lanes takes
+// an equal share of the sorted entries, whatever rows they belong to, so a row with very many
+// entries holds up nobody.  A row whose entries lie in several units is joined in the order of
+// the units: inside a block through shared memory, between blocks by table_join_kernel.  The
+// order of every sum is fixed, so results repeat.
 #include "row_groups.cuh"
 #include "row_types.cuh"
 #include "row_tiles.cuh"
@@ -208,16 +206,16 @@ int lookup(const void* table, long long rows, int width, long long stride, const
 }
 
 // ---- gradient -------------------------------------------------------------------------
-constexpr int kBlockItems = 2048;   // most items of a block: its entries are staged in shared memory
+constexpr int kBlockItems = 1024;   // most entries of a block, staged in shared memory
 
 // What a block leaves for table_join_kernel: the part of a row that began in an earlier
-// block and ends in this one (head), and of the row that is open at its end (tail).
+// block and ends in this one (head), and of the row that goes on behind its end (tail).
 struct Joins {
   float* head;        // block x width
   float* tail;        // block x width
   int* head_row;      // -1: none
   int* tail_row;      // -1: none
-  int* tail_begun;    // the open row's first entry is in this block
+  int* tail_begun;    // the row's first entry is in this block
 };
 
 struct Gradient {
@@ -225,239 +223,199 @@ struct Gradient {
   const uint32_t* entries;   // the entry of each
   const uint32_t* count;     // how many
   long long stride;          // elements between the rows of grad
-  int rows, width;
+  int width;
   int lanes, units;          // lanes of a unit (up to 32), units of a block
-  int items;                 // items of a unit
+  int items;                 // entries of a unit
   float scale;
   uint8_t* mask;             // may be null
 };
 
-// Entries among the first d items of the merge: entry i comes before row end j iff keys[i] <= j,
-// so it is the first i with keys[i] > d - 1 - i.  32 probes at a time; the whole warp calls it.
-__device__ __forceinline__ uint32_t entries_before(const uint32_t* __restrict__ keys, uint32_t n, uint32_t rows,
-                                                   long long d) {
-  long long lo = d > rows ? d - rows : 0, hi = d < n ? d : n;
-  const int lane = threadIdx.x & 31;
-  while (lo < hi) {
-    const long long step = (hi - lo + 31) >> 5, at = lo + (lane + 1) * step - 1;
-    const bool before = at < hi && (long long)keys[at] <= d - 1 - at;
-    const int whole = __popc(__ballot_sync(0xffffffffu, before));
-    const long long next = lo + (whole + 1) * step - 1;
-    lo += whole * step;
-    hi = next < hi ? next : hi;
-  }
-  return (uint32_t)lo;
+// Columns per lane: one pack of aligned rows, or J single elements `lanes` apart (so that a
+// warp's loads are whole lines wherever a row begins).
+template <typename T, bool ALIGNED, int J>
+struct Columns {
+  using R = Row<T, ALIGNED ? kAligned : kElement>;
+  static constexpr int kVec = R::kVec, kEach = ALIGNED ? kVec : J;
+  static constexpr int kBatch = ALIGNED ? 8 : 16 / J;   // rows in flight
+  struct Raw {
+    typename R::Raw v[J];
+  };
+};
+template <int EACH>
+constexpr size_t gradient_shared() {   // staged rows and keys, heads and tails of the units, their rows
+  return (kBlockItems + 1) * (sizeof(uint64_t) + sizeof(uint32_t)) + 4 + 2 * kThreads * EACH * sizeof(float) +
+         3 * kThreads * sizeof(int);
 }
 
-template <int VEC>
-constexpr size_t gradient_shared() {   // staged entries, heads and tails (units x lanes = kThreads), their rows
-  return kBlockItems * 2 * sizeof(uint32_t) + 2 * kThreads * VEC * sizeof(float) + 3 * kThreads * sizeof(int);
-}
-
-// Units of `lanes` lanes; a lane holds one pack of columns; blockIdx.y: column tile.
-template <typename T, Layout L>
-__global__ void __launch_bounds__(kThreads, 4) table_gradient_kernel(Gradient g, const T* __restrict__ grad, Extent extent,
+// blockIdx.y: tile of columns.
+template <typename T, bool ALIGNED, int J>
+__global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, const T* __restrict__ grad,
                                                                   T* __restrict__ out, Joins joins) {
-  using R = Row<T, L>;
-  constexpr int VEC = R::kVec;
-  constexpr int kBatch = L == kSpan ? 4 : 8;   // rows of grad in flight per unit
+  using C = Columns<T, ALIGNED, J>;
+  using R = typename C::R;
+  constexpr int kEach = C::kEach, kBatch = C::kBatch;
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ uint32_t s_bound[2];
   const int lanes = g.lanes, units = g.units;
   const int unit = threadIdx.x / lanes, lane = threadIdx.x - unit * lanes;
   const bool live = unit < units;   // a few threads are left over where the lanes do not divide them
-  const int tile_width = lanes * VEC;
-  uint32_t* keys = reinterpret_cast<uint32_t*>(raw);
-  uint32_t* entries = keys + kBlockItems;
-  float* heads = reinterpret_cast<float*>(entries + kBlockItems);   // units x tile_width
-  float* tails = heads + kThreads * VEC;
-  int* head_row = reinterpret_cast<int*>(tails + kThreads * VEC);
+  const int tile_width = lanes * kEach;
+  const T** rows = reinterpret_cast<const T**>(raw);
+  float* heads = reinterpret_cast<float*>(rows + kBlockItems + 1);   // units x tile_width
+  float* tails = heads + kThreads * kEach;
+  int* head_row = reinterpret_cast<int*>(tails + kThreads * kEach);
   int* tail_row = head_row + kThreads;
   int* tail_begun = tail_row + kThreads;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(tail_begun + kThreads);
   follow();
   let_next_start();
   const uint32_t n = *g.count;
-  const long long total = (long long)n + g.rows;
-  // the block's share of the merge, its entries brought into shared memory
-  const long long block_items = (long long)units * g.items;
-  const long long b0 = min((long long)blockIdx.x * block_items, total), b1 = min(b0 + block_items, total);
-  if (threadIdx.x < 64) {
-    const uint32_t p = entries_before(g.keys, n, g.rows, threadIdx.x < 32 ? b0 : b1);
-    if ((threadIdx.x & 31) == 0) s_bound[threadIdx.x >> 5] = p;
-  }
-  __syncthreads();
-  const uint32_t first = s_bound[0], last = s_bound[1];
+  const uint32_t block_items = units * g.items, first = min(n, blockIdx.x * block_items);
+  const int count = (int)min(block_items, n - first);
   const uint32_t before_first = first > 0 ? g.keys[first - 1] : 0xffffffffu;
-  for (uint32_t i = threadIdx.x; i < last - first; i += kThreads) {
-    keys[i] = g.keys[first + i];
-    entries[i] = g.entries[first + i];
+  for (int i = threadIdx.x; i <= count; i += kThreads) {   // one more: whether the last row goes on
+    const bool in = first + i < n;
+    keys[i] = in ? g.keys[first + i] : 0xffffffffu;
+    if (in && i < count) rows[i] = grad + (long long)g.entries[first + i] * g.stride;
   }
   __syncthreads();
-  // the unit's share, places counted from `first`
-  const long long d0 = live ? min(b0 + (long long)unit * g.items, b1) : b1, d1 = min(d0 + g.items, b1);
-  uint32_t p0, p1;
-  {
-    auto search = [&](long long d) {
-      long long lo = max(d - g.rows, (long long)first) - first, hi = min(d, (long long)last) - first;
-      while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if ((long long)keys[mid] <= d - 1 - mid - first) lo = mid + 1;
-        else hi = mid;
-      }
-      return (uint32_t)lo;
-    };
-    p0 = search(d0);
-    p1 = search(d1);
-  }
-  uint32_t r = (uint32_t)(d0 - first - p0);
-  const uint32_t r1 = (uint32_t)(d1 - first - p1);
-  // whether row r has entries in earlier units
-  bool begun_before = d0 < d1 && (p0 > 0 ? keys[p0 - 1] : before_first) == r;
-  // the lane's first column; a last pack that would end behind the row is moved back into it
-  // (its first columns are then the lane's before, added up twice and written twice, alike)
-  const int first_col = blockIdx.y * tile_width + lane * VEC;
-  const bool in = live && first_col < g.width;
-  const int col = L == kSpan ? min(first_col, g.width - VEC) : first_col;
-  float acc[VEC];
+  const int p0 = live ? min(unit * g.items, count) : count, p1 = min(p0 + g.items, count);
+  const int first_col = blockIdx.y * tile_width + lane * C::kVec;
+  const int left = live ? g.width - first_col : 0;   // columns from the lane's first one on
+  auto in = [&](int j) { return ALIGNED ? left > 0 : j * lanes < left; };
+  float acc[kEach];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-  bool any = false;
+  for (int i = 0; i < kEach; ++i) acc[i] = 0.f;
+  uint32_t row = p0 < p1 ? keys[p0] : 0xffffffffu;
+  bool begun_before = p0 < p1 && (p0 > 0 ? keys[p0 - 1] : before_first) == row;   // in earlier units
   int my_head = -1;
-  float* my_heads = heads + unit * tile_width + lane * VEC;
-  float* my_tails = tails + unit * tile_width + lane * VEC;
-  auto write = [&](uint32_t row, float (&sum)[VEC]) {   // columns of a row that may begin anywhere
+  // a lane's columns of the unit's head and tail, kEach floats apart
+  float* my_head_sum = heads + (unit * lanes + lane) * kEach;
+  float* my_tail_sum = tails + (unit * lanes + lane) * kEach;
+  auto write = [&](uint32_t r, const float (&sum)[kEach]) {
+    T* to = out + (long long)r * g.width + first_col;
+    if constexpr (ALIGNED) {
+      float f[kEach];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] *= g.scale;
-    if (!in) return;
-    T* to = out + (long long)row * g.width + col;
-    if (L == kSpan && ((uintptr_t)to & 15)) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) to[i] = from_float<T>(sum[i]);
+      for (int i = 0; i < kEach; ++i) f[i] = g.scale * sum[i];
+      if (left > 0) R::store(to, R::words(f));
     } else {
-      R::store(to, R::words(sum));
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (in(j)) to[j * lanes] = from_float<T>(g.scale * sum[j]);
     }
+    if (g.mask && lane == 0 && blockIdx.y == 0) g.mask[r] = 1;
   };
-
   auto end_row = [&]() {
     if (begun_before) {   // its other entries are elsewhere: leave the sum for the join
-      my_head = (int)r;
+      my_head = (int)row;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) my_heads[i] = acc[i];
+      for (int i = 0; i < kEach; ++i) my_head_sum[i] = acc[i];
     } else {
-      if (any || L != kSpan) {
-        write(r, acc);
-      } else if (r % gridDim.y == blockIdx.y) {   // the tiles share the rows without entries
-        clear_row<T, L>(out + (long long)r * g.width, g.width, lane, lanes);
-      }
-      if (g.mask && lane == 0 && blockIdx.y == 0) g.mask[r] = any;
+      write(row, acc);
     }
     begun_before = false;
-    any = false;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    ++r;
+    for (int i = 0; i < kEach; ++i) acc[i] = 0.f;
   };
-
-  // the rows of the next batches are called into L2 ahead of their loads, which costs no registers
-  const int tile_bytes = (int)sizeof(T) * min(tile_width, g.width - (int)blockIdx.y * tile_width);
-  const int lines = (tile_bytes + 127) / 128 + (L == kAligned ? 0 : 1);
-  auto call = [&](uint32_t from) {
-    for (int i = lane; i < kBatch * lines; i += lanes) {
-      const int b = i / lines, at = min((i - b * lines) * 128, tile_bytes - (int)sizeof(T));
-      if (from + b < p1)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(
-            grad + (long long)entries[from + b] * g.stride + blockIdx.y * tile_width) + at));
-    }
+  auto load = [&](int p, typename C::Raw& v) {
+    const T* from = rows[p] + first_col;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (in(j)) v.v[j] = R::load(from + j * lanes);
   };
-  if (live) call(p0 + kBatch);
-  for (uint32_t p = p0; p < p1; p += kBatch) {
-    if (live) call(p + 2 * kBatch);
-    typename R::Raw v[kBatch];
-    auto load = [&](auto read) {
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        if (p + b < p1 && in) v[b] = read(grad + (long long)entries[p + b] * g.stride + col);
-    };
-    bool inside = true;
-    if (L == kSpan && extent.checked) {
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        if (p + b < p1) inside = inside && extent.inside(grad + (long long)entries[p + b] * g.stride, g.width);
+  auto add = [&](int p, const typename C::Raw& v) {
+    const uint32_t key = keys[p];
+    if (key != row) {
+      end_row();
+      row = key;
     }
-    if (L != kSpan || inside) load([](const T* at) { return R::load(at); });
-    else load([](const T* at) { return R::load_elements(at); });
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (in(j)) {
+        float f[C::kVec];
+        R::floats(v.v[j], f);
+#pragma unroll
+        for (int i = 0; i < C::kVec; ++i) acc[j * C::kVec + i] += f[i];
+      }
+  };
+  int p = p0;
+  for (; p + kBatch <= p1; p += kBatch) {
+    typename C::Raw v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) load(p + b, v[b]);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) add(p + b, v[b]);
+  }
+  if (p < p1) {
+    typename C::Raw v[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
-      if (p + b < p1) {
-        const uint32_t key = keys[p + b];
-        while (r < key) end_row();
-        if (in) {
-          float f[VEC];
-          R::floats(v[b], f);
+      if (p + b < p1) load(p + b, v[b]);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] += f[i];
-        }
-        any = true;
-      }
+    for (int b = 0; b < kBatch; ++b)
+      if (p + b < p1) add(p + b, v[b]);
   }
-  while (r < r1) end_row();
-
-  // the row that is open at the unit's end
-  const bool open = any || begun_before;
-  if (open) {
+  // the last row, which may go on behind the unit
+  bool open = false;
+  if (p0 < p1) {
+    open = keys[p1] == row;
+    if (!open) {
+      end_row();
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) my_tails[i] = acc[i];
+      for (int i = 0; i < kEach; ++i) my_tail_sum[i] = acc[i];
+    }
   }
   if (live && lane == 0) {
     head_row[unit] = my_head;
-    tail_row[unit] = open ? (int)r : -1;
+    tail_row[unit] = open ? (int)row : -1;
     tail_begun[unit] = open && !begun_before;
   }
   __syncthreads();
   // a row that ends in this unit and began in an earlier one: add the tails before it
   bool unfinished = false;
   if (my_head >= 0) {
-    float sum[VEC];
+    float sum[kEach];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] = my_heads[i];
+    for (int i = 0; i < kEach; ++i) sum[i] = my_head_sum[i];
     bool whole = false;
     for (int q = unit - 1; q >= 0 && !whole; --q) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] += tails[q * tile_width + lane * VEC + i];
+      for (int i = 0; i < kEach; ++i) sum[i] += tails[(q * lanes + lane) * kEach + i];
       whole = tail_begun[q];
     }
     if (whole) {
       write((uint32_t)my_head, sum);
-      if (g.mask && lane == 0 && blockIdx.y == 0) g.mask[my_head] = 1;
     } else {   // it began before this block
       unfinished = true;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (in) joins.head[(long long)blockIdx.x * g.width + col + i] = sum[i];
+      for (int i = 0; i < kEach; ++i)
+        if (in(i)) joins.head[(long long)blockIdx.x * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
       if (lane == 0 && blockIdx.y == 0) joins.head_row[blockIdx.x] = my_head;
     }
   }
   const int block_head = __syncthreads_or(unfinished);
   if (!block_head && threadIdx.x == 0 && blockIdx.y == 0) joins.head_row[blockIdx.x] = -1;
-  // the row that is open at the block's end
-  if (unit == units - 1) {
-    const int row = tail_row[unit];
+  // the row that goes on behind the block: the tail of its last unit with entries
+  const int last = count > 0 ? (count - 1) / g.items : 0;
+  if (unit == last) {
+    const int r = tail_row[unit];
     bool begun = false;
-    if (row >= 0) {
-      float sum[VEC];
+    if (r >= 0) {
+      float sum[kEach];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+      for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
       for (int q = unit; q >= 0 && !begun; --q) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] += tails[q * tile_width + lane * VEC + i];
+        for (int i = 0; i < kEach; ++i) sum[i] += tails[(q * lanes + lane) * kEach + i];
         begun = tail_begun[q];
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (in) joins.tail[(long long)blockIdx.x * g.width + col + i] = sum[i];
+      for (int i = 0; i < kEach; ++i)
+        if (in(i)) joins.tail[(long long)blockIdx.x * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
     }
     if (lane == 0 && blockIdx.y == 0) {
-      joins.tail_row[blockIdx.x] = row;
+      joins.tail_row[blockIdx.x] = r;
       joins.tail_begun[blockIdx.x] = begun;
     }
   }
@@ -499,50 +457,47 @@ __global__ void __launch_bounds__(kThreads) table_join_kernel(Joins joins, int w
   }
 }
 
-constexpr int kMinItems = 8;        // items of a unit at least, or the searches outweigh the rows
+constexpr int kMinItems = 4;        // entries of a unit at least
 
 // Most blocks a gradient can have (x dimension): its joins' rows.
-inline long long most_blocks(long long n, long long rows) {
-  const long long total = n + rows, fewest = 8 * kMinItems;   // 8 units at least in a block
-  constexpr long long share = kBlockItems - kThreads;       // of a block whose units do not divide kBlockItems
-  const long long full = (total + share - 1) / share + 148 * 8;
-  const long long tiny = (total + fewest - 1) / fewest;
+inline long long most_blocks(long long n) {
+  constexpr long long share = kBlockItems - kThreads;        // of a block whose units do not divide kBlockItems
+  const long long full = (n + share - 1) / share + 148 * 8;
+  const long long tiny = (n + 8 * kMinItems - 1) / (8 * kMinItems);   // 8 units at least in a block
   return full < tiny ? full : tiny;
 }
 
-template <typename T, Layout L>
-int launch_gradient(Gradient g, long long n, const void* grad, void* out, float* joins_at, cudaStream_t st) {
-  constexpr int VEC = Row<T, L>::kVec;
-  constexpr size_t shared = gradient_shared<VEC>();
+template <typename T, bool ALIGNED, int J>
+int launch_gradient(Gradient g, int lanes, long long n, const void* grad, void* out, float* joins_at, cudaStream_t st) {
+  constexpr int kEach = Columns<T, ALIGNED, J>::kEach;
+  constexpr size_t shared = gradient_shared<kEach>();
   static_assert(shared <= 48 * 1024, "the default limit of shared memory");
   static const int resident = [] {
     int blocks = 0;
     const cudaError_t e =
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, table_gradient_kernel<T, L>, kThreads, shared);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, table_gradient_kernel<T, ALIGNED, J>, kThreads, shared);
     return e == cudaSuccess && blocks > 0 ? (blocks < 8 ? blocks : 8) : 2;
   }();
-  const int packs = (g.width + VEC - 1) / VEC;
-  g.lanes = packs < 32 ? packs : 32;
-  const int units = g.units = kThreads / g.lanes, tile_width = g.lanes * VEC;
+  g.lanes = lanes;
+  const int units = g.units = kThreads / lanes, tile_width = lanes * kEach;
   const int tiles = (g.width + tile_width - 1) / tile_width;
   // equal blocks that fill the SMs a whole number of times
-  const long long total = n + g.rows;
   long long slots = 148 * resident / tiles;
   if (slots < 1) slots = 1;
-  const long long waves = (total + slots * kBlockItems - 1) / (slots * kBlockItems);
-  long long items = (total + slots * waves * units - 1) / (slots * waves * units);
+  const long long waves = (n + slots * kBlockItems - 1) / (slots * kBlockItems);
+  long long items = (n + slots * waves * units - 1) / (slots * waves * units);
   if (items < kMinItems) items = kMinItems;
   if (items * units > kBlockItems) items = kBlockItems / units;
   g.items = (int)items;
-  const long long blocks = (total + items * units - 1) / (items * units);
+  const long long blocks = (n + items * units - 1) / (items * units);
   Joins joins;
   joins.head = joins_at;
   joins.tail = joins.head + blocks * g.width;
   joins.head_row = (int*)(joins.tail + blocks * g.width);
   joins.tail_row = joins.head_row + blocks;
   joins.tail_begun = joins.tail_row + blocks;
-  CVHRF_CUDA_TRY(launch_after(table_gradient_kernel<T, L>, dim3((unsigned)blocks, tiles), kThreads, shared, st, g,
-                              (const T*)grad, extent_of(grad, n, g.stride, g.width, sizeof(T)), (T*)out, joins));
+  CVHRF_CUDA_TRY(launch_after(table_gradient_kernel<T, ALIGNED, J>, dim3((unsigned)blocks, tiles), kThreads, shared, st,
+                              g, (const T*)grad, (T*)out, joins));
   count_launch(1);
   if (blocks == 1) return CVHRF_OK;
   const int columns = next_pow2(g.width < kThreads ? g.width : kThreads);
@@ -552,16 +507,20 @@ int launch_gradient(Gradient g, long long n, const void* grad, void* out, float*
   return CVHRF_OK;
 }
 
-// Units of as many lanes as a row has packs, a warp at most; wider rows are cut into tiles.
+// Units of as many lanes as a row has packs or elements, a warp at most; wider rows have several
+// elements per lane, then tiles.
 template <typename T>
-int gradient(const void* grad, long long stride, int width, long long n, long long rows, float scale, void* out,
-             uint8_t* mask, const uint32_t* keys, const uint32_t* entries, const uint32_t* count, float* joins,
-             cudaStream_t st) {
-  const Gradient g{keys, entries, count, stride, (int)rows, width, 0, 0, 0, scale, mask};
-  if (rows_16(grad, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0)
-    return launch_gradient<T, kAligned>(g, n, grad, out, joins, st);
-  if (width >= kSpanWidth) return launch_gradient<T, kSpan>(g, n, grad, out, joins, st);
-  return launch_gradient<T, kElement>(g, n, grad, out, joins, st);
+int gradient(const void* grad, long long stride, int width, long long n, float scale, void* out, uint8_t* mask,
+             const uint32_t* keys, const uint32_t* entries, const uint32_t* count, float* joins, cudaStream_t st) {
+  const Gradient g{keys, entries, count, stride, width, 0, 0, 0, scale, mask};
+  if (rows_16(grad, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0) {
+    const int packs = packs_of<T, kAligned>(width);
+    return launch_gradient<T, true, 1>(g, packs < 32 ? packs : 32, n, grad, out, joins, st);
+  }
+  if (width <= 32) return launch_gradient<T, false, 1>(g, width, n, grad, out, joins, st);
+  if (width <= 64) return launch_gradient<T, false, 2>(g, 32, n, grad, out, joins, st);
+  if (width <= 128) return launch_gradient<T, false, 4>(g, 32, n, grad, out, joins, st);
+  return launch_gradient<T, false, 8>(g, 32, n, grad, out, joins, st);
 }
 
 constexpr long long kMaxRows = 0x7ffffffe;
@@ -593,7 +552,7 @@ extern "C" size_t cvhrf_table_gradient_workspace_bytes(long long entries, long l
   if (entries < 0 || entries > kGroupMaxEntries || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth)
     return 0;
   return align_up(group_sort_words(entries) * sizeof(uint32_t), 256) +
-         (size_t)most_blocks(entries, rows) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int));
+         (size_t)most_blocks(entries) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int));
 }
 
 extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* stream) {
@@ -618,15 +577,16 @@ extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* strea
   if ((uintptr_t)workspace & 15) return CVHRF_EINVAL;
   uint32_t* scratch = (uint32_t*)workspace;
   const uint32_t *keys, *sorted, *count;
-  const int rc = group_sort(index, index_bytes, entries, rows, false, scratch, st, &keys, &sorted, &count);
+  const Zeros zeros{{grad_table, row_mask}, {(unsigned long long)rows * width * elem, row_mask ? (unsigned long long)rows : 0}};
+  const int rc = group_sort(index, index_bytes, entries, rows, false, scratch, zeros, st, &keys, &sorted, &count);
   if (rc) return rc;
   float* joins = (float*)((char*)workspace + align_up(group_sort_words(entries) * sizeof(uint32_t), 256));
   if (dtype == CVHRF_F32)
-    return gradient<float>(grad, grad_stride, width, entries, rows, scale, grad_table, row_mask, keys, sorted, count,
+    return gradient<float>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted, count,
                            joins, st);
   if (dtype == CVHRF_BF16)
-    return gradient<__nv_bfloat16>(grad, grad_stride, width, entries, rows, scale, grad_table, row_mask, keys, sorted,
+    return gradient<__nv_bfloat16>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted,
                                    count, joins, st);
-  return gradient<__half>(grad, grad_stride, width, entries, rows, scale, grad_table, row_mask, keys, sorted, count,
+  return gradient<__half>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted, count,
                           joins, st);
 }
