@@ -109,4 +109,14 @@ __device__ __forceinline__ void bulk_copy_g2s(void* dst, const void* src, unsign
                : "memory");
 }
 
+// shared -> global bulk copy of `bytes` (multiple of 16; both addresses 16-byte aligned); the
+// issuing thread waits until its copies have been read from shared memory
+__device__ __forceinline__ void bulk_copy_s2g(void* dst, const void* src, unsigned bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_copy_wait() {
+  asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;\n" ::: "memory");
+}
+
 }  // namespace cvhrf

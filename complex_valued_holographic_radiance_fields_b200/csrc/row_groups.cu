@@ -49,8 +49,14 @@ struct Fill {
   int first_block, part, parts;
 };
 
-__device__ __forceinline__ void fill_zeros(const Fill& f) {
+// The block's share, from 8 KB of zeros in shared memory by bulk copies: one thread issues them,
+// and none of the lanes' stores are in the sort's way.
+constexpr int kFillBytes = 8192;
+__device__ __forceinline__ void fill_zeros(const Fill& f, uint4* shared /* kFillBytes */) {
   const int block = blockIdx.x - f.first_block, blocks = gridDim.x - f.first_block;
+  for (int i = threadIdx.x; i < kFillBytes / 16; i += kThreads) shared[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncthreads();
   for (int k = 0; k < 2; ++k) {
     char* at = (char*)f.z.at[k];
     const unsigned long long head = min((unsigned long long)(-(long long)(uintptr_t)at & 15), f.z.bytes[k]);
@@ -59,11 +65,17 @@ __device__ __forceinline__ void fill_zeros(const Fill& f) {
       for (unsigned long long i = threadIdx.x; i < head; i += kThreads) at[i] = 0;
       for (unsigned long long i = tail + threadIdx.x; i < f.z.bytes[k]; i += kThreads) at[i] = 0;
     }
-    uint4* w = reinterpret_cast<uint4*>(at + head);
-    const unsigned long long begin = words * f.part / f.parts, end = words * (f.part + 1) / f.parts;
-    for (unsigned long long i = begin + (unsigned long long)block * kThreads + threadIdx.x; i < end;
-         i += (unsigned long long)blocks * kThreads)
-      w[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x == 0) {
+      const unsigned long long begin = words * f.part / f.parts, n = words * (f.part + 1) / f.parts - begin;
+      char* to = at + head + (begin + n * block / blocks) * 16;
+      char* end = at + head + (begin + n * (block + 1) / blocks) * 16;
+      while (to < end) {
+        const unsigned bytes = (unsigned)min((unsigned long long)(end - to), (unsigned long long)kFillBytes);
+        bulk_copy_s2g(to, shared, bytes);
+        to += bytes;
+      }
+      bulk_copy_wait();
+    }
   }
 }
 
@@ -80,10 +92,11 @@ __device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
 __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, uint32_t chunk, int shift, int radix,
                                                                uint32_t* __restrict__ counts, int clear, Fill fill) {
   let_next_start();
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
-  const uint32_t chunks = fill.first_block;
   constexpr int kCopies = 8;   // histograms, so that equal digits of different warps do not meet
-  __shared__ uint32_t h[kCopies][kMaxRadix];
+  __shared__ __align__(16) uint32_t h[kCopies][kMaxRadix];
+  static_assert(sizeof(h) >= kFillBytes);
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(h));
+  const uint32_t chunks = fill.first_block;
   for (int i = threadIdx.x; i < kCopies * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
   for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < (uint32_t)clear; i += chunks * kThreads)
     counts[(size_t)chunks * radix + i] = 0;
@@ -115,6 +128,7 @@ struct Shared {
   uint32_t key[kTile], entry[kTile];   // the tile in digit order
   uint32_t base[kMaxRadix];            // place of the chunk's next key with this digit
   uint32_t start[kMaxRadix];           // start of the digit inside the tile
+  uint32_t delta[kMaxRadix];           // base - start
   uint32_t sh[9];
 };
 
@@ -158,23 +172,30 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
   for (int i = tid; i < kWarps * kMaxRadix; i += kThreads) (&sh.cnt[0][0])[i] = 0;
   __syncthreads();
   const unsigned lt = (1u << lane) - 1u;
+  // the lanes with the same digit, bit by bit (__match_any_sync takes a step per distinct digit)
+  unsigned peers[kItems];
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    if (r >= rounds) break;
+    const uint32_t d = key[r] >> shift;
+    peers[r] = __ballot_sync(0xffffffffu, key[r] != kNone);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      if (b >= width) break;
+      const unsigned ones = __ballot_sync(0xffffffffu, d & (1u << b));
+      peers[r] &= d & (1u << b) ? ones : ~ones;
+    }
+  }
 #pragma unroll
   for (int r = 0; r < kItems; ++r) {
     if (r >= rounds) break;
     const bool in = key[r] != kNone;
     const uint32_t d = (key[r] >> shift) & mask;
-    // the lanes with the same digit, bit by bit (__match_any_sync takes a step per distinct digit)
-    unsigned peers = __ballot_sync(0xffffffffu, in);
-    for (int b = 0; b < width; ++b) {
-      const bool one = (d >> b) & 1u;
-      const unsigned ones = __ballot_sync(0xffffffffu, one);
-      peers &= one ? ones : ~ones;
-    }
     uint32_t before = 0;
     if (in) before = sh.cnt[warp][d];
-    place[r] = before + __popc(peers & lt);
+    place[r] = before + __popc(peers[r] & lt);
     __syncwarp();
-    if (in && (peers & lt) == 0) sh.cnt[warp][d] = before + __popc(peers);
+    if (in && (peers[r] & lt) == 0) sh.cnt[warp][d] = before + __popc(peers[r]);
     __syncwarp();
   }
   __syncthreads();
@@ -206,6 +227,7 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
 
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
                                                                  const uint32_t* __restrict__ n_dev, uint32_t chunk,
+                                                                 uint32_t reciprocal /* 2^32 / chunk, up */,
                                                                  int shift, int radix,
                                                                  const uint32_t* __restrict__ counts, Target out,
                                                                  Fill fill) {
@@ -214,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   follow();
   let_next_start();
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(raw));
   const int chunks = fill.first_block;
   if (n_dev) n = min(n, *n_dev);
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
@@ -284,12 +306,18 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
               key[r] < (uint32_t)out.groups ? (int)(sh.base[(key[r] >> shift) & mask] + place[r]) : -1;
     }
     // the tile is in digit order: each digit's keys go out as one run
+    if (tid < kMaxRadix) sh.delta[tid] = sh.base[tid] - sh.start[tid];
+    __syncthreads();
     for (uint32_t i = tid; i < kept; i += kThreads) {
       const uint32_t k = sh.key[i], d = (k >> shift) & mask;
-      const uint32_t at = sh.base[d] + i - sh.start[d];
+      const uint32_t at = sh.delta[d] + i;
       if (out.keys) out.keys[at] = k;
       out.entries[at] = sh.entry[i];
-      if (out.next) atomicAdd(&out.next[(size_t)(at / chunk) * out.next_radix + ((k >> out.next_shift) & (out.next_radix - 1))], 1u);
+      if (out.next) {
+        uint32_t c = __umulhi(at, reciprocal);   // at / chunk, or one more
+        if (c * chunk > at) --c;
+        atomicAdd(&out.next[c * out.next_radix + ((k >> out.next_shift) & (out.next_radix - 1))], 1u);
+      }
     }
     __syncthreads();
     if (tid < kMaxRadix) sh.base[tid] += run;
@@ -304,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   let_next_start();
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill);
+  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(raw));
   uint32_t key[kItems], entry[kItems], place[kItems];
   uint32_t kept = n;
   int done = 0;
@@ -421,7 +449,7 @@ int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* b
     if (p + 1 < passes) t = Target{to, to + len, nullptr, nullptr, 0, nullptr, next, shift[p + 1], radix[p + 1]};
     t.count = p == 0 ? count : nullptr;
     CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count + more), kThreads, sizeof(Shared), st, src,
-                                (uint32_t)n, p == 0 ? nullptr : count, c.size, shift[p], radix[p], counts, t,
+                                (uint32_t)n, p == 0 ? nullptr : count, c.size, (uint32_t)(0xffffffffull / c.size + 1), shift[p], radix[p], counts, t,
                                 Fill{zeros, c.count, p + 1, parts}));
     count_launch(1);
     src = Source{nullptr, 0, to, to + len, src.rows, 1};

@@ -552,7 +552,7 @@ extern "C" size_t cvhrf_table_gradient_workspace_bytes(long long entries, long l
   if (entries < 0 || entries > kGroupMaxEntries || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth)
     return 0;
   return align_up(group_sort_words(entries) * sizeof(uint32_t), 256) +
-         (size_t)most_blocks(entries) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int));
+         align_up((size_t)most_blocks(entries) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int)), 256);
 }
 
 extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* stream) {

@@ -40,14 +40,9 @@ __device__ __forceinline__ void send_tile(const T* tile, int n, int width, T* ou
   fence_proxy_async_smem();
   __syncthreads();
   const int total = n * width, whole = total / (16 / (int)sizeof(T)) * (16 / (int)sizeof(T));
-  if (threadIdx.x == 0 && whole > 0) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(out), "r"(smem_u32(tile)),
-                 "r"(whole * (int)sizeof(T))
-                 : "memory");
-    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-  }
+  if (threadIdx.x == 0 && whole > 0) bulk_copy_s2g(out, tile, whole * (int)sizeof(T));
   for (int i = whole + threadIdx.x; i < total; i += kTileThreads) out[i] = tile[i];
-  if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+  if (threadIdx.x == 0) bulk_copy_wait();
 }
 
 // What entries without a row read.

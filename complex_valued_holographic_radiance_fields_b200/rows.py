@@ -49,6 +49,8 @@ def _call(name, what, device, args):
         _lib.check(rc, name)
 
 
+# Workspaces are multiples of 8 bytes, allocated as elements of the index's type (new_empty of
+# the same type is the cheapest allocation there is).
 @functools.lru_cache(maxsize=256)
 def _gradient_workspace(n, num_rows, width):
     return _lib.lib().cvhrf_table_gradient_workspace_bytes(n, num_rows, width)
@@ -99,7 +101,7 @@ def _lookup(table, index, scale):
     table, code, width, stride = _rows(table, "table")
     device = table.device
     index, nbytes, n = _index(index, device)
-    out = torch.empty((*index.shape, width), dtype=table.dtype, device=device)
+    out = table.new_empty((*index.shape, width))
     _call("cvhrf_table_lookup", "table_lookup", device, _lib.LOOKUP_ARGS.pack(
         table.data_ptr(), index.data_ptr(), out.data_ptr(), table.shape[0], stride, n, width, code, nbytes, scale))
     return out
@@ -113,10 +115,10 @@ def _gradient(grad, index, num_rows, scale, with_mask):
     grad, code, width, stride = _rows(grad, "grad")
     device = grad.device
     index, nbytes, n = _index(index, device)
-    out = torch.empty((num_rows, width), dtype=grad.dtype, device=device)
-    mask = torch.empty(num_rows, dtype=torch.uint8, device=device) if with_mask else None
+    out = grad.new_empty((num_rows, width))
+    mask = index.new_empty(num_rows, dtype=torch.uint8) if with_mask else None
     need = _gradient_workspace(n, num_rows, width)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    ws = index.new_empty(need // nbytes)
     _call("cvhrf_table_gradient", "table_gradient", device, _lib.GRADIENT_ARGS.pack(
         grad.data_ptr(), index.data_ptr(), out.data_ptr(), mask.data_ptr() if with_mask else 0, ws.data_ptr(), need,
         stride, n, num_rows, width, code, nbytes, scale))
@@ -188,11 +190,11 @@ def group_rows(index, num_groups):
         raise ValueError(f"num_groups must be in [1, 2^31 - 1), got {num_groups}")
     device = index.device
     index, nbytes, n = _index(index, device)
-    order = torch.empty(n, dtype=torch.int32, device=device)
-    slots = torch.empty(shape, dtype=torch.int32, device=device)
-    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
+    order = index.new_empty(n, dtype=torch.int32)
+    slots = index.new_empty(shape, dtype=torch.int32)
+    offsets = index.new_empty(num_groups + 1, dtype=torch.int32)
     need = _group_workspace(n, num_groups)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    ws = index.new_empty(need // nbytes) if need else None
     _call("cvhrf_group_rows", "group_rows", device, _lib.GROUP_ARGS.pack(
         index.data_ptr(), order.data_ptr(), slots.data_ptr(), offsets.data_ptr(), ws.data_ptr() if need else 0, need,
         n, num_groups, nbytes))
@@ -202,7 +204,7 @@ def group_rows(index, num_groups):
 def _to_groups(x, groups):
     x, code, width, stride = _rows(x, "x")
     device, n, k = x.device, groups.num_rows, groups.choices
-    out = torch.empty((n * k, width), dtype=x.dtype, device=device)
+    out = x.new_empty((n * k, width))
     _call("cvhrf_rows_to_groups", "rows_to_groups", device, _lib.MOVES_ARGS.pack(
         x.data_ptr(), out.data_ptr(), groups.order.data_ptr(), groups.slots.data_ptr(), groups._used(), 0, n, stride, k,
         width, code, 0))
@@ -212,7 +214,7 @@ def _to_groups(x, groups):
 def _to_rows(y, groups, weights):
     y, code, width, stride = _rows(y, "y")
     device, n = y.device, groups.num_rows
-    out = torch.empty((n, width), dtype=y.dtype, device=device)
+    out = y.new_empty((n, width))
     w, w_code = (0, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
     _call("cvhrf_groups_to_rows", "groups_to_rows", device, _lib.MOVES_ARGS.pack(
         y.data_ptr(), out.data_ptr(), 0, groups.slots.data_ptr(), 0, w, n, stride, groups.choices, width, code, w_code))
@@ -245,7 +247,7 @@ class GroupsToRows(torch.autograd.Function):
         y, _, _, stride = _rows(y, "y")
         device = y.device
         need_y, _, need_w = ctx.needs_input_grad
-        grad_y = torch.empty(y.shape, dtype=y.dtype, device=device) if need_y else None
+        grad_y = y.new_empty(y.shape) if need_y else None
         grad_w = torch.empty_like(weights) if need_w else None
         w, w_code = (0, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
         _call("cvhrf_groups_to_rows_backward", "groups_to_rows_backward", device, _lib.MOVES_BACKWARD_ARGS.pack(
