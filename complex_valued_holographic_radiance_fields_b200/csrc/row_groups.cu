@@ -1,10 +1,11 @@
 // Integer indices sorted stably by value (see row_groups.cuh), and cvhrf_group_rows.
 //
-// LSD radix sort, digits of at most 8 bits, the bits shared evenly between the passes.
-// chunk_count_kernel counts the first digits of each contiguous chunk of keys into a chunk x
-// digit matrix; each pass (chunk_scatter_kernel) reads its matrix, adds up what lies before
-// its own chunk, writes each key to its place, and counts the key's next digit for the chunk
-// it goes to.  No block waits for another one, and a sort is 1 launch more than its passes.
+// LSD radix sort, digits of at most 9 bits (two passes up to 262144 values), the bits shared evenly between the passes.  A pass
+// is two launches: chunk_count_kernel counts the digits of each contiguous chunk of keys into
+// a chunk x digit matrix, and chunk_scatter_kernel reads that matrix, adds up what lies before
+// its own chunk, and writes each key to its place.  No block waits for another one and nothing
+// has to be cleared beforehand.  (Counting a key's next digit where it is scattered saves a
+// launch, but its atomics cost 8 us for 1M keys, and the launch 3.)
 // (A look-back between tiles, as in scan_sort.cu, needs a cleared status array, one more
 // launch for the histogram, and a walk over the earlier tiles in L2 latency.)
 // The first pass reads the caller's indices as they are (4 or 8 bytes).
@@ -20,7 +21,7 @@ namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32, kItems = 8, kTile = kThreads * kItems;
 constexpr int kMaxChunks = 148;   // one block per SM
-constexpr int kMaxRadix = 256;
+constexpr int kMaxBits = 9, kMaxRadix = 1 << kMaxBits;
 constexpr uint32_t kNone = 0xffffffffu;
 
 struct Source {
@@ -39,43 +40,19 @@ struct Target {
   int* offsets;        // ... and where each of the `groups` groups begins, and the last one ends
   int groups;
   uint32_t* count;     // number of sorted items
-  uint32_t* next;      // where the next pass counts: chunk x next_radix; null: last pass
-  int next_shift, next_radix;
+  uint8_t* touched;    // 1 for every key
 };
 
-// A launch's share of Zeros: its blocks from `first_block` on write the zeros.
-struct Fill {
-  Zeros z;
-  int first_block, part, parts;
-};
-
-// The block's share, from 8 KB of zeros in shared memory by bulk copies: one thread issues them,
-// and none of the lanes' stores are in the sort's way.
-constexpr int kFillBytes = 8192;
-__device__ __forceinline__ void fill_zeros(const Fill& f, uint4* shared /* kFillBytes */) {
-  const int block = blockIdx.x - f.first_block, blocks = gridDim.x - f.first_block;
-  for (int i = threadIdx.x; i < kFillBytes / 16; i += kThreads) shared[i] = make_uint4(0u, 0u, 0u, 0u);
-  fence_proxy_async_smem();
-  __syncthreads();
-  for (int k = 0; k < 2; ++k) {
-    char* at = (char*)f.z.at[k];
-    const unsigned long long head = min((unsigned long long)(-(long long)(uintptr_t)at & 15), f.z.bytes[k]);
-    const unsigned long long words = (f.z.bytes[k] - head) >> 4, tail = head + (words << 4);
-    if (f.part == 0 && block == 0) {   // the ends that are not whole words
-      for (unsigned long long i = threadIdx.x; i < head; i += kThreads) at[i] = 0;
-      for (unsigned long long i = tail + threadIdx.x; i < f.z.bytes[k]; i += kThreads) at[i] = 0;
-    }
-    if (threadIdx.x == 0) {
-      const unsigned long long begin = words * f.part / f.parts, n = words * (f.part + 1) / f.parts - begin;
-      char* to = at + head + (begin + n * block / blocks) * 16;
-      char* end = at + head + (begin + n * (block + 1) / blocks) * 16;
-      while (to < end) {
-        const unsigned bytes = (unsigned)min((unsigned long long)(end - to), (unsigned long long)kFillBytes);
-        bulk_copy_s2g(to, shared, bytes);
-        to += bytes;
-      }
-      bulk_copy_wait();
-    }
+// Zeros into `touched` before the passes set its ones.
+__device__ __forceinline__ void clear_touched(uint8_t* touched, uint32_t rows) {
+  if (!touched) return;
+  const uint32_t head = min((uint32_t)(-(long long)(uintptr_t)touched & 15), rows), words = (rows - head) >> 4;
+  uint4* w = reinterpret_cast<uint4*>(touched + head);
+  for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < words; i += gridDim.x * kThreads)
+    w[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x < head) touched[threadIdx.x] = 0;
+    for (uint32_t i = head + (words << 4) + threadIdx.x; i < rows; i += kThreads) touched[i] = 0;
   }
 }
 
@@ -87,19 +64,18 @@ __device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
   return v < s.rows ? (uint32_t)v : (s.keep ? s.rows : kNone);
 }
 
-// counts[chunk][digit] over the keys of each chunk; the `clear` words behind the matrix, where
-// the later passes count, are set to zero.
-__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, uint32_t chunk, int shift, int radix,
-                                                               uint32_t* __restrict__ counts, int clear, Fill fill) {
+// counts[chunk][digit] over the keys of each chunk.
+__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, const uint32_t* __restrict__ n_dev,
+                                                               uint32_t chunk, int shift, int radix,
+                                                               uint32_t* __restrict__ counts,
+                                                               uint8_t* __restrict__ clear) {
+  follow();
   let_next_start();
   constexpr int kCopies = 8;   // histograms, so that equal digits of different warps do not meet
-  __shared__ __align__(16) uint32_t h[kCopies][kMaxRadix];
-  static_assert(sizeof(h) >= kFillBytes);
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(h));
-  const uint32_t chunks = fill.first_block;
+  __shared__ uint32_t h[kCopies][kMaxRadix];
+  clear_touched(clear, s.rows);
+  if (n_dev) n = min(n, *n_dev);
   for (int i = threadIdx.x; i < kCopies * kMaxRadix; i += kThreads) (&h[0][0])[i] = 0;
-  for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < (uint32_t)clear; i += chunks * kThreads)
-    counts[(size_t)chunks * radix + i] = 0;
   __syncthreads();
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   uint32_t* mine = h[(threadIdx.x >> 5) % kCopies];
@@ -124,16 +100,17 @@ __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_
 }
 
 struct Shared {
-  uint32_t cnt[kWarps][kMaxRadix];
+  uint32_t cnt[kWarps * kMaxRadix];    // warp x digit
   uint32_t key[kTile], entry[kTile];   // the tile in digit order
   uint32_t base[kMaxRadix];            // place of the chunk's next key with this digit
   uint32_t start[kMaxRadix];           // start of the digit inside the tile
   uint32_t delta[kMaxRadix];           // base - start
-  uint32_t sh[9];
+  uint32_t sh[kMaxRadix / 32 + 1];
 };
 
-// Exclusive scan over the values of a block's first 256 threads; all threads call it.
-__device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, uint32_t& total) {
+// Exclusive scan over the values of a block's first kMaxRadix threads; all threads call it.
+__device__ __forceinline__ uint32_t scan_radix(uint32_t v, uint32_t* sh /* kMaxRadix / 32 + 1 */, uint32_t& total) {
+  constexpr int kParts = kMaxRadix / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t inc = v;
 #pragma unroll
@@ -141,21 +118,21 @@ __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, u
     const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += t;
   }
-  if (warp < 8 && lane == 31) sh[warp] = inc;
+  if (warp < kParts && lane == 31) sh[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    uint32_t t = lane < 8 ? sh[lane] : 0u, run = t;
+    uint32_t t = lane < kParts ? sh[lane] : 0u, run = t;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < kParts; o <<= 1) {
       const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += u;
     }
-    if (lane < 8) sh[lane] = run - t;
-    if (lane == 7) sh[8] = run;
+    if (lane < kParts) sh[lane] = run - t;
+    if (lane == kParts - 1) sh[kParts] = run;
   }
   __syncthreads();
-  const uint32_t r = (warp < 8 ? sh[warp] : 0u) + inc - v;
-  total = sh[8];
+  const uint32_t r = (warp < kParts ? sh[warp] : 0u) + inc - v;
+  total = sh[kParts];
   __syncthreads();
   return r;
 }
@@ -167,11 +144,13 @@ __device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* sh /* 9 */, u
 __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[kItems], const uint32_t (&entry)[kItems],
                                               uint32_t (&place)[kItems], int rounds, int shift, int width,
                                               uint32_t& kept) {
-  const uint32_t mask = (1u << width) - 1u;
+  const int radix = 1 << width;
+  const uint32_t mask = radix - 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < kWarps * kMaxRadix; i += kThreads) (&sh.cnt[0][0])[i] = 0;
+  for (int i = tid; i < kWarps * radix; i += kThreads) sh.cnt[i] = 0;
   __syncthreads();
   const unsigned lt = (1u << lane) - 1u;
+  uint32_t* mine = sh.cnt + warp * radix;
   // the lanes with the same digit, bit by bit (__match_any_sync takes a step per distinct digit)
   unsigned peers[kItems];
 #pragma unroll
@@ -180,7 +159,7 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
     const uint32_t d = key[r] >> shift;
     peers[r] = __ballot_sync(0xffffffffu, key[r] != kNone);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < kMaxBits; ++b) {
       if (b >= width) break;
       const unsigned ones = __ballot_sync(0xffffffffu, d & (1u << b));
       peers[r] &= d & (1u << b) ? ones : ~ones;
@@ -192,23 +171,23 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
     const bool in = key[r] != kNone;
     const uint32_t d = (key[r] >> shift) & mask;
     uint32_t before = 0;
-    if (in) before = sh.cnt[warp][d];
+    if (in) before = mine[d];
     place[r] = before + __popc(peers[r] & lt);
     __syncwarp();
-    if (in && (peers[r] & lt) == 0) sh.cnt[warp][d] = before + __popc(peers[r]);
+    if (in && (peers[r] & lt) == 0) mine[d] = before + __popc(peers[r]);
     __syncwarp();
   }
   __syncthreads();
   uint32_t run = 0;
-  if (tid < kMaxRadix) {
+  if (tid < radix) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const uint32_t c = sh.cnt[w][tid];
-      sh.cnt[w][tid] = run;
+      const uint32_t c = sh.cnt[w * radix + tid];
+      sh.cnt[w * radix + tid] = run;
       run += c;
     }
   }
-  const uint32_t start = scan_256(run, sh.sh, kept);
+  const uint32_t start = scan_radix(run, sh.sh, kept);
   if (tid < kMaxRadix) sh.start[tid] = start;
   __syncthreads();
 #pragma unroll
@@ -216,7 +195,7 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
     if (r >= rounds) break;
     if (key[r] == kNone) continue;
     const uint32_t d = (key[r] >> shift) & mask;
-    place[r] += sh.cnt[warp][d];
+    place[r] += mine[d];
     const uint32_t at = sh.start[d] + place[r];
     sh.key[at] = key[r];
     sh.entry[at] = entry[r];
@@ -227,17 +206,14 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
 
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
                                                                  const uint32_t* __restrict__ n_dev, uint32_t chunk,
-                                                                 uint32_t reciprocal /* 2^32 / chunk, up */,
                                                                  int shift, int radix,
-                                                                 const uint32_t* __restrict__ counts, Target out,
-                                                                 Fill fill) {
+                                                                 const uint32_t* __restrict__ counts, Target out) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   follow();
   let_next_start();
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(raw));
-  const int chunks = fill.first_block;
+  const int chunks = gridDim.x;
   if (n_dev) n = min(n, *n_dev);
   const uint32_t begin = min(n, blockIdx.x * chunk), end = min(n, begin + chunk);
   const uint32_t mask = radix - 1;
@@ -256,37 +232,26 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
     }
   };
   if (begin < end) load(begin);   // on its way while the matrix of counts is added up
-  // the matrix of counts: 16 shares of the chunks, four digits per thread
+  // the matrix of counts: four digits per thread, the chunks shared between the threads
   {
-    constexpr int kShares = 16, kLoads = (kMaxChunks + kShares - 1) / kShares;
-    const int quads = radix >> 2, share = tid / quads, q = tid - share * quads;
-    uint4* before4 = reinterpret_cast<uint4*>(sh.key);
-    uint4* all4 = reinterpret_cast<uint4*>(sh.entry);
-    if (share < kShares) {
-      uint4 v[kLoads];
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int c = share + i * kShares;
-        v[i] = c < chunks ? reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q] : make_uint4(0, 0, 0, 0);
-      }
-      uint4 before = make_uint4(0, 0, 0, 0), all = before;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        all.x += v[i].x, all.y += v[i].y, all.z += v[i].z, all.w += v[i].w;
-        if (share + i * kShares < (int)blockIdx.x)
-          before.x += v[i].x, before.y += v[i].y, before.z += v[i].z, before.w += v[i].w;
-      }
-      before4[share * quads + q] = before;
-      all4[share * quads + q] = all;
+    const int quads = radix >> 2, shares = kThreads / quads, share = tid / quads, q = tid - share * quads;
+    uint4 before4 = make_uint4(0, 0, 0, 0), all4 = before4;
+#pragma unroll 10
+    for (int c = share; c < chunks; c += shares) {
+      const uint4 v = reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q];
+      all4.x += v.x, all4.y += v.y, all4.z += v.z, all4.w += v.w;
+      if (c < (int)blockIdx.x) before4.x += v.x, before4.y += v.y, before4.z += v.z, before4.w += v.w;
     }
+    reinterpret_cast<uint4*>(sh.key)[tid] = before4;   // shares x radix
+    reinterpret_cast<uint4*>(sh.entry)[tid] = all4;
     __syncthreads();
     uint32_t before = 0, all = 0;
     if (tid < radix) {
-#pragma unroll
-      for (int i = 0; i < kShares; ++i) before += sh.key[i * radix + tid], all += sh.entry[i * radix + tid];
+#pragma unroll 8
+      for (int i = 0; i < shares; ++i) before += sh.key[i * radix + tid], all += sh.entry[i * radix + tid];
     }
     uint32_t total;
-    const uint32_t first = scan_256(all, sh.sh, total);
+    const uint32_t first = scan_radix(all, sh.sh, total);
     if (tid < kMaxRadix) sh.base[tid] = first + before;
     if (blockIdx.x == 0 && tid == 0 && out.count) *out.count = total;
     if (blockIdx.x == 0 && out.offsets) {
@@ -313,11 +278,8 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
       const uint32_t at = sh.delta[d] + i;
       if (out.keys) out.keys[at] = k;
       out.entries[at] = sh.entry[i];
-      if (out.next) {
-        uint32_t c = __umulhi(at, reciprocal);   // at / chunk, or one more
-        if (c * chunk > at) --c;
-        atomicAdd(&out.next[c * out.next_radix + ((k >> out.next_shift) & (out.next_radix - 1))], 1u);
-      }
+      // (the tile is in order of the whole key by the last pass)
+      if (out.touched && (i == 0 || sh.key[i - 1] != k)) out.touched[k] = 1;
     }
     __syncthreads();
     if (tid < kMaxRadix) sh.base[tid] += run;
@@ -327,12 +289,12 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
 
 // All passes on up to kTile keys, in one block.
 __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t n, int bits, int passes, Target out,
-                                                              Fill fill) {
+                                                              bool clear) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   let_next_start();
-  if ((int)blockIdx.x >= fill.first_block) return fill_zeros(fill, reinterpret_cast<uint4*>(raw));
+  if (clear) clear_touched(out.touched, s.rows);
   uint32_t key[kItems], entry[kItems], place[kItems];
   uint32_t kept = n;
   int done = 0;
@@ -355,6 +317,7 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
     if (out.keys) out.keys[i] = k;
     out.entries[i] = e;
     if (out.slots) out.slots[e] = k < (uint32_t)out.groups ? (int)i : -1;
+    if (out.touched && (i == 0 || sh.key[i - 1] != k)) out.touched[k] = 1;
   }
   if (tid == 0 && out.count) *out.count = kept;
   if (out.offsets) {
@@ -370,7 +333,7 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
   }
 }
 
-// The places of the entries and the beginnings of the groups from the sorted keys (more than 255 groups).
+// The places of the entries and the beginnings of the groups from the sorted keys (more groups than one pass sorts).
 __global__ void __launch_bounds__(256) places_kernel(const uint32_t* __restrict__ keys,
                                                      const uint32_t* __restrict__ entries, uint32_t n, int groups,
                                                      int* __restrict__ order, int* __restrict__ slots,
@@ -413,73 +376,65 @@ inline Chunks chunks_for(long long n) {
   return {(int)((n + size - 1) / (size > 0 ? size : 1)), (uint32_t)size};
 }
 
-inline int passes_for(int bits) { return (bits + 7) / 8; }
-
-// Blocks for zeros beside a launch: 64 KB each at least, one per SM at most.
-inline int fill_blocks(const Zeros& z, int parts) {
-  const unsigned long long b = ((z.bytes[0] + z.bytes[1]) / parts + 65535) / 65536;
-  return (int)(b < 148 ? b : 148);
-}
+inline int passes_for(int bits) { return (bits + kMaxBits - 1) / kMaxBits; }
 
 // All passes over the low `bits` bits.  The last one writes `out`; the ones before it go to and
 // fro between the two buffers of keys and entries at `buffers` (of `len` words each).
 int sort_chunks(Source src, long long n, int bits, uint32_t* counts, uint32_t* buffers, size_t len, uint32_t* count,
-                Target out, const Zeros& zeros, cudaStream_t st) {
+                Target out, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed{0};
   CVHRF_CUDA_TRY(allow_shared(chunk_scatter_kernel, sizeof(Shared), allowed));
   const Chunks c = chunks_for(n);
   const int passes = passes_for(bits);
-  int shift[5] = {0}, radix[4];
+  int shift = 0;
   for (int p = 0; p < passes; ++p) {
-    int width = (bits - shift[p] + (passes - p) - 1) / (passes - p);   // the bits left, shared evenly
+    int width = (bits - shift + (passes - p) - 1) / (passes - p);   // the bits left, shared evenly
     if (width < 2) width = 2;   // the counts are read four digits at a time
-    radix[p] = 1 << width;
-    shift[p + 1] = shift[p] + width;
-  }
-  int clear = 0;
-  for (int p = 1; p < passes; ++p) clear += c.count * radix[p];
-  const int parts = passes + 1, more = fill_blocks(zeros, parts);
-  chunk_count_kernel<<<c.count + more, kThreads, 0, st>>>(src, (uint32_t)n, c.size, 0, radix[0], counts, clear,
-                                                          Fill{zeros, c.count, 0, parts});
-  CVHRF_LAUNCH_CHECK();
-  for (int p = 0; p < passes; ++p) {
     uint32_t* to = buffers + (p & 1) * 2 * len;
-    uint32_t* next = counts + (size_t)c.count * radix[p];
     Target t = out;
-    if (p + 1 < passes) t = Target{to, to + len, nullptr, nullptr, 0, nullptr, next, shift[p + 1], radix[p + 1]};
+    if (p + 1 < passes) t = Target{to, to + len, nullptr, nullptr, 0, nullptr, nullptr};
     t.count = p == 0 ? count : nullptr;
-    CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count + more), kThreads, sizeof(Shared), st, src,
-                                (uint32_t)n, p == 0 ? nullptr : count, c.size, (uint32_t)(0xffffffffull / c.size + 1), shift[p], radix[p], counts, t,
-                                Fill{zeros, c.count, p + 1, parts}));
+    const uint32_t* n_dev = p == 0 ? nullptr : count;
+    if (p == 0) {
+      chunk_count_kernel<<<c.count, kThreads, 0, st>>>(src, (uint32_t)n, n_dev, c.size, shift, 1 << width, counts,
+                                                       out.touched);
+      CVHRF_LAUNCH_CHECK();
+    } else {
+      CVHRF_CUDA_TRY(launch_after(chunk_count_kernel, dim3(c.count), kThreads, 0, st, src, (uint32_t)n, n_dev, c.size,
+                                  shift, 1 << width, counts, nullptr));
+      count_launch(1);
+    }
+    CVHRF_CUDA_TRY(launch_after(chunk_scatter_kernel, dim3(c.count), kThreads, sizeof(Shared), st, src, (uint32_t)n,
+                                n_dev, c.size, shift, 1 << width, counts, t));
     count_launch(1);
     src = Source{nullptr, 0, to, to + len, src.rows, 1};
-    counts = next;
+    shift += width;
   }
   return CVHRF_OK;
 }
 
-int small_sort(const Source& src, long long n, int bits, Target out, const Zeros& zeros, cudaStream_t st) {
+int small_sort(const Source& src, long long n, int bits, Target out, cudaStream_t st) {
   static std::atomic<unsigned long long> allowed{0};
   CVHRF_CUDA_TRY(allow_shared(small_sort_kernel, sizeof(Shared), allowed));
-  small_sort_kernel<<<1 + fill_blocks(zeros, 1), kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits,
-                                                                                 passes_for(bits), out,
-                                                                                 Fill{zeros, 1, 0, 1});
+  const bool clear = src.rows <= 1u << 20;   // more marks than the one block clears in a few microseconds
+  if (out.touched && !clear) CVHRF_CUDA_TRY(cudaMemsetAsync(out.touched, 0, src.rows, st));
+  small_sort_kernel<<<1, kThreads, sizeof(Shared), st>>>(src, (uint32_t)n, bits, passes_for(bits), out, clear);
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;
 }
 
 }  // namespace
 
-// scratch: count (64 words), the passes' matrices of counts, two buffers of keys and entries
-// (up to kTile keys only the result, of exactly that many)
-constexpr size_t kCountWords = 4 * (size_t)kMaxChunks * kMaxRadix;
+// scratch: count (64 words), the matrix of counts, two buffers of keys and entries (up to kTile
+// keys the result alone)
+constexpr size_t kCountWords = (size_t)kMaxChunks * kMaxRadix;
 size_t group_sort_words(long long n) {
   const size_t len = align_up((size_t)n, 64);
   return n <= kTile ? 64 + 2 * len : 64 + kCountWords + 4 * len;
 }
 
 int group_sort(const void* index, int index_bytes, long long n, long long rows, bool keep_outside, uint32_t* scratch,
-               const Zeros& zeros, cudaStream_t st, const uint32_t** keys, const uint32_t** entries,
+               uint8_t* touched, cudaStream_t st, const uint32_t** keys, const uint32_t** entries,
                const uint32_t** count_dev) {
   uint32_t* count = scratch;
   *count_dev = count;
@@ -490,9 +445,9 @@ int group_sort(const void* index, int index_bytes, long long n, long long rows, 
   uint32_t* to = buffers + (n <= kTile ? 0 : ((passes_for(bits) - 1) & 1) * 2 * len);
   *keys = to;
   *entries = to + len;
-  const Target out{to, to + len, nullptr, nullptr, 0, count, nullptr, 0, 0};
-  if (n <= kTile) return small_sort(src, n, bits, out, zeros, st);
-  return sort_chunks(src, n, bits, scratch + 64, buffers, len, count, out, zeros, st);
+  const Target out{to, to + len, nullptr, nullptr, 0, count, touched};
+  if (n <= kTile) return small_sort(src, n, bits, out, st);
+  return sort_chunks(src, n, bits, scratch + 64, buffers, len, count, out, st);
 }
 
 }  // namespace cvhrf
@@ -521,14 +476,13 @@ extern "C" int cvhrf_group_rows(const cvhrf_group_args* args, void* stream) {
   if ((uintptr_t)workspace & 15) return CVHRF_EINVAL;
   uint32_t* scratch = (uint32_t*)workspace;
   const Source src{index, index_bytes, nullptr, nullptr, (uint32_t)groups, 1};
-  const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr, nullptr, 0, 0};
+  const Target out{nullptr, (uint32_t*)order, slots, offsets, groups, nullptr, nullptr};
   const int bits = bits_for((unsigned long long)groups + 1);
-  const Zeros none{};
-  if (entries <= kTile) return small_sort(src, entries, bits, out, none, st);
-  // up to 255 groups (and the entries left out) one pass writes everything
-  if (groups < kMaxRadix) return sort_chunks(src, entries, bits, scratch + 64, nullptr, 0, scratch, out, none, st);
+  if (entries <= kTile) return small_sort(src, entries, bits, out, st);
+  // up to 511 groups (and the entries left out) one pass writes everything
+  if (groups < kMaxRadix) return sort_chunks(src, entries, bits, scratch + 64, nullptr, 0, scratch, out, st);
   const uint32_t *keys, *sorted, *count;
-  const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, none, st, &keys, &sorted, &count);
+  const int rc = group_sort(index, index_bytes, entries, groups, true, scratch, nullptr, st, &keys, &sorted, &count);
   if (rc) return rc;
   const long long most = entries > (long long)groups + 1 ? entries : (long long)groups + 1;
   CVHRF_CUDA_TRY(launch_after(places_kernel, dim3((unsigned)((most + 255) / 256)), 256, 0, st, keys, sorted,

@@ -6,12 +6,14 @@
 // Both are bound by memory: the lookup reads the distinct rows and writes T rows; the
 // gradient reads T rows and writes V.
 //
-// The gradient sorts the entries by row (row_groups.cu), which also sets the table to zero
-// beside its own work, and adds up runs of entries with the same row.  Every unit of lanes takes
-// an equal share of the sorted entries, whatever rows they belong to, so a row with very many
-// entries holds up nobody.  A row whose entries lie in several units is joined in the order of
-// the units: inside a block through shared memory, between blocks by table_join_kernel.  The
-// order of every sum is fixed, so results repeat.
+// The gradient sorts the entries by row (row_groups.cu, which also marks the rows that occur)
+// and adds up runs of entries with the same row.  Every unit of lanes takes an equal share of
+// the sorted entries, whatever rows they belong to, so a row with very many entries holds up
+// nobody.  A row whose entries lie in several units is joined in the order of the units: inside
+// a block through shared memory, between blocks by table_join_kernel.  The order of every sum
+// is fixed, so results repeat.  Blocks between those that add up write zeros into the rows that
+// do not occur: they only write and the others mostly read, and every row is written once.
+#include <algorithm>
 #include "row_groups.cuh"
 #include "row_types.cuh"
 #include "row_tiles.cuh"
@@ -227,7 +229,11 @@ struct Gradient {
   int lanes, units;          // lanes of a unit (up to 32), units of a block
   int items;                 // entries of a unit
   float scale;
-  uint8_t* mask;             // may be null
+  const uint8_t* touched;    // rows that occur
+  uint32_t table_rows;
+  int blocks, tiles;         // that add up: runs of entries x tiles of columns
+  int clear_blocks;          // that clear, spread between them
+  int clear_step;            // rows that a warp of theirs looks at together, 32 at most
 };
 
 // Columns per lane: one pack of aligned rows, or J single elements `lanes` apart (so that a
@@ -247,7 +253,25 @@ constexpr size_t gradient_shared() {   // staged rows and keys, heads and tails 
          3 * kThreads * sizeof(int);
 }
 
-// blockIdx.y: tile of columns.
+// Zeros into a share of the rows that do not occur, a warp per row.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void clear_rows(const Gradient& g, int share, T* __restrict__ out) {
+  const uint32_t warps = (uint32_t)g.clear_blocks * (kThreads / 32), lane = threadIdx.x & 31;
+  const uint32_t warp = (uint32_t)share * (kThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t step = g.clear_step;
+  for (unsigned long long r0 = (unsigned long long)warp * step; r0 < g.table_rows; r0 += (unsigned long long)warps * step) {
+    unsigned empty = __ballot_sync(0xffffffffu, lane < step && r0 + lane < g.table_rows && !g.touched[r0 + lane]);
+    if (!ALIGNED && g.width < 32) {   // narrow rows as one run of elements
+      T* to = out + (long long)r0 * g.width;
+      for (int e = lane; e < (int)step * g.width; e += 32)
+        if (empty >> (e / g.width) & 1) to[e] = from_float<T>(0.f);
+    } else {
+      for (; empty; empty &= empty - 1)
+        clear_row<T, ALIGNED ? kAligned : kSpan>(out + (long long)(r0 + __ffs(empty) - 1) * g.width, g.width, lane, 32);
+    }
+  }
+}
+
 template <typename T, bool ALIGNED, int J>
 __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, const T* __restrict__ grad,
                                                                   T* __restrict__ out, Joins joins) {
@@ -268,8 +292,14 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   uint32_t* keys = reinterpret_cast<uint32_t*>(tail_begun + kThreads);
   follow();
   let_next_start();
+  // block b adds up, or clears where b's share of the clearing blocks goes up by one
+  const int add_blocks = g.blocks * g.tiles;
+  const long long all = add_blocks + g.clear_blocks;
+  const int clears = (int)((long long)blockIdx.x * g.clear_blocks / all);
+  if ((int)(((long long)blockIdx.x + 1) * g.clear_blocks / all) > clears) return clear_rows<T, ALIGNED>(g, clears, out);
+  const int block = ((int)blockIdx.x - clears) / g.tiles, tile = ((int)blockIdx.x - clears) - block * g.tiles;
   const uint32_t n = *g.count;
-  const uint32_t block_items = units * g.items, first = min(n, blockIdx.x * block_items);
+  const uint32_t block_items = units * g.items, first = min(n, block * block_items);
   const int count = (int)min(block_items, n - first);
   const uint32_t before_first = first > 0 ? g.keys[first - 1] : 0xffffffffu;
   for (int i = threadIdx.x; i <= count; i += kThreads) {   // one more: whether the last row goes on
@@ -279,7 +309,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
   }
   __syncthreads();
   const int p0 = live ? min(unit * g.items, count) : count, p1 = min(p0 + g.items, count);
-  const int first_col = blockIdx.y * tile_width + lane * C::kVec;
+  const int first_col = tile * tile_width + lane * C::kVec;
   const int left = live ? g.width - first_col : 0;   // columns from the lane's first one on
   auto in = [&](int j) { return ALIGNED ? left > 0 : j * lanes < left; };
   float acc[kEach];
@@ -303,7 +333,6 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
       for (int j = 0; j < J; ++j)
         if (in(j)) to[j * lanes] = from_float<T>(g.scale * sum[j]);
     }
-    if (g.mask && lane == 0 && blockIdx.y == 0) g.mask[r] = 1;
   };
   auto end_row = [&]() {
     if (begun_before) {   // its other entries are elsewhere: leave the sum for the join
@@ -390,12 +419,12 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
       unfinished = true;
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        if (in(i)) joins.head[(long long)blockIdx.x * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
-      if (lane == 0 && blockIdx.y == 0) joins.head_row[blockIdx.x] = my_head;
+        if (in(i)) joins.head[(long long)block * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
+      if (lane == 0 && tile == 0) joins.head_row[block] = my_head;
     }
   }
   const int block_head = __syncthreads_or(unfinished);
-  if (!block_head && threadIdx.x == 0 && blockIdx.y == 0) joins.head_row[blockIdx.x] = -1;
+  if (!block_head && threadIdx.x == 0 && tile == 0) joins.head_row[block] = -1;
   // the row that goes on behind the block: the tail of its last unit with entries
   const int last = count > 0 ? (count - 1) / g.items : 0;
   if (unit == last) {
@@ -412,11 +441,11 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
       }
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        if (in(i)) joins.tail[(long long)blockIdx.x * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
+        if (in(i)) joins.tail[(long long)block * g.width + first_col + (ALIGNED ? i : i * lanes)] = sum[i];
     }
-    if (lane == 0 && blockIdx.y == 0) {
-      joins.tail_row[blockIdx.x] = r;
-      joins.tail_begun[blockIdx.x] = begun;
+    if (lane == 0 && tile == 0) {
+      joins.tail_row[block] = r;
+      joins.tail_begun[block] = begun;
     }
   }
 }
@@ -425,7 +454,7 @@ __global__ void __launch_bounds__(kThreads) table_gradient_kernel(Gradient g, co
 // blocks shared between `slices` threads of a column and then added in the slices' order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) table_join_kernel(Joins joins, int width, int columns, float scale,
-                                                              T* __restrict__ out, uint8_t* __restrict__ mask) {
+                                                              T* __restrict__ out) {
   __shared__ float part[kThreads];
   __shared__ int s_first;
   follow();
@@ -453,7 +482,6 @@ __global__ void __launch_bounds__(kThreads) table_join_kernel(Joins joins, int w
     for (int s = 1; s < slices; ++s) sum += part[s * columns + threadIdx.x];
     sum += joins.head[(long long)block * width + c];
     out[(long long)row * width + c] = from_float<T>(scale * sum);
-    if (mask && c == 0) mask[row] = 1;
   }
 }
 
@@ -496,13 +524,20 @@ int launch_gradient(Gradient g, int lanes, long long n, const void* grad, void* 
   joins.head_row = (int*)(joins.tail + blocks * g.width);
   joins.tail_row = joins.head_row + blocks;
   joins.tail_begun = joins.tail_row + blocks;
-  CVHRF_CUDA_TRY(launch_after(table_gradient_kernel<T, ALIGNED, J>, dim3((unsigned)blocks, tiles), kThreads, shared, st,
-                              g, (const T*)grad, (T*)out, joins));
+  g.blocks = (int)blocks;
+  g.tiles = tiles;
+  // enough blocks that clear for every SM, each warp with 4 to 32 rows
+  g.clear_step = (int)std::min(32ll, std::max(4ll, (long long)g.table_rows / (148 * 32)));
+  const long long per_block = g.clear_step * (kThreads / 32);
+  g.clear_blocks = (int)std::min((g.table_rows + per_block - 1) / per_block, 148ll * 64);
+  if (blocks * tiles > 0x7fffffff - g.clear_blocks) return CVHRF_EUNSUPPORTED;
+  CVHRF_CUDA_TRY(launch_after(table_gradient_kernel<T, ALIGNED, J>, dim3((unsigned)(blocks * tiles + g.clear_blocks)),
+                              kThreads, shared, st, g, (const T*)grad, (T*)out, joins));
   count_launch(1);
   if (blocks == 1) return CVHRF_OK;
   const int columns = next_pow2(g.width < kThreads ? g.width : kThreads);
   CVHRF_CUDA_TRY(launch_after(table_join_kernel<T>, dim3((unsigned)blocks, (g.width + columns - 1) / columns), kThreads,
-                              0, st, joins, g.width, columns, g.scale, (T*)out, g.mask));
+                              0, st, joins, g.width, columns, g.scale, (T*)out));
   count_launch(1);
   return CVHRF_OK;
 }
@@ -510,9 +545,9 @@ int launch_gradient(Gradient g, int lanes, long long n, const void* grad, void* 
 // Units of as many lanes as a row has packs or elements, a warp at most; wider rows have several
 // elements per lane, then tiles.
 template <typename T>
-int gradient(const void* grad, long long stride, int width, long long n, float scale, void* out, uint8_t* mask,
-             const uint32_t* keys, const uint32_t* entries, const uint32_t* count, float* joins, cudaStream_t st) {
-  const Gradient g{keys, entries, count, stride, width, 0, 0, 0, scale, mask};
+int gradient(const void* grad, long long stride, int width, long long n, long long rows, float scale, void* out,
+             const uint8_t* touched, const uint32_t* keys, const uint32_t* entries, const uint32_t* count, float* joins, cudaStream_t st) {
+  const Gradient g{keys, entries, count, stride, width, 0, 0, 0, scale, touched, (uint32_t)rows, 0, 0, 0};
   if (rows_16(grad, stride, width, sizeof(T)) && ((uintptr_t)out & 15) == 0) {
     const int packs = packs_of<T, kAligned>(width);
     return launch_gradient<T, true, 1>(g, packs < 32 ? packs : 32, n, grad, out, joins, st);
@@ -551,7 +586,7 @@ extern "C" int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream) {
 extern "C" size_t cvhrf_table_gradient_workspace_bytes(long long entries, long long rows, int width) {
   if (entries < 0 || entries > kGroupMaxEntries || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth)
     return 0;
-  return align_up(group_sort_words(entries) * sizeof(uint32_t), 256) +
+  return align_up(group_sort_words(entries) * sizeof(uint32_t), 256) + align_up((size_t)rows, 256) +
          align_up((size_t)most_blocks(entries) * (2 * (size_t)width * sizeof(float) + 3 * sizeof(int)), 256);
 }
 
@@ -577,16 +612,17 @@ extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* strea
   if ((uintptr_t)workspace & 15) return CVHRF_EINVAL;
   uint32_t* scratch = (uint32_t*)workspace;
   const uint32_t *keys, *sorted, *count;
-  const Zeros zeros{{grad_table, row_mask}, {(unsigned long long)rows * width * elem, row_mask ? (unsigned long long)rows : 0}};
-  const int rc = group_sort(index, index_bytes, entries, rows, false, scratch, zeros, st, &keys, &sorted, &count);
+  char* after = (char*)workspace + align_up(group_sort_words(entries) * sizeof(uint32_t), 256);
+  uint8_t* touched = row_mask ? row_mask : (uint8_t*)after;
+  float* joins = (float*)(after + align_up((size_t)rows, 256));
+  const int rc = group_sort(index, index_bytes, entries, rows, false, scratch, touched, st, &keys, &sorted, &count);
   if (rc) return rc;
-  float* joins = (float*)((char*)workspace + align_up(group_sort_words(entries) * sizeof(uint32_t), 256));
   if (dtype == CVHRF_F32)
-    return gradient<float>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted, count,
+    return gradient<float>(grad, grad_stride, width, entries, rows, scale, grad_table, touched, keys, sorted, count,
                            joins, st);
   if (dtype == CVHRF_BF16)
-    return gradient<__nv_bfloat16>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted,
+    return gradient<__nv_bfloat16>(grad, grad_stride, width, entries, rows, scale, grad_table, touched, keys, sorted,
                                    count, joins, st);
-  return gradient<__half>(grad, grad_stride, width, entries, scale, grad_table, row_mask, keys, sorted, count,
+  return gradient<__half>(grad, grad_stride, width, entries, rows, scale, grad_table, touched, keys, sorted, count,
                           joins, st);
 }

@@ -133,7 +133,7 @@ def test_gradient_of_skewed_rows(cuda, kind, n, rows, width, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [255, 256, 257, 65535, 65536, 65537, (1 << 24) + 3])
+@pytest.mark.parametrize("rows", [255, 256, 257, 511, 512, 513, 65536, 262144, 262145, (1 << 24) + 3])
 def test_gradient_at_the_edges_of_the_sort(cuda, rows):
     index = torch.cat([integers(5000, rows, rows), torch.tensor([0, rows - 1, rows - 1, rows, -1], device="cuda")])
     grad = normal((index.numel(), 2), torch.float32, 1)
@@ -244,8 +244,8 @@ def places_64(index, groups):
 
 
 @gpu
-@pytest.mark.parametrize("groups", [1, 2, 3, 7, 64, 254, 255, 256, 257, 1000, 70000])
-@pytest.mark.parametrize("n,k", [(1, 1), (31, 1), (5, 3), (1024, 1), (1025, 2), (20011, 4), (310007, 1)])
+@pytest.mark.parametrize("groups", [1, 2, 3, 7, 64, 255, 256, 510, 511, 512, 1000, 70000])
+@pytest.mark.parametrize("n,k", [(1, 1), (31, 1), (5, 3), (1024, 1), (1025, 2), (4096, 2), (8193, 1), (20011, 4), (310007, 1)])
 def test_groups(cuda, groups, n, k):
     for itype in (torch.int32, torch.int64):
         index = integers(n * k, groups + 1, n + groups, -1, itype).reshape(n, k)
