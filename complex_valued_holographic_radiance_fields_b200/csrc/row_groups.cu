@@ -10,8 +10,9 @@
 // launch for the histogram, and a walk over the earlier tiles in L2 latency.)
 // The first pass reads the caller's indices as they are (4 or 8 bytes).
 //
-// Bound by latency: one block of 1024 threads per SM takes a chunk of up to 8192 keys in
-// registers, so a pass is a handful of dependent steps.  Up to 8192 keys in all, one block
+// Bound by latency and by the instructions around the keys: one block of 1024 threads per SM
+// takes a chunk of up to 8192 keys in registers, so a pass is a handful of dependent steps
+// (512 threads: 18 us a pass for 1M keys, against 15).  Up to 8192 keys in all, one block
 // does every pass in shared memory (small_sort_kernel, one launch).
 #include "row_groups.cuh"
 #include "row_types.cuh"
@@ -23,6 +24,7 @@ constexpr int kThreads = 1024, kWarps = kThreads / 32, kItems = 8, kTile = kThre
 constexpr int kMaxChunks = 148;   // one block per SM
 constexpr int kMaxBits = 9, kMaxRadix = 1 << kMaxBits;
 constexpr uint32_t kNone = 0xffffffffu;
+static_assert(kThreads == 2 * kMaxRadix, "two threads per digit");
 
 struct Source {
   const void* index;         // the caller's indices in the first pass
@@ -83,19 +85,23 @@ __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_
     uint32_t key[kItems];
 #pragma unroll
     for (int r = 0; r < kItems; ++r) {
+      key[r] = kNone;
+      if (tile + r * kThreads >= end) continue;
       const uint32_t i = tile + r * kThreads + threadIdx.x;
-      key[r] = i < end ? source_key(s, i) : kNone;
+      if (i < end) key[r] = source_key(s, i);
     }
 #pragma unroll
-    for (int r = 0; r < kItems; ++r)
+    for (int r = 0; r < kItems; ++r) {
+      if (tile + r * kThreads >= end) break;
       if (key[r] != kNone) atomicAdd(&mine[(key[r] >> shift) & (radix - 1)], 1u);
+    }
   }
   __syncthreads();
-  if (threadIdx.x < radix) {
+  for (int d = threadIdx.x; d < radix; d += kThreads) {
     uint32_t c = 0;
 #pragma unroll
-    for (int w = 0; w < kCopies; ++w) c += h[w][threadIdx.x];
-    counts[(size_t)blockIdx.x * radix + threadIdx.x] = c;
+    for (int w = 0; w < kCopies; ++w) c += h[w][d];
+    counts[(size_t)blockIdx.x * radix + d] = c;
   }
 }
 
@@ -105,6 +111,7 @@ struct Shared {
   uint32_t base[kMaxRadix];            // place of the chunk's next key with this digit
   uint32_t start[kMaxRadix];           // start of the digit inside the tile
   uint32_t delta[kMaxRadix];           // base - start
+  uint32_t lower[kMaxRadix], upper[kMaxRadix];   // keys of the digit in either half of the warps
   uint32_t sh[kMaxRadix / 32 + 1];
 };
 
@@ -147,7 +154,7 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
   const int radix = 1 << width;
   const uint32_t mask = radix - 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < kWarps * radix; i += kThreads) sh.cnt[i] = 0;
+  for (int i = tid; i < kWarps * radix / 4; i += kThreads) reinterpret_cast<uint4*>(sh.cnt)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   const unsigned lt = (1u << lane) - 1u;
   uint32_t* mine = sh.cnt + warp * radix;
@@ -178,16 +185,23 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
     __syncwarp();
   }
   __syncthreads();
+  // per digit: where each warp's keys begin, the upper half of the warps by the upper threads
+  constexpr int kHalf = kWarps / 2;
+  const int d0 = tid & (kMaxRadix - 1), w0 = tid / kMaxRadix * kHalf;
   uint32_t run = 0;
-  if (tid < radix) {
+  if (d0 < radix) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const uint32_t c = sh.cnt[w * radix + tid];
-      sh.cnt[w * radix + tid] = run;
+    for (int w = 0; w < kHalf; ++w) {
+      const uint32_t c = sh.cnt[(w0 + w) * radix + d0];
+      sh.cnt[(w0 + w) * radix + d0] = run;
       run += c;
     }
   }
-  const uint32_t start = scan_radix(run, sh.sh, kept);
+  if (tid < kMaxRadix) sh.lower[tid] = run;
+  else sh.upper[tid - kMaxRadix] = run;
+  __syncthreads();
+  if (tid < kMaxRadix) run += sh.upper[tid];
+  const uint32_t start = scan_radix(tid < kMaxRadix ? run : 0u, sh.sh, kept);
   if (tid < kMaxRadix) sh.start[tid] = start;
   __syncthreads();
 #pragma unroll
@@ -195,7 +209,7 @@ __device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[
     if (r >= rounds) break;
     if (key[r] == kNone) continue;
     const uint32_t d = (key[r] >> shift) & mask;
-    place[r] += mine[d];
+    place[r] += mine[d] + (warp >= kHalf ? sh.lower[d] : 0u);
     const uint32_t at = sh.start[d] + place[r];
     sh.key[at] = key[r];
     sh.entry[at] = entry[r];
@@ -225,25 +239,39 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
     const uint32_t base = tile + warp * (32 * rounds) + lane;
 #pragma unroll
     for (int r = 0; r < kItems; ++r) {
+      key[r] = kNone;
+      if (r >= rounds) continue;
       const uint32_t i = base + r * 32;
-      const bool in = r < rounds && i < end;
-      key[r] = in ? source_key(s, i) : kNone;
-      entry[r] = in ? (s.bytes ? i : s.entries[i]) : 0u;
+      if (i < end) {
+        key[r] = source_key(s, i);
+        entry[r] = s.bytes ? i : s.entries[i];
+      }
     }
   };
   if (begin < end) load(begin);   // on its way while the matrix of counts is added up
   // the matrix of counts: four digits per thread, the chunks shared between the threads
   {
-    const int quads = radix >> 2, shares = kThreads / quads, share = tid / quads, q = tid - share * quads;
+    const int quads = radix >> 2, shares = min(kThreads / quads, 16), share = tid / quads, q = tid - share * quads;
     uint4 before4 = make_uint4(0, 0, 0, 0), all4 = before4;
-#pragma unroll 10
-    for (int c = share; c < chunks; c += shares) {
-      const uint4 v = reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q];
-      all4.x += v.x, all4.y += v.y, all4.z += v.z, all4.w += v.w;
-      if (c < (int)blockIdx.x) before4.x += v.x, before4.y += v.y, before4.z += v.z, before4.w += v.w;
+    constexpr int kLoads = 10;   // in flight: all of them up to 256 digits
+    for (int c0 = share; share < shares && c0 < chunks; c0 += kLoads * shares) {
+      uint4 v[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int c = c0 + i * shares;
+        v[i] = c < chunks ? reinterpret_cast<const uint4*>(counts)[(size_t)c * quads + q] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        all4.x += v[i].x, all4.y += v[i].y, all4.z += v[i].z, all4.w += v[i].w;
+        if (c0 + i * shares < (int)blockIdx.x)
+          before4.x += v[i].x, before4.y += v[i].y, before4.z += v[i].z, before4.w += v[i].w;
+      }
     }
-    reinterpret_cast<uint4*>(sh.key)[tid] = before4;   // shares x radix
-    reinterpret_cast<uint4*>(sh.entry)[tid] = all4;
+    if (share < shares) {
+      reinterpret_cast<uint4*>(sh.key)[tid] = before4;   // shares x radix
+      reinterpret_cast<uint4*>(sh.entry)[tid] = all4;
+    }
     __syncthreads();
     uint32_t before = 0, all = 0;
     if (tid < radix) {
@@ -266,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint3
     if (out.slots) {   // first and only pass: the entries are the items in order
 #pragma unroll
       for (int r = 0; r < kItems; ++r)
-        if (key[r] != kNone)
+        if (r < rounds && key[r] != kNone)
           out.slots[entry[r]] =
               key[r] < (uint32_t)out.groups ? (int)(sh.base[(key[r] >> shift) & mask] + place[r]) : -1;
     }
@@ -303,10 +331,13 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
     const int rounds = (int)((kept + kThreads - 1) / kThreads);
 #pragma unroll
     for (int r = 0; r < kItems; ++r) {
+      key[r] = kNone;
+      if (r >= rounds) continue;
       const uint32_t i = warp * (32 * rounds) + r * 32 + lane;
-      const bool in = r < rounds && i < kept;
-      key[r] = !in ? kNone : p == 0 ? source_key(s, i) : sh.key[i];
-      entry[r] = !in ? 0u : p == 0 ? i : sh.entry[i];
+      if (i < kept) {
+        key[r] = p == 0 ? source_key(s, i) : sh.key[i];
+        entry[r] = p == 0 ? i : sh.entry[i];
+      }
     }
     __syncthreads();
     sort_tile(sh, key, entry, place, rounds, done, width, kept);

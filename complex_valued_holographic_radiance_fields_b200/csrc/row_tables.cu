@@ -208,7 +208,7 @@ int lookup(const void* table, long long rows, int width, long long stride, const
 }
 
 // ---- gradient -------------------------------------------------------------------------
-constexpr int kBlockItems = 1024;   // most entries of a block, staged in shared memory
+constexpr int kBlockItems = 2048;   // most entries of a block, staged in shared memory
 
 // What a block leaves for table_join_kernel: the part of a row that began in an earlier
 // block and ends in this one (head), and of the row that goes on behind its end (tail).
