@@ -136,11 +136,11 @@ struct Places {
   }
 };
 
-template <typename T, bool WIDE, int ROWS, int J>
+template <typename T, typename S>
 __global__ void __launch_bounds__(kTileThreads) rows_to_groups_tile_kernel(Places places, long long count, int tile,
                                                                            int width, const T* __restrict__ x,
                                                                            long long stride, T* __restrict__ out) {
-  gather_tile<T, false, WIDE, ROWS, J>(
+  gather_tile<T, false, S::kPairs, S::kWide, S::kRows, S::kJ>(
       [&](long long p) -> const T* {
         const long long n = places.row(p);
         return n >= 0 ? x + n * stride : nullptr;
@@ -191,7 +191,7 @@ __device__ __forceinline__ void load_choices(const Moves& m, const Weights& weig
 
 // An owner has one pack of CHOICES choices of each of ROWS rows in flight.
 template <typename T, Layout L, int ROWS, int CHOICES>
-__global__ void __launch_bounds__(kThreads, 4) groups_to_rows_kernel(Moves m, const T* __restrict__ y, Extent extent,
+__global__ void __launch_bounds__(kThreads, 5) groups_to_rows_kernel(Moves m, const T* __restrict__ y, Extent extent,
                                                                      long long stride, Weights weights,
                                                                      T* __restrict__ out) {
   using R = Row<T, L>;
@@ -534,16 +534,12 @@ int to_groups(bool aligned, const void* x, long long stride, Moves m, const int*
     const int tile = tile_rows(count, m.width, sizeof(T));
     const unsigned blocks = (unsigned)((count + tile - 1) / tile);
     const size_t shared = (size_t)tile * m.width * sizeof(T);
-#define CVHRF_LAUNCH(WIDE, ROWS, J)                                                        \
-  rows_to_groups_tile_kernel<T, WIDE, ROWS, J><<<blocks, kTileThreads, shared, st>>>(      \
-      places, count, tile, m.width, (const T*)x, stride, (T*)out)
-    if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
-    else if (m.width > 64) CVHRF_LAUNCH(false, 2, 4);
-    else if (m.width > 32) CVHRF_LAUNCH(false, 4, 2);
-    else CVHRF_LAUNCH(false, 8, 1);
-#undef CVHRF_LAUNCH
-    CVHRF_LAUNCH_CHECK();
-    return CVHRF_OK;
+    return with_shape<T>(m.width, [&](auto shape) {
+      rows_to_groups_tile_kernel<T, decltype(shape)><<<blocks, kTileThreads, shared, st>>>(
+          places, count, tile, m.width, (const T*)x, stride, (T*)out);
+      CVHRF_LAUNCH_CHECK();
+      return CVHRF_OK;
+    });
   }
   return with_layout<T>(aligned, m.width, [&](auto layout, int lanes) {
     constexpr Layout L = decltype(layout)::value;
@@ -574,7 +570,9 @@ int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weig
 #define CVHRF_LAUNCH(WIDE, J)                                                          \
   groups_to_rows_tile_kernel<T, WIDE, J><<<blocks, kTileThreads, shared, st>>>(        \
       m.n, m.choices, tile, m.width, m.slots, (const T*)y, stride, weights, (T*)out)
-    if (m.width > 128) CVHRF_LAUNCH(true, 8);
+    const int steps = (m.width + 255) / 256;   // J shares the row evenly between them
+    if (m.width > 128 && m.width <= steps * 192) CVHRF_LAUNCH(true, 6);
+    else if (m.width > 128) CVHRF_LAUNCH(true, 8);
     else if (m.width > 64) CVHRF_LAUNCH(false, 4);
     else if (m.width > 32) CVHRF_LAUNCH(false, 2);
     else CVHRF_LAUNCH(false, 1);
@@ -616,7 +614,9 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
 #define CVHRF_LAUNCH(WIDE, ROWS, J)                                                               \
   groups_to_rows_backward_tile_kernel<T, WIDE, ROWS, J><<<blocks, kTileThreads, shared, st>>>(    \
       places, count, tile, m.width, (const T*)grad, grad_stride, (const T*)y, stride, weights, (T*)grad_y, grad_weights)
-    if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
+    const int steps = (m.width + 255) / 256;
+    if (m.width > 128 && m.width <= steps * 192) CVHRF_LAUNCH(true, 1, 6);
+    else if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
     else if (m.width > 64) CVHRF_LAUNCH(false, 1, 4);
     else if (m.width > 32) CVHRF_LAUNCH(false, 2, 2);
     else CVHRF_LAUNCH(false, 4, 1);

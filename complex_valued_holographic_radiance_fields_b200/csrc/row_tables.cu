@@ -85,29 +85,18 @@ __global__ void __launch_bounds__(kThreads, 4) table_lookup_kernel(const T* __re
 }
 
 // Rows that are not aligned, up to 4 KB.
-template <typename T, bool WIDE, int ROWS, int J>
+template <typename T, typename S>
 __global__ void __launch_bounds__(kTileThreads) table_lookup_tile_kernel(const T* __restrict__ table, long long rows,
                                                                          int width, long long stride,
                                                                          const void* __restrict__ index,
                                                                          int index_bytes, long long entries, int tile,
                                                                          float scale, T* __restrict__ out) {
-  gather_tile<T, true, WIDE, ROWS, J>(
+  gather_tile<T, true, S::kPairs, S::kWide, S::kRows, S::kJ>(
       [&](long long t) -> const T* {
         const long long v = table_row(index, index_bytes, t, rows);
         return v >= 0 ? table + v * stride : nullptr;
       },
       entries, tile, width, scale, out);
-}
-
-template <typename T, bool WIDE, int ROWS, int J>
-int launch_lookup_tile(const void* table, long long rows, int width, long long stride, const void* index,
-                       int index_bytes, long long entries, float scale, void* out, cudaStream_t st) {
-  const int tile = tile_rows(entries, width, sizeof(T));
-  table_lookup_tile_kernel<T, WIDE, ROWS, J>
-      <<<(unsigned)((entries + tile - 1) / tile), kTileThreads, (size_t)tile * width * sizeof(T), st>>>(
-          (const T*)table, rows, width, stride, index, index_bytes, entries, tile, scale, (T*)out);
-  CVHRF_LAUNCH_CHECK();
-  return CVHRF_OK;
 }
 
 // ... of a few elements.
@@ -191,13 +180,14 @@ int lookup(const void* table, long long rows, int width, long long stride, const
     return CVHRF_OK;
   }
   if (tile_fits(width, sizeof(T), out)) {
-#define CVHRF_LOOKUP_TILE(WIDE, ROWS, J) \
-  launch_lookup_tile<T, WIDE, ROWS, J>(table, rows, width, stride, index, index_bytes, entries, scale, out, st)
-    if (width > 128) return CVHRF_LOOKUP_TILE(true, 1, 8);
-    if (width > 64) return CVHRF_LOOKUP_TILE(false, 2, 4);
-    if (width > 32) return CVHRF_LOOKUP_TILE(false, 4, 2);
-    return CVHRF_LOOKUP_TILE(false, 8, 1);
-#undef CVHRF_LOOKUP_TILE
+    const int tile = tile_rows(entries, width, sizeof(T));
+    return with_shape<T>(width, [&](auto shape) {
+      table_lookup_tile_kernel<T, decltype(shape)>
+          <<<(unsigned)((entries + tile - 1) / tile), kTileThreads, (size_t)tile * width * sizeof(T), st>>>(
+              (const T*)table, rows, width, stride, index, index_bytes, entries, tile, scale, (T*)out);
+      CVHRF_LAUNCH_CHECK();
+      return CVHRF_OK;
+    });
   }
   const int words = words_of<T>(width);
   if (words > 64)

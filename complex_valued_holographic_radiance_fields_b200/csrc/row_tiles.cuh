@@ -7,6 +7,7 @@
 // and were bound by that: 63 us against 45 for 1M rows of 59 floats.  Addresses are worked out
 // by one lane per row and shuffled.
 #pragma once
+#include <type_traits>
 #include "row_types.cuh"
 
 namespace cvhrf {
@@ -74,9 +75,51 @@ __device__ __forceinline__ void rows_to_tile(const T* (&from)[ROWS], T* to, int 
   }
 }
 
+// The same for 16-bit elements by pairs: words of the row that is read, stored as they are or in
+// two halves where the tile has them on the other side of a word.
+template <typename T, bool SCALE, bool WIDE, int ROWS, int J>
+__device__ __forceinline__ void pairs_to_tile(const T* (&from)[ROWS], T* to, int width, int lane, float scale) {
+  static_assert(sizeof(T) == 2);
+  struct alignas(4) Two { T a, b; };
+  int head[ROWS], words[ROWS];   // elements before the first whole word, whole words
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q) {
+    head[q] = (int)((uintptr_t)from[q] >> 1) & 1;
+    words[q] = (width - head[q]) >> 1;
+  }
+#pragma unroll 1
+  for (int c = lane;; c += 32 * J) {
+    Two v[ROWS][J];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (c + 32 * j < words[q]) v[q][j] = reinterpret_cast<const Two*>(from[q] + head[q])[c + 32 * j];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      T* d = to + q * width + head[q] + 2 * c;
+      const bool whole = ((uintptr_t)d & 2) == 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (c + 32 * j < words[q]) {
+          Two o = v[q][j];
+          if (SCALE) o = {from_float<T>(scale * to_float(o.a)), from_float<T>(scale * to_float(o.b))};
+          if (whole) *reinterpret_cast<Two*>(d + 64 * j) = o;
+          else d[64 * j] = o.a, d[64 * j + 1] = o.b;
+        }
+    }
+    if (!WIDE || (c - lane + 32 * J) * 2 >= width) break;
+  }
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q) {
+    const int e = lane == 0 && head[q] ? 0 : lane == 1 && ((width - head[q]) & 1) ? width - 1 : -1;
+    if (e >= 0) to[q * width + e] = SCALE ? from_float<T>(scale * to_float(from[q][e])) : from[q][e];
+  }
+}
+
 // out[i] = scale * (the row get(i), null: zeros), SCALE; else the row bit for bit.  A lane has
-// ROWS x J elements in flight.
-template <typename T, bool SCALE, bool WIDE, int ROWS, int J, typename Get>
+// ROWS x J elements (PAIRS: pairs) in flight.
+template <typename T, bool SCALE, bool PAIRS, bool WIDE, int ROWS, int J, typename Get>
 __device__ __forceinline__ void gather_tile(const Get& get, long long rows, int tile, int width, float scale,
                                             T* __restrict__ out) {
   extern __shared__ __align__(16) unsigned char raw[];
@@ -87,21 +130,49 @@ __device__ __forceinline__ void gather_tile(const Get& get, long long rows, int 
   const T* row = nullptr;
   if (lane < each && r0 + lane < n) row = get(first + r0 + lane);
   const unsigned long long mine = (unsigned long long)(uintptr_t)(row ? row : reinterpret_cast<const T*>(g_zero_row));
-  T* to = buf + r0 * width + lane;
-  int r = 0;
-  for (; r + ROWS <= each; r += ROWS) {
-    const T* from[ROWS];
+  T* to = buf + r0 * width + (PAIRS ? 0 : lane);
+  auto copy = [&](auto count, int r) {
+    constexpr int kCount = decltype(count)::value;
+    const T* from[kCount];
 #pragma unroll
-    for (int q = 0; q < ROWS; ++q) from[q] = reinterpret_cast<const T*>((uintptr_t)shuffle(mine, r + q)) + lane;
-    rows_to_tile<T, SCALE, WIDE, ROWS, J>(from, to, width, width - lane, scale);
-    to += ROWS * width;
-  }
-  for (; ROWS > 1 && r < each; ++r) {
-    const T* from[1] = {reinterpret_cast<const T*>((uintptr_t)shuffle(mine, r)) + lane};
-    rows_to_tile<T, SCALE, WIDE, 1, J>(from, to, width, width - lane, scale);
-    to += width;
-  }
+    for (int q = 0; q < kCount; ++q)
+      from[q] = reinterpret_cast<const T*>((uintptr_t)shuffle(mine, r + q)) + (PAIRS ? 0 : lane);
+    if constexpr (PAIRS) pairs_to_tile<T, SCALE, WIDE, kCount, J>(from, to, width, lane, scale);
+    else rows_to_tile<T, SCALE, WIDE, kCount, J>(from, to, width, width - lane, scale);
+    to += kCount * width;
+  };
+  int r = 0;
+  for (; r + ROWS <= each; r += ROWS) copy(std::integral_constant<int, ROWS>(), r);
+  for (; ROWS > 1 && r < each; ++r) copy(std::integral_constant<int, 1>(), r);
   send_tile(buf, n, width, out + first * width);
+}
+
+// Calls f<PAIRS, WIDE, ROWS, J> for rows of `width` elements: J shares the row evenly between
+// the lanes' steps (333 elements in two steps of 6, not of 8 and 3), narrow rows go several at
+// a time.
+template <int A, int B, int C, int D>
+struct Shape4 {
+  static constexpr bool kPairs = A, kWide = B;
+  static constexpr int kRows = C, kJ = D;
+};
+template <typename T, typename F>
+int with_shape(int width, F f) {
+  if constexpr (sizeof(T) == 2) {
+    if (width >= 64) {
+      const int words = (width + 1) / 2, steps = (words + 255) / 256, j = (words + 32 * steps - 1) / (32 * steps);
+      if (steps > 1) return j <= 6 ? f(Shape4<1, 1, 1, 6>()) : f(Shape4<1, 1, 1, 8>());
+      if (j > 6) return f(Shape4<1, 0, 1, 8>());
+      if (j > 4) return f(Shape4<1, 0, 1, 6>());
+      if (j > 2) return f(Shape4<1, 0, 2, 4>());
+      return f(Shape4<1, 0, 4, 2>());
+    }
+  }
+  const int steps = (width + 255) / 256, j = (width + 32 * steps - 1) / (32 * steps);
+  if (steps > 1) return j <= 6 ? f(Shape4<0, 1, 1, 6>()) : f(Shape4<0, 1, 1, 8>());
+  if (j > 4) return f(Shape4<0, 0, 1, 8>());
+  if (j > 2) return f(Shape4<0, 0, 2, 4>());
+  if (j > 1) return f(Shape4<0, 0, 4, 2>());
+  return f(Shape4<0, 0, 8, 1>());
 }
 
 // The same for rows of a few elements, where a row would leave most of a warp idle: four bytes
