@@ -112,6 +112,8 @@ def dp_step(trainer, target=None, group=None):
     """
     from . import _lib
     import ctypes
+    if getattr(trainer, "tables", None):
+        raise ValueError("shared_rows trains on one GPU: their gradients are not exchanged")
     for p in trainer.params.values():
         p.grad = None
     loss, visible = trainer.forward(target)

@@ -21,8 +21,16 @@ re-captures with a larger capacity.
 The reference optimizer receives the rasterizer's ``visible_indices``, which index the
 depth-sorted subset, not the parameter rows; here they are mapped back through the
 sort permutation (``idxs[visible]``) so the update lands on the rows that were seen.
+
+With ``shared_rows`` some attributes come from codebooks: a table of rows per attribute and
+an integer code per Gaussian (``rows.table_lookup``).  The tables are trained in place of
+the attributes, sparse Adam updating the table rows that a visible Gaussian names.
 """
+import ctypes
+
 import torch
+
+from . import _lib
 
 from . import scene as SC
 from .density import density_control, opacity_regularization
@@ -30,6 +38,7 @@ from .loss import intensity_l2_loss
 from .optimizer import Adan, SparseGaussianAdam
 from .propagation import propagate_planes
 from .reconstruction import MultiplaneLoss, Propagator, hologram_training_loss
+from .rows import table_lookup
 from . import rasterizer as RZ
 from .rasterizer import SplatTileCudaCapacity, splat_tile_cuda
 
@@ -45,7 +54,12 @@ def plane_distances(K, volume_depth=4e-3, d_val=-2e-3):
 class HoloTrainer:
     def __init__(self, N=300000, W=800, H=800, K=3, pitch=8e-6, lr=1e-3, eps=1e-15, seed=0, device="cuda",
                  camera=None, wavelengths=None, target=None, S=None, frustum=None, optimizer="sparse_adam",
-                 loss="l2", image=None, depth=None):
+                 loss="l2", image=None, depth=None, shared_rows=None):
+        """`shared_rows`: {attribute: number of table rows} of the attributes that come from a
+        codebook (2-D ones: pre_act_quats, pre_act_scales, colours, pre_act_phase,
+        pre_act_plane_assignment).  `tables[attribute]` holds the rows (trained),
+        `codes[attribute]` each Gaussian's row (int32, seeded at random; assign your own).
+        One GPU, no densification."""
         self.device = torch.device(device)
         self.W, self.H, self.K = W, H, K
         self.S = S or max(W, H)   # pad size (train.py: max(W, H) unless configured)
@@ -61,6 +75,18 @@ class HoloTrainer:
         if optimizer not in ("adan", "sparse_adam"):
             raise ValueError(f"unknown optimizer {optimizer!r}")
         self.optimizer, self.lr, self.eps = optimizer, lr, eps
+        self.tables, self.codes = {}, {}
+        g = torch.Generator().manual_seed(seed + 1)
+        for k, rows in (shared_rows or {}).items():
+            if k == "means" or k not in self.params or self.params[k].dim() != 2:
+                raise ValueError(f"{k!r} cannot come from shared rows")
+            if not 1 <= rows <= N:
+                raise ValueError(f"{k}: {rows} shared rows for {N} Gaussians")
+            if type(self) is not HoloTrainer:
+                raise ValueError("shared_rows trains on one GPU (HoloTrainer)")
+            # the first rows of the scene's own values; the Gaussians' own are dropped
+            self.tables[k] = self.params.pop(k).detach()[:rows].clone().requires_grad_(True)
+            self.codes[k] = torch.randint(0, rows, (N,), generator=g, dtype=torch.int32).to(self.device)
         self.opt = self._make_optimizer()
         if loss not in ("l2", "multiplane"):
             raise ValueError(f"unknown loss {loss!r}")
@@ -95,9 +121,35 @@ class HoloTrainer:
             # (utils/optimizer.py:44-65); dense, eager steps only (its scalars change every step)
             lrs = {"pre_act_scales": 0.005, "pre_act_phase": 0.0025, "colours": 0.0025, "means": self.lr,
                    "pre_act_opacities": 0.025, "pre_act_plane_assignment": self.lr, "pre_act_quats": 0.001}
-            return Adan([{"params": [p], "lr": lrs[k]} for k, p in self.params.items()], lr=0, eps=1e-8)
+            return Adan([{"params": [p], "lr": lrs[k]} for k, p in self._leaves()], lr=0, eps=1e-8)
+        self.table_opts = {k: SparseGaussianAdam([{"params": [t], "lr": self.lr}], lr=self.lr, eps=self.eps)
+                           for k, t in self.tables.items()}
         return SparseGaussianAdam([{"params": [p], "lr": self.lr} for p in self.params.values()], lr=self.lr,
                                   eps=self.eps)
+
+    def _leaves(self):
+        """(name, tensor) of everything that is trained."""
+        return [*self.params.items(), *self.tables.items()]
+
+    def _zero_grad(self):
+        for _, p in self._leaves():
+            p.grad = None
+
+    def scene_params(self):
+        """The Gaussians' attributes, shared ones looked up."""
+        if not self.tables:
+            return self.params
+        return {**self.params, **{k: table_lookup(t, self.codes[k]) for k, t in self.tables.items()}}
+
+    def _step_tables(self, row_mask):
+        """Sparse Adam on the table rows that a Gaussian in `row_mask` (uint8, one per Gaussian) names."""
+        for k, t in self.tables.items():
+            named = torch.where(row_mask.bool(), self.codes[k], -1).long()
+            mask = torch.empty(t.shape[0], dtype=torch.uint8, device=self.device)
+            _lib.check(_lib.lib().cvhrf_rows_to_mask(
+                ctypes.c_void_p(named.data_ptr()), named.numel(), ctypes.c_void_p(mask.data_ptr()), mask.numel(),
+                ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)), "cvhrf_rows_to_mask")
+            self.table_opts[k].step(row_mask=mask)
 
     def densify(self, grad_threshold=0.000005, decrease_amount=0.001, **kw):
         """The densification block of train.py:327-337, after an optimizer step: density
@@ -105,6 +157,8 @@ class HoloTrainer:
         regularisation, and a new optimizer whose per-parameter state is carried over only
         where the shape did not change (utils/optimizer.py:67-101).  A captured graph is
         dropped (the Gaussian count changed); call capture() again.  Returns the counts."""
+        if self.tables:
+            raise ValueError("densify works on Gaussians that own their attributes, not on shared_rows")
         old_params, old_opt = self.params, self.opt
         self.params, counts = density_control(old_params, grad_threshold=grad_threshold, **kw)
         counts["affected"] = opacity_regularization(self.params, decrease_amount)
@@ -122,7 +176,7 @@ class HoloTrainer:
     owned_mask = 0xFFFFFFFF
 
     def _render_inputs(self):
-        kw, idxs = SC.render_inputs_fused(self.params, self.camera, self.owned_mask)
+        kw, idxs = SC.render_inputs_fused(self.scene_params(), self.camera, self.owned_mask)
         if self.planes is not None:
             kw["plane_probs"] = kw["plane_probs"].index_select(1, self._plane_idx)
         return kw, idxs
@@ -148,14 +202,17 @@ class HoloTrainer:
         return loss, idxs[visible]
 
     def step(self, target=None):
-        for p in self.params.values():
-            p.grad = None
+        self._zero_grad()
         loss, visible = self.forward(target)
         loss.backward()
         if self.optimizer == "adan":
             self.opt.step()
         else:
             self.opt.step(visible)
+            if self.tables:
+                row_mask = torch.zeros(self.params["means"].shape[0], dtype=torch.uint8, device=self.device)
+                row_mask[visible] = 1
+                self._step_tables(row_mask)
         return loss.detach()
 
     # ---- CUDA-graph mode ------------------------------------------------------------
@@ -171,13 +228,13 @@ class HoloTrainer:
         return loss, row_mask
 
     def _step_capacity(self, exchange=None):
-        for p in self.params.values():
-            p.grad = None
+        self._zero_grad()
         loss, row_mask = self._forward_capacity(self._static_target)
         loss.backward()
         if exchange is not None:
             row_mask = exchange(self, row_mask)
         self.opt.step(row_mask=row_mask)
+        self._step_tables(row_mask)
         return loss.detach()
 
     def capture(self, headroom=1.5, exchange=None, warmup=2, eager_step=None):
@@ -186,6 +243,8 @@ class HoloTrainer:
         of an eager iteration.  `exchange(trainer, row_mask) -> row_mask` is called between
         backward and optimizer (the data-parallel gradient exchange); `eager_step` replaces
         the first (eager) iteration, e.g. with its data-parallel form."""
+        if self.tables and (exchange is not None or eager_step is not None):
+            raise ValueError("shared_rows trains on one GPU")
         (eager_step or self.step)()
         self.pairs_capacity = int(RZ.last_num_pairs * headroom) + 4096
         self._static_target = self.target.clone()

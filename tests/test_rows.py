@@ -411,6 +411,72 @@ def test_round_trip_through_groups(cuda):
     assert torch.equal(R.groups_to_rows(R.rows_to_groups(x, g), g), 3 * x)
 
 
+SHARED = {"colours": 64, "pre_act_phase": 300, "pre_act_scales": 1}
+
+
+def shared_trainer(cuda, **kw):
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer
+    return HoloTrainer(N=5000, W=128, H=96, K=3, device=cuda, seed=5, shared_rows=dict(SHARED), **kw)
+
+
+@gpu
+def test_trainer_with_shared_rows(cuda):
+    """The tables' gradients are the per-Gaussian ones summed; the step leaves unnamed rows alone."""
+    tr = shared_trainer(cuda)
+    tr.codes["colours"] = tr.codes["colours"] % 60            # rows 60 to 63 are named by nobody
+    own = {k: v.detach().clone().requires_grad_(True) for k, v in tr.scene_params().items()}
+    for k, v in own.items():
+        assert torch.equal(v, tr.tables[k][tr.codes[k]] if k in SHARED else tr.params[k])
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer
+    plain = HoloTrainer(N=5000, W=128, H=96, K=3, device=cuda, seed=5)
+    plain.params = own
+    loss, _ = plain.forward()
+    loss.backward()
+    before = {k: t.detach().clone() for k, t in tr.tables.items()}
+    assert torch.equal(tr.step(), loss.detach())
+    for k, t in tr.tables.items():
+        total, size, count = gradient_64(own[k].grad, tr.codes[k], t.shape[0], 1.0)
+        close(t.grad, total, (count[:, None] + 1) * U * size)
+    assert torch.equal(tr.tables["colours"][60:], before["colours"][60:])
+    moved = (tr.tables["colours"] != before["colours"]).any(1)
+    assert moved[:60].any() and all((t.grad is not None) for _, t in tr._leaves())
+
+
+@gpu
+def test_trainer_with_shared_rows_captured(cuda):
+    a, b = shared_trainer(cuda), shared_trainer(cuda)
+    b.capture(warmup=2)                                       # three steps
+    losses = [float(a.step()) for _ in range(6)]
+    assert losses[3:] == [float(b.replay()) for _ in range(3)]
+    assert not b.graph_overflowed()
+    for (k, x), (_, y) in zip(a._leaves(), b._leaves()):
+        assert torch.equal(x, y), k
+
+
+@gpu
+def test_trainer_with_shared_rows_and_adan(cuda):
+    tr = shared_trainer(cuda, optimizer="adan")
+    before = tr.tables["pre_act_phase"].detach().clone()
+    tr.step()
+    assert not torch.equal(tr.tables["pre_act_phase"].detach(), before)
+
+
+def test_trainer_refusals_of_shared_rows():
+    from complex_valued_holographic_radiance_fields_b200.distributed import dp_step
+    from complex_valued_holographic_radiance_fields_b200.scene import PinholeCamera
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer, MultiViewTrainer
+    small = dict(N=20, W=16, H=16, K=2, device="cpu")
+    for bad in ({"means": 4}, {"pre_act_opacities": 4}, {"colour": 4}, {"colours": 0}, {"colours": 21}):
+        with pytest.raises(ValueError):
+            HoloTrainer(shared_rows=bad, **small)
+    with pytest.raises(ValueError, match="one GPU"):
+        MultiViewTrainer(cameras=[PinholeCamera(16, 16)], shared_rows={"colours": 4}, **small)
+    tr = HoloTrainer(shared_rows={"colours": 4}, **small)
+    for call in (tr.densify, lambda: tr.capture(exchange=lambda t, m: m), lambda: dp_step(tr)):
+        with pytest.raises(ValueError, match="shared_rows"):
+            call()
+
+
 # ---- streams, graphs, devices ------------------------------------------------------------
 @gpu
 def test_captured_and_replayed(cuda):
