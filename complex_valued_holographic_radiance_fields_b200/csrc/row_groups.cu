@@ -1,7 +1,7 @@
 // Integer indices sorted stably by value (see row_groups.cuh), and cvhrf_group_rows.
 //
-// LSD radix sort, digits of at most 9 bits (two passes up to 262144 values), the bits shared evenly between the passes.  A pass
-// is two launches: chunk_count_kernel counts the digits of each contiguous chunk of keys into
+// LSD radix sort, digits of at most 9 bits (two passes up to 262144 values), the bits shared
+// evenly between the passes.  A pass is two launches: chunk_count_kernel counts the digits of each contiguous chunk of keys into
 // a chunk x digit matrix, and chunk_scatter_kernel reads that matrix, adds up what lies before
 // its own chunk, and writes each key to its place.  No block waits for another one and nothing
 // has to be cleared beforehand.  (Counting a key's next digit where it is scattered saves a
@@ -15,25 +15,15 @@
 // (512 threads: 18 us a pass for 1M keys, against 15).  Up to 8192 keys in all, one block
 // does every pass in shared memory (small_sort_kernel, one launch).
 #include "row_groups.cuh"
+#include "row_sort.cuh"
 #include "row_types.cuh"
 
 namespace cvhrf {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kItems = 8, kTile = kThreads * kItems;
-constexpr int kMaxChunks = 148;   // one block per SM
-constexpr int kMaxBits = 9, kMaxRadix = 1 << kMaxBits;
-constexpr uint32_t kNone = 0xffffffffu;
-static_assert(kThreads == 2 * kMaxRadix, "two threads per digit");
+using namespace row_sort;
 
-struct Source {
-  const void* index;         // the caller's indices in the first pass
-  int bytes;                 // 4 or 8; 0: sorted keys and entries of the pass before
-  const uint32_t* keys;
-  const uint32_t* entries;
-  uint32_t rows;             // values outside [0, rows) are left out, or become `rows`
-  int keep;
-};
+constexpr int kMaxChunks = 148;   // one block per SM
 
 struct Target {
   uint32_t* keys;      // null: not wanted
@@ -56,14 +46,6 @@ __device__ __forceinline__ void clear_touched(uint8_t* touched, uint32_t rows) {
     if (threadIdx.x < head) touched[threadIdx.x] = 0;
     for (uint32_t i = head + (words << 4) + threadIdx.x; i < rows; i += kThreads) touched[i] = 0;
   }
-}
-
-// Key of item i, kNone if it is left out (keys are below 2^31).
-__device__ __forceinline__ uint32_t source_key(const Source& s, uint32_t i) {
-  if (s.bytes == 0) return s.keys[i];
-  const unsigned long long v = s.bytes == 4 ? (unsigned long long)(long long)((const int*)s.index)[i]
-                                            : ((const unsigned long long*)s.index)[i];
-  return v < s.rows ? (uint32_t)v : (s.keep ? s.rows : kNone);
 }
 
 // counts[chunk][digit] over the keys of each chunk.
@@ -103,119 +85,6 @@ __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_
     for (int w = 0; w < kCopies; ++w) c += h[w][d];
     counts[(size_t)blockIdx.x * radix + d] = c;
   }
-}
-
-struct Shared {
-  uint32_t cnt[kWarps * kMaxRadix];    // warp x digit
-  uint32_t key[kTile], entry[kTile];   // the tile in digit order
-  uint32_t base[kMaxRadix];            // place of the chunk's next key with this digit
-  uint32_t start[kMaxRadix];           // start of the digit inside the tile
-  uint32_t delta[kMaxRadix];           // base - start
-  uint32_t lower[kMaxRadix], upper[kMaxRadix];   // keys of the digit in either half of the warps
-  uint32_t sh[kMaxRadix / 32 + 1];
-};
-
-// Exclusive scan over the values of a block's first kMaxRadix threads; all threads call it.
-__device__ __forceinline__ uint32_t scan_radix(uint32_t v, uint32_t* sh /* kMaxRadix / 32 + 1 */, uint32_t& total) {
-  constexpr int kParts = kMaxRadix / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t inc = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += t;
-  }
-  if (warp < kParts && lane == 31) sh[warp] = inc;
-  __syncthreads();
-  if (warp == 0) {
-    uint32_t t = lane < kParts ? sh[lane] : 0u, run = t;
-#pragma unroll
-    for (int o = 1; o < kParts; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += u;
-    }
-    if (lane < kParts) sh[lane] = run - t;
-    if (lane == kParts - 1) sh[kParts] = run;
-  }
-  __syncthreads();
-  const uint32_t r = (warp < kParts ? sh[warp] : 0u) + inc - v;
-  total = sh[kParts];
-  __syncthreads();
-  return r;
-}
-
-// Sorts one tile by a digit into sh.key / sh.entry.  Warp w holds the `rounds` x 32 keys from
-// w * rounds * 32 on (key[r] of lane l is the r * 32 + l-th of them; kNone: no key).  place[r]
-// becomes the key's place inside its digit's run.  Returns how many of digit threadIdx.x
-// there are; kept = keys in the tile.
-__device__ __forceinline__ uint32_t sort_tile(Shared& sh, const uint32_t (&key)[kItems], const uint32_t (&entry)[kItems],
-                                              uint32_t (&place)[kItems], int rounds, int shift, int width,
-                                              uint32_t& kept) {
-  const int radix = 1 << width;
-  const uint32_t mask = radix - 1;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < kWarps * radix / 4; i += kThreads) reinterpret_cast<uint4*>(sh.cnt)[i] = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  const unsigned lt = (1u << lane) - 1u;
-  uint32_t* mine = sh.cnt + warp * radix;
-  // the lanes with the same digit, bit by bit (__match_any_sync takes a step per distinct digit)
-  unsigned peers[kItems];
-#pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    if (r >= rounds) break;
-    const uint32_t d = key[r] >> shift;
-    peers[r] = __ballot_sync(0xffffffffu, key[r] != kNone);
-#pragma unroll
-    for (int b = 0; b < kMaxBits; ++b) {
-      if (b >= width) break;
-      const unsigned ones = __ballot_sync(0xffffffffu, d & (1u << b));
-      peers[r] &= d & (1u << b) ? ones : ~ones;
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    if (r >= rounds) break;
-    const bool in = key[r] != kNone;
-    const uint32_t d = (key[r] >> shift) & mask;
-    uint32_t before = 0;
-    if (in) before = mine[d];
-    place[r] = before + __popc(peers[r] & lt);
-    __syncwarp();
-    if (in && (peers[r] & lt) == 0) mine[d] = before + __popc(peers[r]);
-    __syncwarp();
-  }
-  __syncthreads();
-  // per digit: where each warp's keys begin, the upper half of the warps by the upper threads
-  constexpr int kHalf = kWarps / 2;
-  const int d0 = tid & (kMaxRadix - 1), w0 = tid / kMaxRadix * kHalf;
-  uint32_t run = 0;
-  if (d0 < radix) {
-#pragma unroll
-    for (int w = 0; w < kHalf; ++w) {
-      const uint32_t c = sh.cnt[(w0 + w) * radix + d0];
-      sh.cnt[(w0 + w) * radix + d0] = run;
-      run += c;
-    }
-  }
-  if (tid < kMaxRadix) sh.lower[tid] = run;
-  else sh.upper[tid - kMaxRadix] = run;
-  __syncthreads();
-  if (tid < kMaxRadix) run += sh.upper[tid];
-  const uint32_t start = scan_radix(tid < kMaxRadix ? run : 0u, sh.sh, kept);
-  if (tid < kMaxRadix) sh.start[tid] = start;
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    if (r >= rounds) break;
-    if (key[r] == kNone) continue;
-    const uint32_t d = (key[r] >> shift) & mask;
-    place[r] += mine[d] + (warp >= kHalf ? sh.lower[d] : 0u);
-    const uint32_t at = sh.start[d] + place[r];
-    sh.key[at] = key[r];
-    sh.entry[at] = entry[r];
-  }
-  __syncthreads();
-  return run;
 }
 
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
@@ -320,29 +189,10 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
                                                               bool clear) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   let_next_start();
   if (clear) clear_touched(out.touched, s.rows);
-  uint32_t key[kItems], entry[kItems], place[kItems];
-  uint32_t kept = n;
-  int done = 0;
-  for (int p = 0; p < passes; ++p) {
-    const int width = (bits - done + (passes - p) - 1) / (passes - p);
-    const int rounds = (int)((kept + kThreads - 1) / kThreads);
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      key[r] = kNone;
-      if (r >= rounds) continue;
-      const uint32_t i = warp * (32 * rounds) + r * 32 + lane;
-      if (i < kept) {
-        key[r] = p == 0 ? source_key(s, i) : sh.key[i];
-        entry[r] = p == 0 ? i : sh.entry[i];
-      }
-    }
-    __syncthreads();
-    sort_tile(sh, key, entry, place, rounds, done, width, kept);
-    done += width;
-  }
+  const uint32_t kept = sort_run(sh, s, 0, n, bits, passes);
   for (uint32_t i = tid; i < kept; i += kThreads) {
     const uint32_t k = sh.key[i], e = sh.entry[i];
     if (out.keys) out.keys[i] = k;
@@ -387,12 +237,6 @@ __global__ void __launch_bounds__(256) places_kernel(const uint32_t* __restrict_
   }
 }
 
-inline int bits_for(unsigned long long values) {   // bits that hold 0 .. values - 1
-  int b = 1;
-  while ((1ull << b) < values) ++b;
-  return b;
-}
-
 struct Chunks {
   int count;
   uint32_t size;
@@ -406,8 +250,6 @@ inline Chunks chunks_for(long long n) {
   const long long size = ((n + c - 1) / c + 31) / 32 * 32;
   return {(int)((n + size - 1) / (size > 0 ? size : 1)), (uint32_t)size};
 }
-
-inline int passes_for(int bits) { return (bits + kMaxBits - 1) / kMaxBits; }
 
 // All passes over the low `bits` bits.  The last one writes `out`; the ones before it go to and
 // fro between the two buffers of keys and entries at `buffers` (of `len` words each).

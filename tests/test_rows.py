@@ -122,7 +122,9 @@ def skewed(kind, n, rows):
 @pytest.mark.parametrize("kind", ["one_row", "first_and_last", "none", "sorted", "reversed", "half_in_one", "popular"])
 @pytest.mark.parametrize("n,rows,width,dtype", [(100003, 4096, 3, torch.float32), (70001, 257, 59, torch.float32),
                                                 (20000, 30000, 264, torch.bfloat16), (40000, 2, 130, torch.float16),
-                                                (3001, 1, 8, torch.float32), (300000, 65536, 4, torch.float32)])
+                                                (3001, 1, 8, torch.float32), (300000, 65536, 4, torch.float32),
+                                                (1500001, 100, 5, torch.float32), (100003, 511, 32, torch.bfloat16),
+                                                (90001, 16384, 1, torch.float16), (90001, 512, 33, torch.float32)])
 def test_gradient_of_skewed_rows(cuda, kind, n, rows, width, dtype):
     grad = (normal((n, width), torch.float32, n) * 0.05).to(dtype)
     index = skewed(kind, n, rows)
