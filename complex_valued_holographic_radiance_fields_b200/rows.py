@@ -118,9 +118,10 @@ def _gradient(grad, index, num_rows, scale, with_mask):
     out = grad.new_empty((num_rows, width))
     mask = index.new_empty(num_rows, dtype=torch.uint8) if with_mask else None
     need = _gradient_workspace(n, num_rows, width)
-    ws = index.new_empty(need // nbytes)
+    ws = index.new_empty(need // nbytes) if need else None
     _call("cvhrf_table_gradient", "table_gradient", device, _lib.GRADIENT_ARGS.pack(
-        grad.data_ptr(), index.data_ptr(), out.data_ptr(), mask.data_ptr() if with_mask else 0, ws.data_ptr(), need,
+        grad.data_ptr(), index.data_ptr(), out.data_ptr(), mask.data_ptr() if with_mask else 0,
+        ws.data_ptr() if need else 0, need,
         stride, n, num_rows, width, code, nbytes, scale))
     return out, mask
 
@@ -190,9 +191,10 @@ def group_rows(index, num_groups):
         raise ValueError(f"num_groups must be in [1, 2^31 - 1), got {num_groups}")
     device = index.device
     index, nbytes, n = _index(index, device)
-    order = index.new_empty(n, dtype=torch.int32)
-    slots = index.new_empty(shape, dtype=torch.int32)
-    offsets = index.new_empty(num_groups + 1, dtype=torch.int32)
+    if nbytes == 4:
+        order, slots, offsets = index.new_empty(n), index.new_empty(shape), index.new_empty(num_groups + 1)
+    else:
+        order, slots, offsets = (index.new_empty(s, dtype=torch.int32) for s in (n, shape, num_groups + 1))
     need = _group_workspace(n, num_groups)
     ws = index.new_empty(need // nbytes) if need else None
     _call("cvhrf_group_rows", "group_rows", device, _lib.GROUP_ARGS.pack(

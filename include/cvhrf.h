@@ -571,7 +571,7 @@ int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream);
  * (zeros where there is none), every row written; row_mask[v] (may be null) = 1 where
  * there is one, the mask cvhrf_sparse_adam_masked takes.  The order of the sums is fixed
  * (the entries' order, joined between blocks in a fixed order): results repeat bit for
- * bit.  An entry whose index is outside [0, rows) is left out and its row not read.
+ * bit.  The workspace query returns 0 where none is needed.  An entry whose index is outside [0, rows) is left out and its row not read.
  */
 typedef struct {
   const void* grad;

@@ -91,7 +91,7 @@ def test_lookup(cuda, dtype, width, n, rows):
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 8, 12, 20, 59, 64, 130, 256, 333, 1000, 2056])
-@pytest.mark.parametrize("n,rows", [(1, 1), (1, 3000), (5, 2), (513, 1), (2049, 40), (300, 20011), (9000, 700)])
+@pytest.mark.parametrize("n,rows", [(1, 1), (1, 3000), (5, 2), (513, 1), (2048, 40), (2049, 40), (300, 20011), (3000, 20011), (9000, 700)])
 def test_gradient(cuda, dtype, width, n, rows):
     grad = normal((n, width), dtype, width + n)
     for itype in (torch.int32, torch.int64):
@@ -585,10 +585,12 @@ def test_c_abi_refusals_need_no_gpu():
     assert lookup(n=2 ** 30) == 4
     assert lookup(n=0) == 0
 
-    need = L.cvhrf_table_gradient_workspace_bytes(1000, 10, 8)
-    assert need > 0 and L.cvhrf_table_gradient_workspace_bytes(-1, 10, 8) == 0
+    need = L.cvhrf_table_gradient_workspace_bytes(10000, 10, 8)
+    assert need > 0 and L.cvhrf_table_gradient_workspace_bytes(100000, 10 ** 5, 80) > 100000
+    assert L.cvhrf_table_gradient_workspace_bytes(-1, 10, 8) == 0
+    assert L.cvhrf_table_gradient_workspace_bytes(100, 10, 8) == 0     # a few entries need none
 
-    def gradient(grad=p, index=p, out=p, ws=p, need=need, stride=8, n=1000, rows=10, width=8, dtype=0, nbytes=8):
+    def gradient(grad=p, index=p, out=p, ws=p, need=need, stride=8, n=10000, rows=10, width=8, dtype=0, nbytes=8):
         return L.cvhrf_table_gradient(_lib.GRADIENT_ARGS.pack(grad, index, out, 0, ws, need, stride, n, rows, width,
                                                               dtype, nbytes, 1.0), None)
 
