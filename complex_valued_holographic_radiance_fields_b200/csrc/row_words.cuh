@@ -1,4 +1,5 @@
-// Rows that do not begin on 16 bytes (an odd width, a slice), moved in 4-byte words.
+// Rows that do not begin on 16 bytes, moved in 4-byte words where they do not go through a tile
+// (row_tiles.cuh): rows of more than 4 KB, and outputs that do not begin on 16 bytes.
 //
 // A word is one float32 or two 16-bit elements, aligned on the row that is written; with 16-bit
 // elements the row that is read may begin on the other half of a word, and then two of its
@@ -7,8 +8,6 @@
 // stores are whole lines up to their ends.  What is done per row (its place, its address, its
 // edges) is as much work as the words of a short row, so a warp takes up to 32 entries, each
 // lane works out one of them, and the owners of rows get them by shuffle.
-// (Packs of 16 bytes shifted out of two aligned ones took twice the instructions for rows of
-// 333 halves, and so twice the time.)
 #pragma once
 #include "row_tiles.cuh"
 

@@ -19,7 +19,8 @@ An index or group outside its range (-1, say) leaves the entry out: it looks up 
 nothing to a gradient or a sum, and whatever its weight or gradient holds is not read.
 Rows are float32, bfloat16 or float16, contiguous within a row (a slice of a wider tensor
 or a row expanded over a batch is used as it is); sums are float32 in a fixed order, so
-results repeat bit for bit, and are rounded once.  Nothing is read back to the host: every
+results repeat bit for bit, and are rounded once; gradients are not differentiable again.
+Nothing is read back to the host: every
 call can be captured in a CUDA graph.  Every step runs in libcvhrf (cvhrf_table_lookup,
 cvhrf_table_gradient, cvhrf_group_rows, cvhrf_rows_to_groups, cvhrf_groups_to_rows); the
 reference, whose Gaussians own all their attributes, has no counterpart.
@@ -27,6 +28,7 @@ reference, whose Gaussians own all their attributes, has no counterpart.
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, profiling
 
@@ -34,6 +36,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
 _MAX_ENTRIES = 2 ** 30 - 1
 _MAX_WIDTH = 2 ** 20
+_MAX_SCALE = torch.finfo(torch.float32).max
 
 
 def _call(name, what, device, args):
@@ -93,7 +96,10 @@ def _index(index, device):
 def _scale(scale):
     if isinstance(scale, torch.Tensor):
         raise TypeError("scale must be a number, not a tensor")
-    return float(scale)
+    scale = float(scale)
+    if not -_MAX_SCALE <= scale <= _MAX_SCALE:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
+    return scale
 
 
 # ---- shared rows ----------------------------------------------------------------------
@@ -134,6 +140,7 @@ class TableLookup(torch.autograd.Function):
         return _lookup(table, index, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         index, = ctx.saved_tensors
         return _gradient(grad, index, ctx.num_rows, ctx.scale, False)[0], None, None
@@ -230,6 +237,7 @@ class RowsToGroups(torch.autograd.Function):
         return _to_groups(x, groups)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         return _to_rows(grad, ctx.groups, None), None
 
@@ -242,6 +250,7 @@ class GroupsToRows(torch.autograd.Function):
         return _to_rows(y, groups, weights)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         y, weights = ctx.saved_tensors
         groups = ctx.groups

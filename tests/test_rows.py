@@ -75,7 +75,7 @@ def check_gradient(got, mask, grad, index, rows, scale):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 20, 59, 64, 129, 333, 1024, 4104])
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 17, 20, 59, 64, 129, 333, 515, 1024, 2047, 2049, 4099, 4104])
 @pytest.mark.parametrize("n,rows", [(1, 1), (1, 5000), (7, 3), (2049, 64)])
 def test_lookup(cuda, dtype, width, n, rows):
     table = normal((rows, width), dtype, width)
@@ -90,7 +90,7 @@ def test_lookup(cuda, dtype, width, n, rows):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 8, 12, 20, 59, 64, 130, 256, 333, 1000, 2056])
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 8, 12, 20, 59, 64, 130, 256, 333, 1000, 2049, 2056])
 @pytest.mark.parametrize("n,rows", [(1, 1), (1, 3000), (5, 2), (513, 1), (2048, 40), (2049, 40), (300, 20011), (3000, 20011), (9000, 700)])
 def test_gradient(cuda, dtype, width, n, rows):
     grad = normal((n, width), dtype, width + n)
@@ -270,7 +270,7 @@ def test_groups_of_one_kind(cuda):
 @pytest.mark.parametrize("dtype,wtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
                                          (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
                                          (torch.float16, None)])
-@pytest.mark.parametrize("width", [1, 3, 8, 20, 59, 64, 333, 1024, 2056])
+@pytest.mark.parametrize("width", [1, 3, 8, 17, 20, 59, 64, 333, 530, 1024, 2051, 2056])
 @pytest.mark.parametrize("n,k,groups", [(1, 1, 1), (3, 8, 8), (301, 2, 7), (1000, 3, 300)])
 def test_moves_and_their_gradients(cuda, dtype, wtype, width, n, k, groups):
     index = integers(n * k, groups + 1, n + width, -1).reshape(n, k)
@@ -354,6 +354,69 @@ def test_strided_moves(cuda):
                 (g.slots >= 0)[:, :, None], y.double()[g.slots.long().clamp(min=0)], 0.0)
             for dw in (one[1], two[1]):
                 close(dw, terms.sum(2), y.shape[1] * U * terms.abs().sum(2))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,width", [(torch.float32, 5), (torch.float32, 40), (torch.float32, 64),
+                                         (torch.bfloat16, 3), (torch.bfloat16, 24), (torch.float16, 40),
+                                         (torch.float16, 333), (torch.float16, 2051)])
+@pytest.mark.parametrize("ahead", [1, 3, 8])
+def test_outputs_that_begin_anywhere(cuda, dtype, width, ahead):
+    """Through the C entry points, outputs `ahead` elements behind a boundary: the same values,
+    and nothing before or behind them is written."""
+    L, code = _lib.lib(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    st = torch.cuda.current_stream().cuda_stream
+    n, k, rows = 300, 2, 37
+    guard = 7.0
+
+    def check(call, *expected):
+        bufs = [torch.full((e.numel() + ahead + 64,), guard, dtype=dtype, device="cuda") for e in expected]
+        assert call(*[b[ahead:].data_ptr() for b in bufs]) == 0
+        for b, e in zip(bufs, expected):
+            assert torch.equal(b[ahead:ahead + e.numel()].view(e.shape), e)
+            assert (b[:ahead] == guard).all() and (b[ahead + e.numel():] == guard).all()
+
+    table, index = normal((rows, width), dtype, 0), integers(n * k, rows + 1, 1, -1)
+    p = index.data_ptr()
+    check(lambda o: L.cvhrf_table_lookup(_lib.LOOKUP_ARGS.pack(table.data_ptr(), p, o, rows, width, n * k, width, code,
+                                                               8, 0.5), st), R.table_lookup(table, index, 0.5))
+    grad = torch.randint(-3, 4, (n * k, width), device="cuda").to(dtype)         # exact in any order
+    for entries, table_rows in ((n * k, rows), (n * k, 2000)):
+        check(lambda o: L.cvhrf_table_gradient(_lib.GRADIENT_ARGS.pack(
+            grad.data_ptr(), p, o, 0, 0, 0, width, entries, table_rows, width, code, 8, 0.5), st),
+            R.table_gradient(grad, index, table_rows, 0.5)[0])
+    many, more = torch.cat([index] * 8), torch.cat([grad] * 8)
+    need = L.cvhrf_table_gradient_workspace_bytes(many.numel(), 5000, width)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    check(lambda o: L.cvhrf_table_gradient(_lib.GRADIENT_ARGS.pack(
+        more.data_ptr(), many.data_ptr(), o, 0, ws.data_ptr(), need, width, many.numel(), 5000, width, code, 8, 1.0),
+        st), R.table_gradient(more, many, 5000)[0])
+
+    g = R.group_rows(index.reshape(n, k), rows)
+    x, y, w = normal((n, width), dtype, 2), grad, torch.randint(0, 3, (n, k), device="cuda").float()
+    ptrs = (g.order.data_ptr(), g.slots.data_ptr(), g._used())
+    check(lambda o: L.cvhrf_rows_to_groups(_lib.MOVES_ARGS.pack(x.data_ptr(), o, *ptrs, 0, n, width, k, width, code, 0),
+                                           st), R.rows_to_groups(x, g))
+    check(lambda o: L.cvhrf_groups_to_rows(_lib.MOVES_ARGS.pack(y.data_ptr(), o, *ptrs, w.data_ptr(), n, width, k, width,
+                                                                code, 0), st), R.groups_to_rows(y, g, w))
+    yl, wl = y.clone().requires_grad_(), w.clone().requires_grad_()
+    up = torch.randint(-2, 3, (n, width), device="cuda").to(dtype)
+    dy, dw = torch.autograd.grad(R.groups_to_rows(yl, g, wl), (yl, wl), up)
+    got_w = torch.empty_like(w)
+    check(lambda o: L.cvhrf_groups_to_rows_backward(_lib.MOVES_BACKWARD_ARGS.pack(
+        up.data_ptr(), y.data_ptr(), *ptrs, w.data_ptr(), o, got_w.data_ptr(), n, width, width, k, width, code, 0), st),
+        dy)
+    assert torch.equal(got_w, dw)
+
+
+@gpu
+def test_no_second_derivative(cuda):
+    g = R.group_rows(integers(12, 4, 0).reshape(6, 2), 4)
+    t, x = normal((5, 3), torch.float32, 1).requires_grad_(), normal((6, 3), torch.float32, 2).requires_grad_()
+    for out, leaf in ((R.table_lookup(t, integers(7, 5, 3)), t), (R.rows_to_groups(x, g), x)):
+        first, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
 
 
 # ---- gradients against differences -------------------------------------------------------
@@ -561,6 +624,9 @@ def test_refusals_need_no_gpu():
         R.table_lookup(cpu.double(), index)
     with pytest.raises(TypeError, match="number"):
         R.table_lookup(cpu, index, torch.ones(()))
+    for bad in (float("nan"), float("inf"), -1e39):
+        with pytest.raises(ValueError, match="finite"):
+            R.table_lookup(cpu, index, bad)
     with pytest.raises(ValueError, match="shape"):
         R.table_gradient(torch.zeros(3, 4), index, 3)
     with pytest.raises(ValueError, match="num_rows"):
