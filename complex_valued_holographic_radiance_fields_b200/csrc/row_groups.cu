@@ -1,11 +1,11 @@
 // Integer indices sorted stably by value (see row_groups.cuh), and cvhrf_group_rows.
 //
 // LSD radix sort, digits of at most 9 bits (two passes up to 262144 values), the bits shared
-// evenly between the passes.  A pass is two launches: chunk_count_kernel counts the digits of each contiguous chunk of keys into
-// a chunk x digit matrix, and chunk_scatter_kernel reads that matrix, adds up what lies before
-// its own chunk, and writes each key to its place.  No block waits for another one and nothing
-// has to be cleared beforehand.  (Counting a key's next digit where it is scattered saves a
-// launch, but its atomics cost 8 us for 1M keys, and the launch 3.)
+// evenly between the passes.  A pass is two launches: chunk_count_kernel counts the digits of
+// each contiguous chunk of keys into a chunk x digit matrix, and chunk_scatter_kernel reads that
+// matrix, adds up what lies before its own chunk, and writes each key to its place.  No block
+// waits for another one and nothing has to be cleared beforehand.  (Counting a key's next digit
+// where it is scattered saves a launch, but its atomics cost 8 us for 1M keys, and the launch 3.)
 // (A look-back between tiles, as in scan_sort.cu, needs a cleared status array, one more
 // launch for the histogram, and a walk over the earlier tiles in L2 latency.)
 // The first pass reads the caller's indices as they are (4 or 8 bytes).

@@ -5,10 +5,13 @@
 //   to rows    out[n] = sum_j w[n, j] y[slot[n, j]]                      (fp32, in the order of j)
 //   gradient   dy[slot[n, j]] = w[n, j] dout[n],  dw[n, j] = <dout[n], y[slot[n, j]]>
 //
-// (The gradient of "to groups" is "to rows" without weights.)  All three go by rows n: a row
-// is owned by a power of two of lanes, up to a warp, that hold its columns, so a row of x or
-// dout is read once however many groups it goes to, and no two owners write to one place.
-// Bound by memory: each touches N + N k rows once.
+// (The gradient of "to groups" is "to rows" without weights.)  Aligned rows go by n: a row is
+// owned by up to a warp of lanes that hold its columns, so a row of x or dout is read once however
+// many groups it goes to, and no two owners write to one place.  Other rows go by the rows that
+// are written, in tiles (row_tiles.cuh).
+// Bound by memory: each touches N + N k rows once.  16384 rows of 2048 bf16 to 4 of 64 groups:
+// 51 us there (6.6 TB/s), 60 back (5.6), 101 for the gradient (5.3, y read for dw).  100003 odd
+// rows of 333 f16 to 2 of 7: 45, 57 and 87 us, where 2-byte loads are what is waited for.
 #include <type_traits>
 #include "row_groups.cuh"
 #include "row_tiles.cuh"

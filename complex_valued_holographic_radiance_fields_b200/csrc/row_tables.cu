@@ -478,9 +478,18 @@ __global__ void __launch_bounds__(kThreads) table_join_kernel(Joins joins, int w
 
 // ---- gradient of few entries -----------------------------------------------------------------
 // A small batch is bound by its launches: every block sorts all entries for itself, then takes a
-// share of the table's rows, adds up those that occur and clears the others.  One launch, nothing
-// in global memory between (512 entries on 4096 rows of 64 floats: 9.7 us, 11.7 in three launches).
+// share of the table's rows and a tile of their columns, adds up the rows that occur and clears
+// some of the others.  One launch, nothing in global memory between (512 entries on 4096 rows of
+// 64 floats: 9.7 us, 11.7 in three launches).  Shares x tiles fill the SMs once: a second wave
+// would sort again (2048 entries on 5000 rows of 1024 floats: 16 us; 80 in 8 waves, 21 in three
+// launches).  Tables of more elements, mostly to be cleared, are left to more blocks (50000 rows of
+// 2047 floats: 130 us against 95; of 1023: 61 against 58).
 constexpr int kFewEntries = 2 * row_sort::kThreads;
+constexpr int kFewBlocks = 148, kFewWidth = 32 * kFewBlocks;   // a tile has 32 columns at least
+constexpr long long kFewElements = 1ll << 26;
+inline bool few(long long entries, long long rows, int width) {
+  return entries <= kFewEntries && width <= kFewWidth && rows * width <= kFewElements;
+}
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(row_sort::kThreads) few_entries_kernel(row_sort::Source index, uint32_t n, int bits,
@@ -508,10 +517,12 @@ __global__ void __launch_bounds__(row_sort::kThreads) few_entries_kernel(row_sor
   const uint32_t r0 = (uint32_t)min((unsigned long long)blockIdx.x * rows_each, (unsigned long long)index.rows);
   const uint32_t r1 = (uint32_t)min((unsigned long long)r0 + rows_each, (unsigned long long)index.rows);
   const int begin = (int)first_of(r0), end = (int)first_of(r1);
-  // the rows that do not occur, whole, `step` at a time per warp (the warps share them evenly)
-  if (blockIdx.y == 0) {
-    const int warp = threadIdx.x >> 5, in_warp = threadIdx.x & 31, step = max(1, min(32, rows_each / kWarps));
-    for (uint32_t r = r0 + warp * step; r < r1; r += kWarps * step) {
+  // the rows that do not occur, whole, `step` at a time per warp (shared evenly between the warps
+  // of all tiles)
+  {
+    const int in_warp = threadIdx.x & 31, warps = kWarps * gridDim.y;
+    const int warp = blockIdx.y * kWarps + (threadIdx.x >> 5), step = max(1, min(32, rows_each / warps));
+    for (uint32_t r = r0 + warp * step; r < r1; r += warps * step) {
       const bool mine = in_warp < step && r + in_warp < r1;
       uint32_t at = 0;
       if (mine) at = first_of(r + in_warp);
@@ -606,16 +617,15 @@ int few_entries(const void* grad, long long stride, int width, const void* index
                 long long rows, float scale, void* out, uint8_t* mask, cudaStream_t st) {
   const row_sort::Source source{index, index_bytes, nullptr, nullptr, (uint32_t)rows, 0};
   const int bits = row_sort::bits_for((unsigned long long)rows);
-  // every SM once; a share has the rows of one look of a warp at least
-  const long long rows_each = std::max(32ll, (rows + 147) / 148);
-  const unsigned blocks = (unsigned)((rows + rows_each - 1) / rows_each);
   auto launch = [&](auto aligned) {
     constexpr bool kAlignedRows = decltype(aligned)::value;
     static std::atomic<unsigned long long> allowed{0};
     CVHRF_CUDA_TRY(allow_shared(few_entries_kernel<T, kAlignedRows>, sizeof(row_sort::Shared), allowed));
     const int packs = width / Columns<T, kAlignedRows, 1>::kVec, lanes = packs < 32 ? packs : 32;
+    const int tiles = (packs + lanes - 1) / lanes, shares = kFewBlocks / tiles;
+    const long long rows_each = std::max(32ll, (rows + shares - 1) / shares);
     few_entries_kernel<T, kAlignedRows>
-        <<<dim3(blocks, (packs + lanes - 1) / lanes), row_sort::kThreads, sizeof(row_sort::Shared), st>>>(
+        <<<dim3((unsigned)((rows + rows_each - 1) / rows_each), tiles), row_sort::kThreads, sizeof(row_sort::Shared), st>>>(
             source, (uint32_t)n, bits, (int)rows_each, lanes, width, (const T*)grad, stride, scale, (T*)out, mask);
     CVHRF_LAUNCH_CHECK();
     return CVHRF_OK;
@@ -884,7 +894,7 @@ extern "C" int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream) {
 extern "C" size_t cvhrf_table_gradient_workspace_bytes(long long entries, long long rows, int width) {
   if (entries < 0 || entries > kGroupMaxEntries || rows < 0 || rows > kMaxRows || width < 1 || width > kMaxWidth)
     return 0;
-  if (entries <= kFewEntries) return 0;
+  if (few(entries, rows, width)) return 0;
   if (small_table(rows, width))
     return align_up((size_t)small_blocks(entries) * ((size_t)rows * width * sizeof(float) + (size_t)rows), 256);
   return align_up(group_sort_words(entries) * sizeof(uint32_t), 256) + align_up((size_t)rows, 256) +
@@ -908,7 +918,7 @@ extern "C" int cvhrf_table_gradient(const cvhrf_gradient_args* args, void* strea
     if (row_mask) CVHRF_CUDA_TRY(cudaMemsetAsync(row_mask, 0, (size_t)rows, st));
     return CVHRF_OK;
   }
-  if (entries <= kFewEntries) {
+  if (few(entries, rows, width)) {
     if (dtype == CVHRF_F32)
       return few_entries<float>(grad, grad_stride, width, index, index_bytes, entries, rows, scale, grad_table,
                                 row_mask, st);

@@ -20,10 +20,11 @@ nothing to a gradient or a sum, and whatever its weight or gradient holds is not
 Rows are float32, bfloat16 or float16, contiguous within a row (a slice of a wider tensor
 or a row expanded over a batch is used as it is); sums are float32 in a fixed order, so
 results repeat bit for bit, and are rounded once; gradients are not differentiable again.
-Nothing is read back to the host: every
-call can be captured in a CUDA graph.  Every step runs in libcvhrf (cvhrf_table_lookup,
-cvhrf_table_gradient, cvhrf_group_rows, cvhrf_rows_to_groups, cvhrf_groups_to_rows); the
-reference, whose Gaussians own all their attributes, has no counterpart.
+Nothing is read back to the host: every call can be captured in a CUDA graph, a backward
+pass as torch captures any (no earlier autograd graph of the same leaves may be alive).
+Every step runs in libcvhrf (cvhrf_table_lookup, cvhrf_table_gradient, cvhrf_group_rows,
+cvhrf_rows_to_groups, cvhrf_groups_to_rows); the reference, whose Gaussians own all their
+attributes, has no counterpart.
 """
 import functools
 
@@ -173,7 +174,8 @@ def table_gradient(grad, index, num_rows, scale=1.0):
 class RowGroups:
     """Entries sorted by group (``group_rows``), all int32 on the device: ``order`` (M,) the
     entry at each place, ``slots`` (the index's shape) the place of each entry or -1,
-    ``offsets`` (num_groups + 1,) where each group begins and the last one ends."""
+    ``offsets`` (num_groups + 1,) where each group begins and the last one ends.  They are
+    read, not written: the moves take their places on trust."""
 
     __slots__ = ("order", "slots", "offsets", "num_groups", "num_rows", "choices")
 

@@ -101,6 +101,30 @@ def test_gradient(cuda, dtype, width, n, rows):
         check_gradient(got, mask, grad, index, rows, 0.75)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [257, 1023, 4736, 4737, 4744, 9001])
+@pytest.mark.parametrize("n,rows", [(1, 1), (1, 200), (7, 33), (2048, 3), (2048, 300), (600, 5000)])
+def test_gradient_of_few_wide_rows(cuda, dtype, width, n, rows):
+    if rows * width > 6_000_000:
+        width = width // 8 * 2 + 1
+    few_wide_rows(dtype, width, n, rows)
+
+
+@gpu
+@pytest.mark.parametrize("n,rows,width", [(5, 70001, 957), (5, 70001, 960), (2048, 2 ** 24, 4), (2048, 2 ** 24 + 1, 4)])
+def test_gradient_of_few_entries_in_large_tables(cuda, n, rows, width):
+    few_wide_rows(torch.bfloat16, width, n, rows)
+
+
+def few_wide_rows(dtype, width, n, rows):
+    grad = normal((n, width), dtype, width + n)
+    for kind in ("mixed", "one_row"):
+        index = integers(n, rows + 1, n + rows, -1) if kind == "mixed" else torch.full((n,), rows - 1, device="cuda")
+        got, mask = R.table_gradient(grad, index, rows, 0.75)
+        check_gradient(got, mask, grad, index, rows, 0.75)
+
+
 def skewed(kind, n, rows):
     if kind == "one_row":
         return torch.full((n,), rows // 2, device="cuda")
