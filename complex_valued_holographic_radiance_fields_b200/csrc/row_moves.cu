@@ -270,9 +270,10 @@ __global__ void __launch_bounds__(kThreads, 5) groups_to_rows_kernel(Moves m, co
   }
 }
 
-// Rows that are not aligned, up to 4 KB: a warp puts its rows into the block's tile, two choices
-// of J elements per lane in flight.  Its slots and weights are 32 at a time, one per lane.
-template <typename T, bool WIDE, int J>
+// Rows that are not aligned, up to 4 KB: a warp puts its rows into the block's tile, J elements
+// per lane of CHOICES choices in flight.  Its slots and weights are 32 at a time, one per lane.
+// (Two rows at once: 75 us against 57 for 100003 rows of 333 f16 from 2 choices.)
+template <typename T, bool WIDE, int CHOICES, int J>
 __global__ void __launch_bounds__(kTileThreads) groups_to_rows_tile_kernel(long long rows, int choices, int tile,
                                                                            int width, const int* __restrict__ slots,
                                                                            const T* __restrict__ y, long long stride,
@@ -304,19 +305,26 @@ __global__ void __launch_bounds__(kTileThreads) groups_to_rows_tile_kernel(long 
       float acc[J];
 #pragma unroll
       for (int j = 0; j < J; ++j) acc[j] = 0.f;
-      for (int i = 0; i < choices; i += 2) {
+      for (int i = 0; i < choices; i += CHOICES) {
         const T *a, *b;
         float wa, wb = 0.f;
         entry(r * choices + i, a, wa);
-        if (i + 1 < choices) entry(r * choices + i + 1, b, wb);
+        // (a row of zeros for a choice too many: loads under a branch would wait one by one)
+        if (CHOICES > 1 && i + 1 < choices) entry(r * choices + i + 1, b, wb);
         else b = reinterpret_cast<const T*>(g_zero_row) + lane;
         T va[J], vb[J];
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (32 * j < left) va[j] = a[c + 32 * j], vb[j] = b[c + 32 * j];
+          if (32 * j < left) {
+            va[j] = a[c + 32 * j];
+            if (CHOICES > 1) vb[j] = b[c + 32 * j];
+          }
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (32 * j < left) acc[j] = fmaf(wb, to_float(vb[j]), fmaf(wa, to_float(va[j]), acc[j]));
+          if (32 * j < left) {
+            acc[j] = fmaf(wa, to_float(va[j]), acc[j]);
+            if (CHOICES > 1) acc[j] = fmaf(wb, to_float(vb[j]), acc[j]);
+          }
       }
 #pragma unroll
       for (int j = 0; j < J; ++j)
@@ -325,6 +333,63 @@ __global__ void __launch_bounds__(kTileThreads) groups_to_rows_tile_kernel(long 
     }
   }
   send_tile(buf, n, width, out + first * width);
+}
+
+// The same for narrow rows, flat as gather_flat: an element (16 bits: two) of the block's run of
+// rows per lane and step, kFlatSteps steps at once, the places and weights in shared memory.
+// (1.6M rows of 31 floats from a choice: 99 us, 135 by warps with two rows each; of 59: 97 and 97.
+// 4M rows of 12 f16: 108 us, 303 by an element per lane and row.)
+constexpr int kFlatSumWidth = 64, kFlatSteps = 4;
+constexpr int kFlatEntries = 1024;   // rows x choices of a block at most
+
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) groups_to_rows_flat_kernel(long long rows, int choices, int tile,
+                                                                           uint32_t reciprocal, int width,
+                                                                           const int* __restrict__ slots,
+                                                                           const T* __restrict__ y, long long stride,
+                                                                           Weights weights, T* __restrict__ out) {
+  constexpr int kEach = 4 / (int)sizeof(T);
+  __shared__ const T* row[kFlatEntries];
+  __shared__ float weight[kFlatEntries];
+  const long long first = (long long)blockIdx.x * tile;
+  const int n = (int)min((long long)tile, rows - first);
+  for (int k = threadIdx.x; k < n * choices; k += kTileThreads) {
+    const int s = slots[first * choices + k];
+    row[k] = s >= 0 ? y + (long long)s * stride : reinterpret_cast<const T*>(g_zero_row);
+    weight[k] = s >= 0 ? weight_at<T>(weights, first * choices + k) : 0.f;   // left out: whatever its weight holds
+  }
+  __syncthreads();
+  T* to = out + first * width;
+  const int total = n * width;
+  for (int p0 = threadIdx.x * kEach; p0 < total; p0 += kTileThreads * kEach * kFlatSteps) {
+    int at[kFlatSteps][kEach], col[kFlatSteps][kEach];
+    float acc[kFlatSteps][kEach];
+#pragma unroll
+    for (int u = 0; u < kFlatSteps; ++u)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int e = min(p0 + u * kTileThreads * kEach + i, total - 1), t = flat_row(e, width, reciprocal);
+        at[u][i] = t * choices;
+        col[u][i] = e - t * width;
+        acc[u][i] = 0.f;
+      }
+    for (int j = 0; j < choices; ++j) {
+      T v[kFlatSteps][kEach];
+#pragma unroll
+      for (int u = 0; u < kFlatSteps; ++u)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[u][i] = row[at[u][i] + j][col[u][i]];
+#pragma unroll
+      for (int u = 0; u < kFlatSteps; ++u)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) acc[u][i] = fmaf(weight[at[u][i] + j], to_float(v[u][i]), acc[u][i]);
+    }
+#pragma unroll
+    for (int u = 0; u < kFlatSteps; ++u) {
+      const int p = p0 + u * kTileThreads * kEach;
+      if (p < total) flat_store(to + p, acc[u], p + kEach <= total);
+    }
+  }
 }
 
 // ... and its gradient, by places: dy[p] = w dout[n], dw = <dout[n], y[p]> for the entry at p.
@@ -398,6 +463,68 @@ __global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_tile_ker
     else ((float*)grad_weights)[entry] = my_dot;
   }
   if (grad_y) send_tile(buf, n, width, grad_y + first * width);
+}
+
+// The same for narrow rows, flat; the products of a place's dot product go through shared memory
+// to one thread, which adds them up in order.  (4M rows of 12 f16: 162 us, 545 by an element per
+// lane and row; 3M of 33: 230, 289 by warps; 1.7M of 59: 225 and 190.  4M rows of 2 floats: 62 and
+// 69, of 1: 59 and 34.)
+constexpr int kFlatGradWidth = 40;
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_flat_kernel(
+    Places places, long long count, int tile, uint32_t reciprocal, int width, const T* __restrict__ grad,
+    long long grad_stride, const T* __restrict__ y, long long stride, Weights weights, T* __restrict__ grad_y,
+    void* __restrict__ grad_weights) {
+  constexpr int kEach = 4 / (int)sizeof(T);
+  __shared__ const T* grad_row[kFlatRows];
+  __shared__ float weight[kFlatRows];
+  __shared__ float product[kTileThreads * kFlatWords * kEach / 2];
+  const T* zeros = reinterpret_cast<const T*>(g_zero_row);
+  const long long first = (long long)blockIdx.x * tile;
+  const int n = (int)min((long long)tile, count - first);
+  const int used = (int)max(0ll, min((long long)n, *places.used - first));   // the others' rows are not read
+  const T* const y0 = y + first * stride;
+  for (int k = threadIdx.x; k < n; k += kTileThreads) {
+    const long long p = first + k, r = places.row(p);
+    grad_row[k] = r >= 0 ? grad + r * grad_stride : zeros;
+    weight[k] = r >= 0 ? weight_at<T>(weights, places.order[p]) : 0.f;
+  }
+  __syncthreads();
+  const int total = n * width;
+  for (int p0 = threadIdx.x * kEach; p0 < total; p0 += kTileThreads * kEach * kFlatSteps) {
+    T g[kFlatSteps][kEach], h[kFlatSteps][kEach];
+    int row[kFlatSteps][kEach];
+#pragma unroll
+    for (int u = 0; u < kFlatSteps; ++u)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int e = min(p0 + u * kTileThreads * kEach + i, total - 1), t = flat_row(e, width, reciprocal);
+        row[u][i] = t;
+        g[u][i] = grad_row[t][e - t * width];
+        if (grad_weights) h[u][i] = *(t < used ? y0 + t * stride + (e - t * width) : zeros);
+      }
+#pragma unroll
+    for (int u = 0; u < kFlatSteps; ++u) {
+      const int p = p0 + u * kTileThreads * kEach;
+      float f[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        f[i] = to_float(g[u][i]);
+        if (grad_weights && p + i < total) product[p + i] = f[i] * to_float(h[u][i]);
+        f[i] *= weight[row[u][i]];
+      }
+      if (grad_y && p < total) flat_store(grad_y + first * width + p, f, p + kEach <= total);
+    }
+  }
+  if (!grad_weights) return;
+  __syncthreads();
+  for (int k = threadIdx.x; k < n; k += kTileThreads) {
+    float dot = 0.f;
+    for (int c = 0; c < width; ++c) dot += product[k * width + c];
+    const int entry = places.order[first + k];
+    if (weights.same) ((T*)grad_weights)[entry] = from_float<T>(dot);
+    else ((float*)grad_weights)[entry] = dot;
+  }
 }
 
 // Packs follow the row of grad_y that is written (with unaligned rows each choice's begins
@@ -566,19 +693,36 @@ int to_groups(bool aligned, const void* x, long long stride, Moves m, const int*
 
 template <typename T>
 int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weights, void* out, cudaStream_t st) {
+  const bool pairs = ((uintptr_t)out & 3) == 0;
+  // (Very narrow rows of many choices read their places again for every element: 22 us against 48
+  // for 500000 rows of 2 f16 from 8 choices; of 12: 110 against 83.)
+  if (!aligned && m.width >= (m.choices > 2 ? 8 : 3) && m.width <= kFlatSumWidth && m.choices <= kFlatEntries / 8 && pairs) {
+    const int most = kFlatEntries / m.choices / 2 * 2, rows = flat_rows(m.width, sizeof(T));
+    const int tile = rows < most ? rows : most;
+    groups_to_rows_flat_kernel<T><<<(unsigned)((m.n + tile - 1) / tile), kTileThreads, 0, st>>>(
+        m.n, m.choices, tile, flat_reciprocal(m.width), m.width, m.slots, (const T*)y, stride, weights, (T*)out);
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
   if (!aligned && m.width > kFlatWidth && tile_fits(m.width, sizeof(T), out)) {
     const int tile = tile_rows(m.n, m.width, sizeof(T));
     const unsigned blocks = (unsigned)((m.n + tile - 1) / tile);
     const size_t shared = (size_t)tile * m.width * sizeof(T);
-#define CVHRF_LAUNCH(WIDE, J)                                                          \
-  groups_to_rows_tile_kernel<T, WIDE, J><<<blocks, kTileThreads, shared, st>>>(        \
+#define CVHRF_SHAPE(WIDE, CHOICES, J)                                                       \
+  groups_to_rows_tile_kernel<T, WIDE, CHOICES, J><<<blocks, kTileThreads, shared, st>>>(    \
       m.n, m.choices, tile, m.width, m.slots, (const T*)y, stride, weights, (T*)out)
+#define CVHRF_LAUNCH(WIDE, J)                      \
+  do {                                             \
+    if (m.choices == 1) CVHRF_SHAPE(WIDE, 1, J);   \
+    else CVHRF_SHAPE(WIDE, 2, J);                  \
+  } while (0)
     const int steps = (m.width + 255) / 256;   // J shares the row evenly between them
     if (m.width > 128 && m.width <= steps * 192) CVHRF_LAUNCH(true, 6);
     else if (m.width > 128) CVHRF_LAUNCH(true, 8);
     else if (m.width > 64) CVHRF_LAUNCH(false, 4);
     else if (m.width > 32) CVHRF_LAUNCH(false, 2);
     else CVHRF_LAUNCH(false, 1);
+#undef CVHRF_SHAPE
 #undef CVHRF_LAUNCH
     CVHRF_LAUNCH_CHECK();
     return CVHRF_OK;
@@ -608,9 +752,17 @@ int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weig
 template <typename T>
 int to_rows_backward(bool aligned, const void* grad, long long grad_stride, const void* y, long long stride, Moves m,
                      const int* order, Weights weights, void* grad_y, void* grad_weights, cudaStream_t st) {
+  const Places places{order, m.used, m.choices};
+  const long long count = m.n * m.choices;
+  if (!aligned && m.width >= 3 && m.width <= kFlatGradWidth && ((uintptr_t)grad_y & 3) == 0) {
+    const int tile = flat_rows(m.width, sizeof(T)) / 4 * 2;
+    groups_to_rows_backward_flat_kernel<T><<<(unsigned)((count + tile - 1) / tile), kTileThreads, 0, st>>>(
+        places, count, tile, flat_reciprocal(m.width), m.width, (const T*)grad, grad_stride, (const T*)y, stride,
+        weights, (T*)grad_y, grad_weights);
+    CVHRF_LAUNCH_CHECK();
+    return CVHRF_OK;
+  }
   if (!aligned && m.width > kFlatWidth && tile_fits(m.width, sizeof(T), grad_y)) {
-    const Places places{order, m.used, m.choices};
-    const long long count = m.n * m.choices;
     const int tile = tile_rows(count, m.width, sizeof(T));
     const unsigned blocks = (unsigned)((count + tile - 1) / tile);
     const size_t shared = (size_t)tile * m.width * sizeof(T);

@@ -861,8 +861,12 @@ int gradient(const void* grad, long long stride, int width, long long n, long lo
     return launch_gradient<T, true, 1>(g, packs < 32 ? packs : 32, n, grad, out, joins, st);
   }
   if (width <= 32) return launch_gradient<T, false, 1>(g, width, n, grad, out, joins, st);
-  if (width <= 64) return launch_gradient<T, false, 2>(g, 32, n, grad, out, joins, st);
-  if (width <= 128) return launch_gradient<T, false, 4>(g, 32, n, grad, out, joins, st);
+  // tiles of equal width: 257 columns are two of 192, not one of 256 and one of a column
+  const int tiles = (width + 255) / 256, each = (width + 32 * tiles - 1) / (32 * tiles);
+  if (each <= 2) return launch_gradient<T, false, 2>(g, 32, n, grad, out, joins, st);
+  if (each <= 3) return launch_gradient<T, false, 3>(g, 32, n, grad, out, joins, st);
+  if (each <= 4) return launch_gradient<T, false, 4>(g, 32, n, grad, out, joins, st);
+  if (each <= 6) return launch_gradient<T, false, 6>(g, 32, n, grad, out, joins, st);
   return launch_gradient<T, false, 8>(g, 32, n, grad, out, joins, st);
 }
 

@@ -192,6 +192,19 @@ inline uint32_t flat_reciprocal(int width) {   // of 1 it would be 2^32: not use
   return width == 1 ? 0u : (uint32_t)((0xffffffffull + width) / width);
 }
 
+// The row of element e of a run.
+__device__ __forceinline__ int flat_row(int e, int width, uint32_t reciprocal) {
+  return width == 1 ? e : (int)__umulhi((uint32_t)e, reciprocal);
+}
+// A lane's word of a run, or its first element where the run ends inside it.
+__device__ __forceinline__ void flat_store(float* to, const float (&f)[1], bool) { *to = f[0]; }
+template <typename T>
+__device__ __forceinline__ void flat_store(T* to, const float (&f)[2], bool whole) {
+  struct alignas(4) Two { T a, b; };
+  if (whole) *reinterpret_cast<Two*>(to) = Two{from_float<T>(f[0]), from_float<T>(f[1])};
+  else *to = from_float<T>(f[0]);
+}
+
 template <typename T, bool SCALE, typename Get>
 __device__ __forceinline__ void gather_flat(const Get& get, long long rows, int tile, uint32_t reciprocal, int width,
                                             float scale, T* __restrict__ out) {
@@ -211,7 +224,7 @@ __device__ __forceinline__ void gather_flat(const Get& get, long long rows, int 
     T v[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int e = min(p + i, total - 1), t = width == 1 ? e : (int)__umulhi((uint32_t)e, reciprocal);
+      const int e = min(p + i, total - 1), t = flat_row(e, width, reciprocal);
       const T x = row[t][e - t * width];
       v[i] = SCALE ? from_float<T>(scale * to_float(x)) : x;
     }

@@ -297,6 +297,18 @@ def test_groups_of_one_kind(cuda):
 @pytest.mark.parametrize("width", [1, 3, 8, 17, 20, 59, 64, 333, 530, 1024, 2051, 2056])
 @pytest.mark.parametrize("n,k,groups", [(1, 1, 1), (3, 8, 8), (301, 2, 7), (1000, 3, 300)])
 def test_moves_and_their_gradients(cuda, dtype, wtype, width, n, k, groups):
+    moves_and_their_gradients(dtype, wtype, width, n, k, groups)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,wtype", [(torch.float32, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("width", [2, 5, 6, 7, 12, 33, 40, 41, 63, 66, 129])
+@pytest.mark.parametrize("n,k,groups", [(1, 128, 200), (70, 129, 200), (1200, 1, 3), (777, 7, 9), (20, 300, 40)])
+def test_moves_of_narrow_rows_and_many_choices(cuda, dtype, wtype, width, n, k, groups):
+    moves_and_their_gradients(dtype, wtype, width, n, k, groups)
+
+
+def moves_and_their_gradients(dtype, wtype, width, n, k, groups):
     index = integers(n * k, groups + 1, n + width, -1).reshape(n, k)
     if n > 1:
         index[n // 2] = -1                                   # a row without any group
