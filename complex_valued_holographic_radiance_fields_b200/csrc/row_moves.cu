@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) rows_to_groups_kernel(Moves m, const
   const long long first = (long long)blockIdx.x * (owners * ROWS) + o.index;
   if (!o.live) return;
   const int used = *m.used;
-  for (int c0 = lane * R::kVec; c0 < m.width; c0 += step * J) {
+  for (int c0 = lane * R::kVec + (int)blockIdx.y * step * J; c0 < m.width; c0 += step * J * (int)gridDim.y) {
     uint4 p[ROWS][J];
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kThreads) rows_to_groups_kernel(Moves m, const
   }
 #pragma unroll
   for (int q = 0; q < ROWS; ++q)
-    if (first + q * owners < m.n) clear_behind<T, kAligned>(m, used, first + q * owners, m.n, lane, out);
+    if (first + q * owners < m.n && blockIdx.y == 0)
+      clear_behind<T, kAligned>(m, used, first + q * owners, m.n, lane, out);
 }
 
 // Other rows: packs follow the row that is written, which begins elsewhere for every choice,
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) entries_to_groups_kernel(Moves m, co
     if (s < 0) edges[q].packs = edges[q].count = 0;
     else inside = inside && extent.inside(from[q], m.width);
   }
-  for (int k = lane; k < packs_of<T, L>(m.width); k += m.lanes) {
+  for (int k = lane + (int)blockIdx.y * m.lanes; k < packs_of<T, L>(m.width); k += m.lanes * (int)gridDim.y) {
     typename R::Raw p[ENTRIES];
     if (inside) {
 #pragma unroll
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(kThreads) entries_to_groups_kernel(Moves m, co
     for (int q = 0; q < ENTRIES; ++q)
       if (k < edges[q].packs) R::store(to[q] + edges[q].head + k * R::kVec, R::words(p[q]));
   }
+  if (blockIdx.y) return;
 #pragma unroll
   for (int q = 0; q < ENTRIES; ++q) {
     if (L == kSpan)
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 5) groups_to_rows_kernel(Moves m, co
         if (s >= 0) inside = inside && extent.inside(y + (long long)s * stride, m.width);
       }
   }
-  for (int k = lane; k < packs_of<T, L>(m.width); k += m.lanes) {
+  for (int k = lane + (int)blockIdx.y * m.lanes; k < packs_of<T, L>(m.width); k += m.lanes * (int)gridDim.y) {
     float acc[ROWS][R::kVec];
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 5) groups_to_rows_kernel(Moves m, co
       if (k < edges[q].packs)
         R::store(out + (first + q * owners) * m.width + edges[q].head + k * R::kVec, R::words(acc[q]));
   }
-  if (L == kSpan) {
+  if (L == kSpan && blockIdx.y == 0) {
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const long long row = first + q * owners;
@@ -539,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
   const int owners = m.owners, lane = o.lane;
   // lanes without an owner stay for the shuffles, behind the last row
   const long long first = o.live ? (long long)blockIdx.x * (owners * ROWS) + o.index : m.n;
-  for (int i0 = 0; i0 < m.choices; i0 += CHOICES) {
+  for (int i0 = (int)blockIdx.y * CHOICES; i0 < m.choices; i0 += CHOICES * (int)gridDim.y) {
     int slot[ROWS][CHOICES];
     float w[ROWS][CHOICES], dot[ROWS][CHOICES];
     Edges edges[ROWS][CHOICES];
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
         }
     }
   }
-  if (grad_y) {
+  if (grad_y && blockIdx.y == 0) {
     const int used = *m.used;
 #pragma unroll
     for (int q = 0; q < ROWS; ++q)
@@ -678,12 +680,21 @@ int to_groups(bool aligned, const void* x, long long stride, Moves m, const int*
     const T* from = (const T*)x;
     if constexpr (L == kAligned) {
       const int packs = packs_of<T, L>(m.width);
-      if (packs > 64) rows_to_groups_kernel<T, 1, 4><<<blocks_for(m.n, m.owners, 1), kThreads, 0, st>>>(m, from, stride, (T*)out);
-      else if (packs > 32) rows_to_groups_kernel<T, 2, 2><<<blocks_for(m.n, m.owners, 2), kThreads, 0, st>>>(m, from, stride, (T*)out);
-      else rows_to_groups_kernel<T, 4, 1><<<blocks_for(m.n, m.owners, 4), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      if (packs > 64) {
+        // (2 per SM: 2000 rows of 4096 floats to 4 places each 33 us, 35 in two parts)
+        const unsigned blocks = blocks_for(m.n, m.owners, 1);
+        const unsigned parts = parts_for(blocks, (packs + lanes * 4 - 1) / (lanes * 4), 2);
+        rows_to_groups_kernel<T, 1, 4><<<dim3(blocks, parts), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      } else if (packs > 32) {
+        rows_to_groups_kernel<T, 2, 2><<<blocks_for(m.n, m.owners, 2), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      } else {
+        rows_to_groups_kernel<T, 4, 1><<<blocks_for(m.n, m.owners, 4), kThreads, 0, st>>>(m, from, stride, (T*)out);
+      }
     } else {
       constexpr int kEntries = L == kSpan ? 2 : 4;
-      entries_to_groups_kernel<T, L, kEntries><<<blocks_for(m.n * m.choices, m.owners, kEntries), kThreads, 0, st>>>(
+      const unsigned blocks = blocks_for(m.n * m.choices, m.owners, kEntries);
+      const unsigned parts = parts_for(blocks, (packs_of<T, L>(m.width) + lanes - 1) / lanes);
+      entries_to_groups_kernel<T, L, kEntries><<<dim3(blocks, parts), kThreads, 0, st>>>(
           m, from, extent_of(x, m.n, stride, m.width, sizeof(T)), stride, (T*)out);
     }
     CVHRF_LAUNCH_CHECK();
@@ -732,9 +743,11 @@ int to_rows(bool aligned, const void* y, long long stride, Moves m, Weights weig
     m.lanes = lanes;
     m.owners = owners_of(kThreads, lanes);
     const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
-#define CVHRF_LAUNCH(ROWS, CHOICES)                                                               \
-  groups_to_rows_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, m.owners, ROWS), kThreads, 0, st>>>(  \
-      m, (const T*)y, extent, stride, weights, (T*)out)
+    const int steps = (packs_of<T, L>(m.width) + lanes - 1) / lanes;
+#define CVHRF_LAUNCH(ROWS, CHOICES)                                                                      \
+  groups_to_rows_kernel<T, L, ROWS, CHOICES>                                                             \
+      <<<dim3(blocks_for(m.n, m.owners, ROWS), parts_for(blocks_for(m.n, m.owners, ROWS), steps)), kThreads, 0, st>>>( \
+          m, (const T*)y, extent, stride, weights, (T*)out)
     if constexpr (L == kSpan) {   // twice the registers per pack
       if (m.choices > 1) CVHRF_LAUNCH(1, 2);
       else CVHRF_LAUNCH(1, 1);
@@ -785,8 +798,12 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
     m.owners = owners_of(kThreads, lanes);
     const Extent grad_extent = extent_of(grad, m.n, grad_stride, m.width, sizeof(T));
     const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
+    // (few rows: the choices are shared between blocks, each dot product stays with one owner)
 #define CVHRF_LAUNCH(ROWS, CHOICES)                                                                        \
-  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES><<<blocks_for(m.n, m.owners, ROWS), kThreads, 0, st>>>(  \
+  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES>                                                      \
+      <<<dim3(blocks_for(m.n, m.owners, ROWS),                                                             \
+              parts_for(blocks_for(m.n, m.owners, ROWS), (m.choices + CHOICES - 1) / CHOICES)),            \
+         kThreads, 0, st>>>(                                                                               \
       m, (const T*)grad, grad_extent, grad_stride, (const T*)y, extent, stride, weights, (T*)grad_y, grad_weights)
     if constexpr (L == kSpan) {   // four times: the pack of grad and of y
       CVHRF_LAUNCH(1, 1);

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, 4) table_lookup_kernel(const T* __re
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) from[k] = v[k] >= 0 ? table + v[k] * stride : nullptr;
     bool next = true;
-    for (int c = o.lane * R::kVec; c < width; c += step * J) {
+    for (int c = o.lane * R::kVec + (int)blockIdx.y * step * J; c < width; c += step * J * (int)gridDim.y) {
       typename R::Raw p[ROWS][J];
 #pragma unroll
       for (int k = 0; k < ROWS; ++k)
@@ -155,7 +155,9 @@ int launch_lookup(const void* table, long long rows, int width, long long stride
   const int owners = owners_of(kThreads, lanes);
   const long long per_block = (long long)owners * ROWS, blocks = (entries + per_block - 1) / per_block;
   const long long most = 148 * resident;
-  table_lookup_kernel<T, ROWS, J><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, st>>>(
+  const unsigned parts = parts_for((unsigned)(blocks < most ? blocks : most),
+                                   (packs_of<T, kAligned>(width) + lanes * J - 1) / (lanes * J));
+  table_lookup_kernel<T, ROWS, J><<<dim3((unsigned)(blocks < most ? blocks : most), parts), kThreads, 0, st>>>(
       (const T*)table, rows, width, stride, index, index_bytes, entries, lanes, owners, scale, (T*)out);
   CVHRF_LAUNCH_CHECK();
   return CVHRF_OK;

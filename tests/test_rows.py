@@ -308,6 +308,25 @@ def test_moves_of_narrow_rows_and_many_choices(cuda, dtype, wtype, width, n, k, 
     moves_and_their_gradients(dtype, wtype, width, n, k, groups)
 
 
+@gpu
+@pytest.mark.parametrize("dtype,wtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("width", [260, 1032, 4096, 4097, 8200, 9001])
+@pytest.mark.parametrize("n,k,groups", [(1, 1, 1), (1, 8, 16), (2, 3, 5), (64, 4, 32), (700, 2, 9)])
+def test_moves_of_few_wide_rows(cuda, dtype, wtype, width, n, k, groups):
+    moves_and_their_gradients(dtype, wtype, width, n, k, groups)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [4096, 8200, 65544])
+@pytest.mark.parametrize("n", [1, 3, 64])
+def test_lookup_of_few_wide_rows(cuda, dtype, width, n):
+    table, index = normal((50, width), dtype, 1), integers(n, 51, 2, -1)
+    inside = index >= 0
+    exact = torch.where(inside[:, None], table[index.clamp(min=0)].double() * 0.75, 0.0)
+    close(R.table_lookup(table, index, 0.75), exact, 0 * exact)
+
+
 def moves_and_their_gradients(dtype, wtype, width, n, k, groups):
     index = integers(n * k, groups + 1, n + width, -1).reshape(n, k)
     if n > 1:
