@@ -775,7 +775,7 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
     CVHRF_LAUNCH_CHECK();
     return CVHRF_OK;
   }
-  if (!aligned && m.width > kFlatWidth && tile_fits(m.width, sizeof(T), grad_y)) {
+  if (!aligned && m.width > kFlatGradWidth && tile_fits(m.width, sizeof(T), grad_y)) {
     const int tile = tile_rows(count, m.width, sizeof(T));
     const unsigned blocks = (unsigned)((count + tile - 1) / tile);
     const size_t shared = (size_t)tile * m.width * sizeof(T);
@@ -786,8 +786,7 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
     if (m.width > 128 && m.width <= steps * 192) CVHRF_LAUNCH(true, 1, 6);
     else if (m.width > 128) CVHRF_LAUNCH(true, 1, 8);
     else if (m.width > 64) CVHRF_LAUNCH(false, 1, 4);
-    else if (m.width > 32) CVHRF_LAUNCH(false, 2, 2);
-    else CVHRF_LAUNCH(false, 4, 1);
+    else CVHRF_LAUNCH(false, 2, 2);
 #undef CVHRF_LAUNCH
     CVHRF_LAUNCH_CHECK();
     return CVHRF_OK;

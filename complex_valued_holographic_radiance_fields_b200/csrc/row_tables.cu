@@ -136,7 +136,9 @@ template <typename T, int LANES, int FLIGHT, int J>
 int launch_lookup_words(const void* table, long long rows, int width, long long stride, const void* index,
                         int index_bytes, long long entries, float scale, void* out, cudaStream_t st) {
   const int lanes = word_lanes(words_of<T>(width)), owners = 32 / lanes, rounds = rounds_for(entries, owners, FLIGHT);
-  table_lookup_words_kernel<T, LANES, FLIGHT, J><<<word_blocks(entries, rounds, owners), kWordThreads, 0, st>>>(
+  const unsigned blocks = word_blocks(entries, rounds, owners);
+  const unsigned parts = parts_for(blocks, (words_of<T>(width) + lanes * J - 1) / (lanes * J));
+  table_lookup_words_kernel<T, LANES, FLIGHT, J><<<dim3(blocks, parts), kWordThreads, 0, st>>>(
       (const T*)table, source4_of(table, rows, stride, width, sizeof(T)), rows, width, index, index_bytes, entries,
       rounds, lanes, scale, (T*)out);
   CVHRF_LAUNCH_CHECK();

@@ -153,7 +153,7 @@ __device__ __forceinline__ void copy_rows(const Get& get, long long entries, int
       to[q] = shuffle(my_to, src & 31);
       if (!LANES && (owner >= owners || src > 31)) from[q] = to[q] = 0;
     }
-    for (int c = word; c < width / kEach; c += lanes * J) {
+    for (int c = word + (int)blockIdx.y * lanes * J; c < width / kEach; c += lanes * J * (int)gridDim.y) {
       RawWord v[FLIGHT][J];
 #pragma unroll
       for (int q = 0; q < FLIGHT; ++q) {
@@ -184,7 +184,7 @@ __device__ __forceinline__ void copy_rows(const Get& get, long long entries, int
           }
       }
     }
-    if (sizeof(T) == 2) {
+    if (sizeof(T) == 2 && blockIdx.y == 0) {
 #pragma unroll
       for (int q = 0; q < FLIGHT; ++q) {
         const To<T> t(to[q], width);

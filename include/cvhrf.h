@@ -571,7 +571,8 @@ int cvhrf_table_lookup(const cvhrf_lookup_args* args, void* stream);
  * (zeros where there is none), every row written; row_mask[v] (may be null) = 1 where
  * there is one, the mask cvhrf_sparse_adam_masked takes.  The order of the sums is fixed
  * (the entries' order, joined between blocks in a fixed order): results repeat bit for
- * bit.  The workspace query returns 0 where none is needed.  An entry whose index is outside [0, rows) is left out and its row not read.
+ * bit.  The workspace query returns 0 where none is needed.  An entry whose index is outside
+ * [0, rows) is left out and its row not read.
  */
 typedef struct {
   const void* grad;
@@ -611,8 +612,8 @@ int cvhrf_group_rows(const cvhrf_group_args* args, void* stream);
  * number of places that belong to a group (offsets + groups of cvhrf_group_rows).
  *   cvhrf_rows_to_groups:  to[slot] = from[n]  (n * choices rows; those from *used on are zeros)
  *   cvhrf_groups_to_rows:  to[n] = sum_j weights[n, j] from[slots[n, j]]  (float32 sum; entries
- *     left out count nothing; weights null: ones; order and used are not read).  Without weights it is the
- *     gradient of cvhrf_rows_to_groups.
+ *     left out count nothing; weights null: ones; order and used are not read).  Without
+ *     weights it is the gradient of cvhrf_rows_to_groups.
  *   cvhrf_groups_to_rows_backward: grad_y[slot] = weights[n, j] grad[n] (rows from *used on:
  *     zeros), grad_weights[n, j] = <grad[n], y[slot]> (0 where left out); either may be null.
  * weights are float32 or of type `dtype`, n x choices, contiguous.

@@ -318,7 +318,7 @@ def test_moves_of_few_wide_rows(cuda, dtype, wtype, width, n, k, groups):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("width", [4096, 8200, 65544])
+@pytest.mark.parametrize("width", [4096, 4097, 8200, 9001, 65544])
 @pytest.mark.parametrize("n", [1, 3, 64])
 def test_lookup_of_few_wide_rows(cuda, dtype, width, n):
     table, index = normal((50, width), dtype, 1), integers(n, 51, 2, -1)
