@@ -12,6 +12,7 @@
 // Bound by memory: each touches N + N k rows once.  16384 rows of 2048 bf16 to 4 of 64 groups:
 // 51 us there (6.6 TB/s), 60 back (5.6), 101 for the gradient (5.3, y read for dw).  100003 odd
 // rows of 333 f16 to 2 of 7: 45, 57 and 87 us, where 2-byte loads are what is waited for.
+#include <algorithm>
 #include <type_traits>
 #include "row_groups.cuh"
 #include "row_tiles.cuh"
@@ -530,14 +531,15 @@ __global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_flat_ker
 }
 
 // Packs follow the row of grad_y that is written (with unaligned rows each choice's begins
-// elsewhere, so the row of grad is read again for it, from L1).
-template <typename T, Layout L, int ROWS, int CHOICES>
+// elsewhere, so the row of grad is read again for it, from L1).  BLOCK: a whole block owns a row,
+// its warps' dot products are joined in their order.
+template <typename T, Layout L, int ROWS, int CHOICES, bool BLOCK>
 __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
     Moves m, const T* __restrict__ grad, Extent grad_extent, long long grad_stride, const T* __restrict__ y,
     Extent extent, long long stride, Weights weights, T* __restrict__ grad_y, void* __restrict__ grad_weights) {
   using R = Row<T, L>;
   constexpr bool kShared = L != kSpan;   // one pack of grad for all choices
-  const Owner o = Owner::of(m.lanes);
+  const Owner o = BLOCK ? Owner{0, (int)threadIdx.x, true} : Owner::of(m.lanes);
   const int owners = m.owners, lane = o.lane;
   // lanes without an owner stay for the shuffles, behind the last row
   const long long first = o.live ? (long long)blockIdx.x * (owners * ROWS) + o.index : m.n;
@@ -614,7 +616,17 @@ __global__ void __launch_bounds__(kThreads, 4) groups_to_rows_backward_kernel(
 #pragma unroll
         for (int i = 0; i < CHOICES; ++i) {
           float d = dot[q][i];
-          if ((m.lanes & (m.lanes - 1)) == 0) {
+          if constexpr (BLOCK) {
+            __shared__ float part[kThreads / 32];
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+            if ((lane & 31) == 0) part[lane >> 5] = d;
+            __syncthreads();
+            d = part[0];
+#pragma unroll
+            for (int x = 1; x < kThreads / 32; ++x) d += part[x];
+            __syncthreads();
+          } else if ((m.lanes & (m.lanes - 1)) == 0) {
             for (int x = m.lanes >> 1; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
           } else {   // lanes beside one another: halve what is left, an odd one waits for its turn
             for (int left = m.lanes; left > 1; left = (left + 1) >> 1) {
@@ -797,19 +809,32 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
     m.owners = owners_of(kThreads, lanes);
     const Extent grad_extent = extent_of(grad, m.n, grad_stride, m.width, sizeof(T));
     const Extent extent = extent_of(y, m.n * m.choices, stride, m.width, sizeof(T));
-    // (few rows: the choices are shared between blocks, each dot product stays with one owner)
-#define CVHRF_LAUNCH(ROWS, CHOICES)                                                                        \
-  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES>                                                      \
+    // Few rows: the choices are shared between blocks, and long rows are a whole block's, the longer
+    // the more of them (64 rows of 9000 floats to 8 places: 7.5 us, 75 by warps, 148 without either;
+    // 2000 of 4096 floats to one: 19 and 30; of 1024 floats to 4: 14 and 11).
+#define CVHRF_LAUNCH(ROWS, CHOICES, BLOCK)                                                                 \
+  groups_to_rows_backward_kernel<T, L, ROWS, CHOICES, BLOCK>                                               \
       <<<dim3(blocks_for(m.n, m.owners, ROWS),                                                             \
               parts_for(blocks_for(m.n, m.owners, ROWS), (m.choices + CHOICES - 1) / CHOICES)),            \
          kThreads, 0, st>>>(                                                                               \
       m, (const T*)grad, grad_extent, grad_stride, (const T*)y, extent, stride, weights, (T*)grad_y, grad_weights)
+    if constexpr (L != kElement) {
+      const long long packs = packs_of<T, L>(m.width), entries = (long long)blocks_for(m.n, m.owners, 1) * m.choices;
+      if (packs >= 128 && entries < 148 * std::min(8ll, packs / 128)) {
+        m.lanes = kThreads;
+        m.owners = 1;
+        if (L == kAligned && m.choices > 1) CVHRF_LAUNCH(1, 2, true);
+        else CVHRF_LAUNCH(1, 1, true);
+        CVHRF_LAUNCH_CHECK();
+        return CVHRF_OK;
+      }
+    }
     if constexpr (L == kSpan) {   // four times: the pack of grad and of y
-      CVHRF_LAUNCH(1, 1);
+      CVHRF_LAUNCH(1, 1, false);
     } else {
-      if (m.choices > 2) CVHRF_LAUNCH(1, 4);
-      else if (m.choices > 1) CVHRF_LAUNCH(1, 2);
-      else CVHRF_LAUNCH(2, 1);
+      if (m.choices > 2) CVHRF_LAUNCH(1, 4, false);
+      else if (m.choices > 1) CVHRF_LAUNCH(1, 2, false);
+      else CVHRF_LAUNCH(2, 1, false);
     }
 #undef CVHRF_LAUNCH
     CVHRF_LAUNCH_CHECK();
