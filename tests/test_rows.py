@@ -282,6 +282,17 @@ def test_groups(cuda, groups, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("groups", [8191, 8192, 8193, 65537, 1000003])
+@pytest.mark.parametrize("n", [1, 5000, 8192, 8193])
+def test_more_groups_than_entries(cuda, groups, n):
+    for itype in (torch.int32, torch.int64):
+        index = integers(n, groups + 1, n + groups, -1, itype)
+        got = R.group_rows(index, groups)
+        for a, b in zip((got.order, got.slots, got.offsets), places_64(index, groups)):
+            assert torch.equal(a.long().cpu(), b)
+
+
+@gpu
 def test_groups_of_one_kind(cuda):
     for value in (0, 2, -1, 9):
         index = torch.full((5000,), value, dtype=torch.int32, device="cuda")
