@@ -49,7 +49,7 @@ __device__ __forceinline__ void clear_touched(uint8_t* touched, uint32_t rows) {
 }
 
 // counts[chunk][digit] over the keys of each chunk.
-__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, const uint32_t* __restrict__ n_dev,
+__global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_t n, const uint32_t* n_dev,
                                                                uint32_t chunk, int shift, int radix,
                                                                uint32_t* __restrict__ counts,
                                                                uint8_t* __restrict__ clear) {
@@ -88,9 +88,8 @@ __global__ void __launch_bounds__(kThreads) chunk_count_kernel(Source s, uint32_
 }
 
 __global__ void __launch_bounds__(kThreads) chunk_scatter_kernel(Source s, uint32_t n,
-                                                                 const uint32_t* __restrict__ n_dev, uint32_t chunk,
-                                                                 int shift, int radix,
-                                                                 const uint32_t* __restrict__ counts, Target out) {
+                                                                 const uint32_t* n_dev, uint32_t chunk, int shift,
+                                                                 int radix, const uint32_t* counts, Target out) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -215,9 +214,8 @@ __global__ void __launch_bounds__(kThreads) small_sort_kernel(Source s, uint32_t
 }
 
 // The places of the entries and the beginnings of the groups from the sorted keys (more groups than one pass sorts).
-__global__ void __launch_bounds__(256) places_kernel(const uint32_t* __restrict__ keys,
-                                                     const uint32_t* __restrict__ entries, uint32_t n, int groups,
-                                                     int* __restrict__ order, int* __restrict__ slots,
+__global__ void __launch_bounds__(256) places_kernel(const uint32_t* keys, const uint32_t* entries, uint32_t n,
+                                                     int groups, int* __restrict__ order, int* __restrict__ slots,
                                                      int* __restrict__ offsets) {
   follow();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -241,8 +239,8 @@ __global__ void __launch_bounds__(256) places_kernel(const uint32_t* __restrict_
 // block looks for all of them (5000 entries: 23 us in all at 8192 groups, 23 with this launch
 // beside; at 65536 groups 60 and 25).
 constexpr int kBlockGroups = 1 << 13;   // most that small_sort_kernel writes itself
-__global__ void __launch_bounds__(256) offsets_kernel(Source s, const uint32_t* __restrict__ order, uint32_t n,
-                                                      int groups, int* __restrict__ offsets) {
+__global__ void __launch_bounds__(256) offsets_kernel(Source s, const uint32_t* order, uint32_t n, int groups,
+                                                      int* __restrict__ offsets) {
   follow();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i > groups) return;

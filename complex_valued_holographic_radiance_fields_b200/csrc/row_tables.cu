@@ -741,9 +741,8 @@ __global__ void __launch_bounds__(row_sort::kThreads) small_table_kernel(SmallTa
 // Sums over the blocks' tables, `slices` threads per element.
 constexpr int kSumSlices = 8, kSumElements = kThreads / kSumSlices;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) table_sum_kernel(const float* __restrict__ sums,
-                                                             const uint8_t* __restrict__ touched, int blocks, int rows,
-                                                             int width, float scale, T* __restrict__ out,
+__global__ void __launch_bounds__(kThreads) table_sum_kernel(const float* sums, const uint8_t* touched, int blocks,
+                                                             int rows, int width, float scale, T* __restrict__ out,
                                                              uint8_t* __restrict__ mask) {
   __shared__ float part[kSumSlices][kSumElements];
   __shared__ int any[kSumElements];

@@ -257,6 +257,11 @@ inline unsigned parts_for(unsigned blocks, int steps, unsigned per_sm = 4) {
 // ---- launches that follow one another ----------------------------------------------------
 // A kernel launched with launch_after may start while the one before it ends; it calls
 // follow() before it touches memory, which waits until that one is done and its writes seen.
+// What the kernel before writes is written while this one is already on the GPU, so it must not be
+// read as `const ... __restrict__`: that lets the compiler take it for constant as long as the
+// kernel runs and read it by the read-only path, whose loads neither follow() orders nor the
+// writes reach.  Only what the caller hands in may be (the first kernel of a chain, launched
+// plainly, has waited for it).
 __device__ __forceinline__ void follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // ... and the one before it says early that the next one may start.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -810,3 +810,19 @@ def test_refusals_on_the_gpu(cuda):
     with pytest.raises(TypeError, match="weights must be"):
         R.groups_to_rows(table[:2], g, torch.ones(2, device="cuda", dtype=torch.float16))
 
+
+
+def test_chained_kernels_read_their_inputs_plainly():
+    """A kernel launched with launch_after is on the GPU while the one before it still writes, so
+    what that one writes must not be declared constant for the kernel's life (const __restrict__:
+    read-only loads); the caller's own inputs may be."""
+    csrc = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    chained = 0
+    for name in sorted(os.listdir(csrc)):
+        src = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        for kernel in set(re.findall(r"\blaunch_after\((\w+_kernel)", src)):
+            params, = re.findall(r"__global__[^;{]*?\b" + kernel + r"\(([^{]*?)\)\s*\{", src)
+            chained += 1
+            constant = set(re.findall(r"\bconst\b[^,]*\*\s*__restrict__\s*(\w+)", params))
+            assert constant <= {"grad"}, (name, kernel, constant)
+    assert chained >= 7
