@@ -26,6 +26,7 @@ With ``shared_rows`` some attributes come from codebooks: a table of rows per at
 an integer code per Gaussian (``rows.table_lookup``).  The tables are trained in place of
 the attributes, sparse Adam updating the table rows that a visible Gaussian names.
 """
+import collections.abc
 import ctypes
 
 import torch
@@ -51,6 +52,37 @@ def plane_distances(K, volume_depth=4e-3, d_val=-2e-3):
     return torch.linspace(-volume_depth / 2.0, volume_depth / 2.0, K) + d_val
 
 
+class HeldTensors(collections.abc.Mapping):
+    """Tensors by attribute that stay where they are: the optimizer updates them and a captured
+    iteration reads them there.  Assigning one copies the values into place, so the next step
+    or replay uses them; its shape, type and device have to fit (int32 ones also take int64,
+    where a value that 32 bits do not hold becomes -1)."""
+
+    def __init__(self, tensors):
+        self._at = dict(tensors)
+
+    def __getitem__(self, key):
+        return self._at[key]
+
+    def __iter__(self):
+        return iter(self._at)
+
+    def __len__(self):
+        return len(self._at)
+
+    def __setitem__(self, key, new):
+        at = self._at[key]
+        wide = at.dtype == torch.int32 and getattr(new, "dtype", None) == torch.int64
+        if not isinstance(new, torch.Tensor) or (new.dtype != at.dtype and not wide):
+            raise TypeError(f"{key} must be a tensor of {at.dtype}, got {getattr(new, 'dtype', type(new).__name__)}")
+        if new.shape != at.shape or new.device != at.device:
+            raise ValueError(f"{key} must be {tuple(at.shape)} on {at.device}, got {tuple(new.shape)} on {new.device}")
+        if wide:
+            new = torch.where((new < 0) | (new >= 2 ** 31), -1, new)
+        with torch.no_grad():
+            at.copy_(new)
+
+
 class HoloTrainer:
     def __init__(self, N=300000, W=800, H=800, K=3, pitch=8e-6, lr=1e-3, eps=1e-15, seed=0, device="cuda",
                  camera=None, wavelengths=None, target=None, S=None, frustum=None, optimizer="sparse_adam",
@@ -58,8 +90,9 @@ class HoloTrainer:
         """`shared_rows`: {attribute: number of table rows} of the attributes that come from a
         codebook (2-D ones: pre_act_quats, pre_act_scales, colours, pre_act_phase,
         pre_act_plane_assignment).  `tables[attribute]` holds the rows (trained),
-        `codes[attribute]` each Gaussian's row (int32, seeded at random; assign your own).
-        One GPU, no densification."""
+        `codes[attribute]` each Gaussian's row (int32, seeded at random; assign your own: the
+        values are copied, before or after capture()).  A code outside the table gives an
+        attribute of zeros.  One GPU, no densification."""
         self.device = torch.device(device)
         self.W, self.H, self.K = W, H, K
         self.S = S or max(W, H)   # pad size (train.py: max(W, H) unless configured)
@@ -75,7 +108,7 @@ class HoloTrainer:
         if optimizer not in ("adan", "sparse_adam"):
             raise ValueError(f"unknown optimizer {optimizer!r}")
         self.optimizer, self.lr, self.eps = optimizer, lr, eps
-        self.tables, self.codes = {}, {}
+        tables, codes = {}, {}
         g = torch.Generator().manual_seed(seed + 1)
         for k, rows in (shared_rows or {}).items():
             if k == "means" or k not in self.params or self.params[k].dim() != 2:
@@ -85,8 +118,9 @@ class HoloTrainer:
             if type(self) is not HoloTrainer:
                 raise ValueError("shared_rows trains on one GPU (HoloTrainer)")
             # the first rows of the scene's own values; the Gaussians' own are dropped
-            self.tables[k] = self.params.pop(k).detach()[:rows].clone().requires_grad_(True)
-            self.codes[k] = torch.randint(0, rows, (N,), generator=g, dtype=torch.int32).to(self.device)
+            tables[k] = self.params.pop(k).detach()[:rows].clone().requires_grad_(True)
+            codes[k] = torch.randint(0, rows, (N,), generator=g, dtype=torch.int32).to(self.device)
+        self._tables, self._codes = HeldTensors(tables), HeldTensors(codes)
         self.opt = self._make_optimizer()
         if loss not in ("l2", "multiplane"):
             raise ValueError(f"unknown loss {loss!r}")
@@ -114,6 +148,16 @@ class HoloTrainer:
             g = torch.Generator().manual_seed(1)
             target = torch.rand(len(self.wavelengths), self.S, self.S, generator=g)
         self.target = target.to(self.device)
+
+    @property
+    def tables(self):
+        """The rows of each shared attribute; an assigned tensor is copied into place."""
+        return self._tables
+
+    @property
+    def codes(self):
+        """Each Gaussian's row of each shared attribute; an assigned tensor is copied into place."""
+        return self._codes
 
     def _make_optimizer(self):
         if self.optimizer == "adan":

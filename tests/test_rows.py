@@ -584,6 +584,60 @@ def test_trainer_with_shared_rows_captured(cuda):
         assert torch.equal(x, y), k
 
 
+def test_assigned_codes_and_tables_are_copied_into_place():
+    """A captured iteration reads the tensors it was captured with: assigning must fill those."""
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer
+    tr = HoloTrainer(shared_rows={"colours": 4, "pre_act_phase": 7}, N=20, W=16, H=16, K=2, device="cpu")
+    at, table = tr.codes["colours"], tr.tables["colours"]
+    for new in (torch.arange(20, dtype=torch.int32) % 4, torch.arange(20) % 3, at % 2,
+                torch.full((40,), 5, dtype=torch.int32)[::2]):
+        tr.codes["colours"] = new
+        assert tr.codes["colours"] is at and torch.equal(at, new.int())
+    tr.codes["colours"] %= 3
+    assert tr.codes["colours"] is at and bool((at == 2).all())
+    tr.codes["colours"] = torch.tensor([2 ** 32 + 1, -2 ** 40, 2 ** 31, 2 ** 31 - 1] * 5)   # no row in 64 bits either
+    assert at.tolist() == [-1, -1, -1, 2 ** 31 - 1] * 5
+    tr.tables["colours"] = torch.ones(4, 3)
+    assert tr.tables["colours"] is table and table.requires_grad and table.is_leaf and bool((table == 1).all())
+    assert any(p is table for _, p in tr._leaves())
+    for bad in (torch.zeros(19, dtype=torch.int32), torch.zeros(21, dtype=torch.int32),
+                torch.zeros(20, 1, dtype=torch.int32), torch.zeros((), dtype=torch.int32),
+                torch.zeros(20, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="colours must be"):
+            tr.codes["colours"] = bad
+    for bad in (torch.zeros(20), torch.zeros(20, dtype=torch.int16), torch.zeros(20, dtype=torch.bool), [0] * 20, 3):
+        with pytest.raises(TypeError, match="colours must be"):
+            tr.codes["colours"] = bad
+    for bad in (torch.ones(5, 3), torch.ones(4, 4), torch.ones(12)):
+        with pytest.raises(ValueError, match="colours must be"):
+            tr.tables["colours"] = bad
+    for held in (tr.codes, tr.tables):
+        with pytest.raises(KeyError):
+            held["pre_act_scales"] = torch.zeros(20, dtype=torch.int32)
+    with pytest.raises(AttributeError):
+        tr.codes = {"colours": at}
+    assert at.tolist() == [-1, -1, -1, 2 ** 31 - 1] * 5 and bool((table == 1).all())
+
+
+@gpu
+def test_codes_assigned_after_capture(cuda):
+    """Replays use codes and tables assigned after the capture, as eager steps do."""
+    a, b = shared_trainer(cuda), shared_trainer(cuda)
+    b.capture(warmup=2)                                       # three steps
+    for _ in range(3):
+        a.step()
+    for seed in (1, 2):
+        for tr in (a, b):
+            tr.codes["colours"] = integers(5000, 64, seed, 0, torch.int32 if seed == 1 else torch.int64)
+            tr.codes["pre_act_phase"] = integers(5000, 300, seed + 5)
+            tr.tables["colours"] = tr.tables["colours"].detach() * 0.5
+        fill = [torch.full((5000,), 10 ** 9, dtype=torch.int32, device=cuda) for _ in range(50)]   # memory let go
+        assert [float(a.step()) for _ in range(2)] == [float(b.replay()) for _ in range(2)]
+        del fill
+    for (k, x), (_, y) in zip(a._leaves(), b._leaves()):
+        assert torch.equal(x, y), k
+
+
 @gpu
 def test_trainer_with_shared_rows_and_adan(cuda):
     tr = shared_trainer(cuda, optimizer="adan")
