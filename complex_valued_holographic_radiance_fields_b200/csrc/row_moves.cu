@@ -843,7 +843,7 @@ int to_rows_backward(bool aligned, const void* grad, long long grad_stride, cons
 }
 
 int check_moves(int dtype, long long n, int choices, int width) {
-  if (!row_type_ok(dtype) || n < 0 || choices < 1 || width < 1) return CVHRF_EINVAL;
+  if (!row_type_ok(dtype) || n < 0 || choices < 1 || width < 1 || width > kMaxWidth) return CVHRF_EINVAL;
   if (n > kGroupMaxEntries / choices) return CVHRF_EUNSUPPORTED;
   return CVHRF_OK;
 }

@@ -874,7 +874,6 @@ int gradient(const void* grad, long long stride, int width, long long n, long lo
 }
 
 constexpr long long kMaxRows = 0x7ffffffe;
-constexpr int kMaxWidth = 1 << 20;
 
 }  // namespace
 }  // namespace cvhrf

@@ -212,6 +212,8 @@ constexpr int packs_of(int width) {
   return width / Row<T, L>::kVec;
 }
 
+constexpr int kMaxWidth = 1 << 20;   // elements of a row at most: columns are counted in int
+
 inline size_t row_type_bytes(int dtype) { return dtype == CVHRF_F32 ? 4 : 2; }
 inline bool row_type_ok(int dtype) { return dtype == CVHRF_F32 || dtype == CVHRF_BF16 || dtype == CVHRF_F16; }
 inline int next_pow2(int x) {

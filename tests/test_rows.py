@@ -880,3 +880,17 @@ def test_chained_kernels_read_their_inputs_plainly():
             constant = set(re.findall(r"\bconst\b[^,]*\*\s*__restrict__\s*(\w+)", params))
             assert constant <= {"grad"}, (name, kernel, constant)
     assert chained >= 7
+
+
+def test_c_abi_refuses_rows_that_are_too_wide():
+    """Columns are counted in int on the GPU: every entry point refuses more than 2^20 on the host."""
+    L = _lib.lib()
+    p = 256   # never read
+    for width in (2 ** 20 + 1, 2 ** 31 - 1):
+        for f in (L.cvhrf_rows_to_groups, L.cvhrf_groups_to_rows):
+            assert f(_lib.MOVES_ARGS.pack(p, p, p, p, p, 0, 5, width, 1, width, 0, 0), None) == 1
+        assert L.cvhrf_groups_to_rows_backward(_lib.MOVES_BACKWARD_ARGS.pack(
+            p, p, p, p, p, p, p, p, 5, width, width, 1, width, 0, 0), None) == 1
+        assert L.cvhrf_table_lookup(_lib.LOOKUP_ARGS.pack(p, p, p, 4, width, 2, width, 0, 4, 1.0), None) == 1
+        assert L.cvhrf_table_gradient(_lib.GRADIENT_ARGS.pack(p, p, p, 0, 0, 0, width, 9, 4, width, 0, 4, 1.0), None) == 1
+        assert L.cvhrf_table_gradient_workspace_bytes(9, 4, width) == 0
