@@ -248,7 +248,8 @@ class GroupsToRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, groups, weights):
         ctx.groups = groups
-        ctx.save_for_backward(y, weights)
+        # y is read for the weights' gradient alone: it may change or go where none is asked for
+        ctx.save_for_backward(y if ctx.needs_input_grad[2] else None, weights)
         return _to_rows(y, groups, weights)
 
     @staticmethod
@@ -257,14 +258,17 @@ class GroupsToRows(torch.autograd.Function):
         y, weights = ctx.saved_tensors
         groups = ctx.groups
         grad, code, width, grad_stride = _rows(grad, "grad")
-        y, _, _, stride = _rows(y, "y")
-        device = y.device
         need_y, _, need_w = ctx.needs_input_grad
-        grad_y = y.new_empty(y.shape) if need_y else None
+        y_at, stride = 0, 0
+        if need_w:
+            y, _, _, stride = _rows(y, "y")
+            y_at = y.data_ptr()
+        device = grad.device
+        grad_y = grad.new_empty((groups.num_rows * groups.choices, width)) if need_y else None
         grad_w = torch.empty_like(weights) if need_w else None
         w, w_code = (0, 0) if weights is None else (weights.data_ptr(), _TYPES[weights.dtype])
         _call("cvhrf_groups_to_rows_backward", "groups_to_rows_backward", device, _lib.MOVES_BACKWARD_ARGS.pack(
-            grad.data_ptr(), y.data_ptr(), groups.order.data_ptr(), groups.slots.data_ptr(), groups._used(), w,
+            grad.data_ptr(), y_at, groups.order.data_ptr(), groups.slots.data_ptr(), groups._used(), w,
             grad_y.data_ptr() if need_y else 0, grad_w.data_ptr() if need_w else 0, groups.num_rows, grad_stride,
             stride, groups.choices, width, code, w_code))
         return grad_y, None, grad_w

@@ -398,6 +398,35 @@ def test_gradients_only_of_what_is_asked(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("width", [1, 2, 12, 20, 33, 59, 64, 333, 1032, 2049, 4097, 9001])
+def test_rows_are_kept_for_the_weights_gradient_alone(cuda, dtype, width):
+    """y may be overwritten or let go after the forward pass unless the weights' gradient reads it."""
+    g = R.group_rows(integers(60, 5, 0, -1).reshape(30, 2), 4)
+    y0, up = normal((60, width), dtype, 1), normal((30, width), dtype, 2)
+    w = torch.rand(30, 2, device="cuda")
+    kept = g.slots >= 0
+    for weights in (None, w):
+        leaf = y0.clone().requires_grad_(True)
+        y = leaf * 1
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t.shape) or t, lambda t: t):
+            out = R.groups_to_rows(y, g, weights)
+        assert y.shape not in saved
+        y.detach().fill_(float("nan"))
+        y.mul_(2)                                            # would be refused if the backward pass needed y
+        exact = torch.zeros(60, width, dtype=torch.float64, device="cuda")
+        terms = (w.double() if weights is not None else torch.ones_like(w).double())[:, :, None] * up.double()[:, None]
+        exact[g.slots[kept].long()] = terms[kept]
+        close(torch.autograd.grad(out, leaf, up)[0], exact, U * exact.abs())
+    y, wl = y0.clone(), w.clone().requires_grad_(True)
+    out = R.groups_to_rows(y, g, wl)
+    y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, wl, up)
+
+
+@gpu
 def test_strided_moves(cuda):
     g = R.group_rows(integers(60, 4, 0).reshape(30, 2), 4)
     big, bigy = normal((30, 50), torch.float32, 1), normal((60, 100), torch.float32, 2)
