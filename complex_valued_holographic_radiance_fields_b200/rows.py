@@ -19,7 +19,8 @@ An index or group outside its range (-1, say) leaves the entry out: it looks up 
 nothing to a gradient or a sum, and whatever its weight or gradient holds is not read.
 Rows are float32, bfloat16 or float16, contiguous within a row (a slice of a wider tensor
 or a row expanded over a batch is used as it is); sums are float32 in a fixed order, so
-results repeat bit for bit, and are rounded once; gradients are not differentiable again.
+results repeat bit for bit, and are rounded once; gradients are not differentiable again, and
+forward-mode derivatives (dual tensors) are refused.
 Nothing is read back to the host: every call can be captured in a CUDA graph, a backward
 pass as torch captures any (no earlier autograd graph of the same leaves may be alive).
 Every step runs in libcvhrf (cvhrf_table_lookup, cvhrf_table_gradient, cvhrf_group_rows,
@@ -29,6 +30,7 @@ attributes, has no counterpart.
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, profiling
@@ -103,6 +105,11 @@ def _scale(scale):
     return scale
 
 
+# A call goes through its autograd function where a tensor needs a gradient, and within a
+# forward-mode level (forward_ad._current_level >= 0), where a dual tensor does not show and the
+# function refuses it.  (The test is written out in each of them: as a function of its own it
+# cost a lookup 0.5 of 9 us.)
+
 # ---- shared rows ----------------------------------------------------------------------
 def _lookup(table, index, scale):
     table, code, width, stride = _rows(table, "table")
@@ -152,7 +159,7 @@ def table_lookup(table, index, scale=1.0):
     shape: (*index.shape, D) in the table's type, zeros where the index is outside [0, V).
     Differentiable in the table (a dense (V, D) gradient, see ``table_gradient``)."""
     scale = _scale(scale)
-    if table.requires_grad and torch.is_grad_enabled():
+    if (table.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         return TableLookup.apply(table, index, scale)
     return _lookup(table, index, scale)
 
@@ -162,7 +169,8 @@ def table_gradient(grad, index, num_rows, scale=1.0):
     scale times the sum of grad[t] over the entries with index[t] = v.  grad has the
     lookup's shape (*index.shape, D).  Returns (gradient (num_rows, D) in grad's type,
     row_mask (num_rows,) uint8: 1 where an entry names the row), so that
-    ``SparseGaussianAdam.step(row_mask=row_mask)`` updates the rows that were used."""
+    ``SparseGaussianAdam.step(row_mask=row_mask)`` updates the rows that were used.  Not
+    differentiable: grad is taken as detached."""
     if grad.shape[:-1] != index.shape or not grad.shape:
         raise ValueError(f"grad must have the shape {tuple(index.shape)} and a row's width, got {tuple(grad.shape)}")
     if not 0 <= num_rows < 2 ** 31 - 1:
@@ -285,7 +293,7 @@ def rows_to_groups(x, groups):
     """Rows x (N, D) at their places: (N * k, D), row p the row of entry groups.order[p]; the
     places behind the last group are zeros.  Differentiable in x (the sum over its places)."""
     _check_groups(x, groups, groups.num_rows, "x")
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         return RowsToGroups.apply(x, groups)
     return _to_groups(x, groups)
 
@@ -303,6 +311,7 @@ def groups_to_rows(y, groups, weights=None):
         if weights.dtype not in (torch.float32, y.dtype):
             raise TypeError(f"weights must be float32 or {y.dtype}, got {weights.dtype}")
         weights = weights.contiguous()
-    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+    if (torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad))) or (
+            forward_ad._current_level >= 0):
         return GroupsToRows.apply(y, groups, weights)
     return _to_rows(y, groups, weights)

@@ -514,6 +514,29 @@ def test_no_second_derivative(cuda):
             first.sum().backward()
 
 
+@gpu
+def test_forward_mode_is_refused(cuda):
+    """A dual tensor needs no backward gradient; its tangent must not vanish without an error."""
+    from torch.autograd import forward_ad
+    g = R.group_rows(integers(12, 4, 0).reshape(6, 2), 4)
+    index = integers(7, 5, 3)
+    table, x, y, w = (normal(s, torch.float32, 1) for s in ((5, 3), (6, 3), (12, 3), (6, 2)))
+    calls = [(lambda t: R.table_lookup(t, index), table), (lambda t: R.rows_to_groups(t, g), x),
+             (lambda t: R.groups_to_rows(t, g), y), (lambda t: R.groups_to_rows(t, g, w), y),
+             (lambda t: R.groups_to_rows(y, g, t), w)]
+    for call, at in calls:
+        plain = call(at)
+        with forward_ad.dual_level():
+            for grads in (torch.enable_grad, torch.no_grad):
+                with grads(), pytest.raises(NotImplementedError, match="forward mode"):
+                    call(forward_ad.make_dual(at, torch.ones_like(at)))
+            inside = call(at)                                # no dual tensor: as outside
+            assert torch.equal(inside, plain) and not inside.requires_grad
+        leaf = at.clone().requires_grad_(True)
+        with forward_ad.dual_level():
+            assert torch.equal(call(leaf), plain) and call(leaf).requires_grad
+
+
 # ---- gradients against differences -------------------------------------------------------
 @gpu
 def test_gradients_against_differences(cuda):
