@@ -68,11 +68,17 @@ def all_reduce_sum(x, group=None):
     return _AllReduceSum.apply(x, group)
 
 
+def _refuse_shared_rows(trainer):
+    if getattr(trainer, "tables", None):
+        raise ValueError("shared_rows trains on one GPU: their gradients are not exchanged")
+
+
 def exchange_and_step(trainer, visible, group=None):
     """Sum the gradients and union the visible rows across ranks, then step the optimizer.
     Ranks that produced no gradients (nothing rendered) contribute zeros."""
     from . import _lib
     import ctypes
+    _refuse_shared_rows(trainer)
     n = trainer.params["means"].shape[0]
     dev = trainer.params["means"].device
     if any(p.grad is None for p in trainer.params.values()):
@@ -112,8 +118,7 @@ def dp_step(trainer, target=None, group=None):
     """
     from . import _lib
     import ctypes
-    if getattr(trainer, "tables", None):
-        raise ValueError("shared_rows trains on one GPU: their gradients are not exchanged")
+    _refuse_shared_rows(trainer)
     for p in trainer.params.values():
         p.grad = None
     loss, visible = trainer.forward(target)
@@ -140,6 +145,7 @@ def graph_exchange(group=None):
     """The exchange of `dp_step` as a callback for `HoloTrainer.capture(exchange=...)`:
     both all-reduces are recorded into the trainer's CUDA graph (NCCL supports capture)."""
     def exchange(trainer, row_mask):
+        _refuse_shared_rows(trainer)
         flat = _shared_flat_buffer(trainer.params)
         if flat is None:
             raise RuntimeError("graph capture needs the gradients in one flat buffer (render_inputs_fused)")

@@ -714,6 +714,18 @@ def test_trainer_refusals_of_shared_rows():
             call()
 
 
+def test_no_exchange_takes_shared_rows():
+    """Every exchange between GPUs steps the Gaussians' own parameters only: the tables would stay
+    behind without an error."""
+    from complex_valued_holographic_radiance_fields_b200 import distributed as D
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer
+    tr = HoloTrainer(shared_rows={"colours": 4}, N=20, W=16, H=16, K=2, device="cpu")
+    for call in (lambda: D.dp_step(tr), lambda: D.exchange_and_step(tr, torch.arange(3)),
+                 lambda: D.graph_exchange()(tr, torch.zeros(20, dtype=torch.uint8))):
+        with pytest.raises(ValueError, match="shared_rows"):
+            call()
+
+
 # ---- streams, graphs, devices ------------------------------------------------------------
 @gpu
 def test_captured_and_replayed(cuda):
