@@ -252,7 +252,12 @@ CHECKPOINT_KEYS = ("pre_act_quats", "means", "pre_act_scales", "colours", "pre_a
 
 def save_gaussians(params, path):
     """The reference's Gaussian checkpoint: torch.save of a dict of the seven pre-activation
-    parameter tensors, moved to the CPU (model.py:610-624; same keys, same layout)."""
+    parameter tensors, moved to the CPU (model.py:610-624; same keys, same layout).  The format
+    has a row per Gaussian: of a trainer with shared rows it takes ``scene_params()``, which
+    looks them up; its tables and codes are saved by ``torch.save`` beside it."""
+    missing = [k for k in CHECKPOINT_KEYS if k not in params]
+    if missing:
+        raise KeyError(f"params lack {missing} (a trainer with shared_rows has all of them in scene_params())")
     torch.save({k: params[k].detach().cpu() for k in CHECKPOINT_KEYS}, path)
 
 

@@ -92,7 +92,9 @@ class HoloTrainer:
         pre_act_plane_assignment).  `tables[attribute]` holds the rows (trained),
         `codes[attribute]` each Gaussian's row (int32, seeded at random; assign your own: the
         values are copied, before or after capture()).  A code outside the table gives an
-        attribute of zeros.  One GPU, no densification."""
+        attribute of zeros.  `save_gaussians(scene_params(), path)` writes the rows looked up;
+        tables and codes are kept by saving them, and assigned to a new trainer.  One GPU, no
+        densification."""
         self.device = torch.device(device)
         self.W, self.H, self.K = W, H, K
         self.S = S or max(W, H)   # pad size (train.py: max(W, H) unless configured)

@@ -714,6 +714,35 @@ def test_trainer_refusals_of_shared_rows():
             call()
 
 
+def test_checkpoint_of_shared_rows_is_refused_in_words(tmp_path):
+    from complex_valued_holographic_radiance_fields_b200 import scene as SC
+    from complex_valued_holographic_radiance_fields_b200.train_step import HoloTrainer
+    tr = HoloTrainer(shared_rows={"colours": 4}, N=20, W=16, H=16, K=2, device="cpu")
+    with pytest.raises(KeyError, match="colours.*scene_params"):
+        SC.save_gaussians(tr.params, tmp_path / "g.pth")
+    assert not (tmp_path / "g.pth").exists()
+
+
+@gpu
+def test_shared_rows_saved_and_assigned_to_another_trainer(cuda, tmp_path):
+    from complex_valued_holographic_radiance_fields_b200 import scene as SC
+    a, b = shared_trainer(cuda), shared_trainer(cuda)
+    for _ in range(2):
+        a.step()
+    SC.save_gaussians(a.scene_params(), tmp_path / "g.pth")
+    whole = SC.load_gaussians(tmp_path / "g.pth", device=cuda)
+    torch.save({"tables": dict(a.tables), "codes": dict(a.codes)}, tmp_path / "shared.pth")
+    shared = torch.load(tmp_path / "shared.pth", map_location=cuda)
+    for k in SHARED:
+        b.codes[k], b.tables[k] = shared["codes"][k], shared["tables"][k]
+    with torch.no_grad():
+        for k, p in b.params.items():
+            p.copy_(whole[k])
+    for k, v in b.scene_params().items():
+        assert torch.equal(v, a.scene_params()[k]) and torch.equal(v, whole[k])
+    assert torch.equal(a.forward()[0], b.forward()[0])
+
+
 def test_no_exchange_takes_shared_rows():
     """Every exchange between GPUs steps the Gaussians' own parameters only: the tables would stay
     behind without an error."""
