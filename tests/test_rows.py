@@ -255,6 +255,45 @@ def test_offsets_beyond_32_bits(cuda):
     assert torch.equal(R.groups_to_rows(xs, groups)[-3:], xs[groups.slots[-3:].long()])
 
 
+@gpu
+@pytest.mark.parametrize("dtype,width,n", [(torch.bfloat16, 2048, 1050000),     # aligned rows
+                                           (torch.bfloat16, 2047, 1050000),     # tiles
+                                           (torch.bfloat16, 4097, 525000),      # words and spans
+                                           (torch.float16, 15, 144000000)])     # flat
+def test_every_layout_beyond_32_bits(cuda, dtype, width, n):
+    """Inputs, outputs and gradients of more than 2^31 elements, checked at their ends and at the border."""
+    border = 2 ** 31 // width
+    assert 4 < border < n - 4
+    some = torch.tensor([0, 1, border - 1, border, border + 1, n - 2, n - 1], device="cuda")
+    x = torch.zeros(n, width, dtype=dtype, device="cuda")
+    x[some] = normal((7, width), dtype, 0)
+    index = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert torch.equal(R.table_lookup(x, some), x[some])
+    assert torch.equal(R.table_lookup(x, index)[some], x[some])
+    got, mask = R.table_gradient(x, n - 1 - index, n)
+    assert torch.equal(got[n - 1 - some], x[some]) and int(mask.sum()) == n
+    assert int(torch.count_nonzero(got)) == int(torch.count_nonzero(x))
+    del got, mask
+
+    g = R.group_rows(index % 3, 3)
+    at = g.slots[some].long()
+    assert torch.equal(g.order[at].long(), some)
+    leaf = x.requires_grad_(True)
+    xs = R.rows_to_groups(leaf, g)
+    assert torch.equal(xs[at], x[some]) and torch.equal(xs[some], x[g.order[some].long()])
+    dx, = torch.autograd.grad(xs, leaf, xs.detach())
+    assert torch.equal(dx[some], x[some])
+    del dx
+    y, w = xs.detach().requires_grad_(True), torch.rand(n, device="cuda").requires_grad_(True)
+    out = R.groups_to_rows(y, g, w)
+    exact = w.detach()[some, None].double() * x.detach()[some].double()
+    close(out.detach()[some], exact, U * exact.abs())
+    dy, dw = torch.autograd.grad(out, (y, w), x.detach())
+    close(dy[at], exact, U * exact.abs())
+    terms = x.detach()[some].double().square()
+    close(dw[some], terms.sum(1), width * U * terms.sum(1))
+
+
 # ---- rows by group --------------------------------------------------------------------
 def places_64(index, groups):
     """(order, slots, offsets) by a stable sort on the host."""
