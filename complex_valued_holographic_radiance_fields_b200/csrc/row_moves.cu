@@ -195,7 +195,9 @@ __device__ __forceinline__ void load_choices(const Moves& m, const Weights& weig
     }
 }
 
-// An owner has one pack of CHOICES choices of each of ROWS rows in flight.
+// An owner has one pack of CHOICES choices of each of ROWS rows in flight.  Five blocks per SM leave
+// 48 registers, which the 16-bit forms of two rows and of four choices, and spans of two, spill 48 to
+// 92 bytes of: 97656 aligned rows of 1024 f16 from one choice take 84 us, the same bytes as floats 71.
 template <typename T, Layout L, int ROWS, int CHOICES>
 __global__ void __launch_bounds__(kThreads, 5) groups_to_rows_kernel(Moves m, const T* __restrict__ y, Extent extent,
                                                                      long long stride, Weights weights,
@@ -470,8 +472,9 @@ __global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_tile_ker
 
 // The same for narrow rows, flat; the products of a place's dot product go through shared memory
 // to one thread, which adds them up in order.  (4M rows of 12 f16: 162 us, 545 by an element per
-// lane and row; 3M of 33: 230, 289 by warps; 1.7M of 59: 225 and 190.  4M rows of 2 floats: 62 and
-// 69, of 1: 59 and 34.)
+// lane and row; 3M of 33: 230, 289 by warps; 1.7M of 59: 225 and 190.  From 3 elements on: 4M rows
+// of 3 floats 90 and 117, of 2: 78 and 74, of 1: 72 and 45; 1M rows of 4 choices of 3 floats 74 and
+// 82, of 2: 70 and 57; 4M of 3 bf16 102 and 100, of 2: 96 and 66.)
 constexpr int kFlatGradWidth = 40;
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads) groups_to_rows_backward_flat_kernel(
